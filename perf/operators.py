@@ -411,8 +411,7 @@ def _run_own(s):
         return q6moe.paged_tree_attention(s["q"], s["k"], s["k_scales"], s["v"], s["v_scales"], s["table"],
                                           s["lengths"], s["starts"], s["masks"], page_size=s["page"],
                                           kv_heads=s["kv_heads"], max_count=s["most"], out=s["out"])
-    pools = list(zip(s["codes"].flatten(0, 1), s["scales"].flatten(0, 1)))
-    q6moe.keep_accepted(pools, s["table"], s["lengths"], s["path"], s["accepted"], page_size=s["page"])
+    q6moe.keep_accepted([(s["codes"], s["scales"])], s["table"], s["lengths"], s["path"], s["accepted"], page_size=s["page"])
     return dict(codes=s["codes"], scales=s["scales"])
 
 
