@@ -259,6 +259,34 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvQuant q, KvWrite w, int
   }
 }
 
+// Rows of a ragged batch into their slots, K (blockIdx.y 0) and V (1) in one launch.
+struct KvRows {
+  const void* x[2];
+  int64_t stride[2];  // values between rows
+  int8_t* codes[2];
+  void* scales[2];
+  const int64_t* slots;
+  int64_t rows, pool_rows;
+};
+
+template <bool kVec>
+__global__ void __launch_bounds__(256) kv_write_rows_kernel(KvQuant q, KvRows w) {
+  const int n = blockIdx.y;
+  q.x = w.x[n];
+  const int64_t th = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int l = (int)(th & ((1 << q.lg) - 1));
+  for (int64_t i = th >> q.lg; i < w.rows * q.groups; i += ((int64_t)gridDim.x * blockDim.x) >> q.lg) {  // (row, group)
+    const int64_t r = i / q.groups, g = i % q.groups;
+    const int64_t slot = w.slots[r], at = r * w.stride[n] + g * q.group;
+    KvGroup<kVec> x;
+    const float m = x.load(q, at, l);
+    if (slot < 0 || slot >= w.pool_rows) continue;
+    const float scale = kv_group_scale(q, m);
+    x.store(q, at, l, scale == 0.f ? 1.f : scale, w.codes[n] + slot * q.chans + g * q.group);
+    if (l == 0) kv_store_scale(w.scales[n], q.scale_bf16, slot * q.groups + g, scale);
+  }
+}
+
 // The lanes per group (log2) of a call and whether they take 8 consecutive
 // values each: groups of 8, 16, .., 512 values with x aligned for 16-byte
 // loads and codes for 8-byte stores. Other groups spread over the largest
@@ -369,6 +397,31 @@ extern "C" int q6moe_kv_write(const q6moe_kv_write_args* a, void* stream) {
   else
     hipLaunchKernelGGL(kv_write_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, q, w, a->batch);
   return check_launch("kv_write");
+}
+
+extern "C" int q6moe_kv_write_rows(const q6moe_kv_write_rows_args* a, void* stream) {
+  Q6MOE_REQUIRE(a, "kv_write_rows: null args");
+  Q6MOE_REQUIRE(a->key && a->value && a->k_codes && a->v_codes && a->k_scales && a->v_scales && a->slots,
+                "kv_write_rows: null pointer");
+  Q6MOE_REQUIRE(a->rows >= 1 && a->pool_rows >= 1 && a->kv_heads >= 1 && a->head_dim >= 1,
+                "kv_write_rows: rows, pool_rows, kv_heads and head_dim must be positive");
+  const int64_t chans = a->kv_heads * a->head_dim;
+  Q6MOE_REQUIRE(a->group >= 1 && chans % a->group == 0, "kv_write_rows: group must divide kv_heads*head_dim");
+  Q6MOE_REQUIRE(a->key_stride >= 0 && a->value_stride >= 0, "kv_write_rows: negative row stride");
+  Q6MOE_REQUIRE(a->x_dtype == Q6MOE_BF16 || a->x_dtype == Q6MOE_F32, "kv_write_rows: x dtype");
+  Q6MOE_REQUIRE(a->scale_dtype == Q6MOE_BF16 || a->scale_dtype == Q6MOE_F32, "kv_write_rows: scale dtype");
+  KvRows w{{a->key, a->value}, {a->key_stride, a->value_stride}, {a->k_codes, a->v_codes},
+           {a->k_scales, a->v_scales}, a->slots, a->rows, a->pool_rows};
+  KvQuant q{a->key, a->x_dtype == Q6MOE_BF16, chans, a->group, chans / a->group, a->scale_dtype == Q6MOE_BF16, 0};
+  bool vec = kv_quant_lanes(q, w.codes[0]);
+  const int64_t step = q.x_bf16 ? 8 : 4;  // values of a 16-byte load
+  if (!aligned(w.x[1], 16) || !aligned(w.codes[1], 8) || w.stride[0] % step || w.stride[1] % step) vec = false;
+  const dim3 grid((unsigned)std::min(cdiv((a->rows * q.groups) << q.lg, 256), kQuantGrid), 2);
+  if (vec)
+    hipLaunchKernelGGL(kv_write_rows_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, q, w);
+  else
+    hipLaunchKernelGGL(kv_write_rows_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, q, w);
+  return check_launch("kv_write_rows");
 }
 
 extern "C" int q6moe_kv_read(const q6moe_kv_args* a, void* stream) {

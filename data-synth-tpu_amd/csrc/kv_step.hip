@@ -1,0 +1,482 @@
+// The bookkeeping of a step that takes several new tokens per sequence over the
+// paged KV cache: pages and slots for the new tokens (q6moe_kv_plan), pages
+// given back (q6moe_kv_release), accepted tokens moved together (q6moe_kv_keep).
+// No counterpart in the reference, whose cache is dense and whose steps take one
+// token per sequence.
+//
+// A sequence b holds lengths[b] cached tokens; its new token j lies at position
+// lengths[b] + j, row starts[b] + j of the ragged batch, starts the running sum of
+// the counts. The free pages are a stack, taken from and given back at its end in
+// the order of (sequence, page index), so all results are deterministic.
+//
+// Latency-bound: a few kilobytes for a decode step. The dependent round trips are
+// what counts, so every sum over earlier sequences is formed by each workgroup for
+// itself, from one load per 256 sequences, instead of by a launch of its own.
+#include "q6moe_api.h"
+#include "q6moe_device.h"
+
+namespace q6moe {
+
+constexpr int kStepThreads = 256;
+constexpr int kStepWaves = kStepThreads / 64;
+constexpr int kMaxTree = 256;  // new tokens per sequence that masks tell apart
+constexpr int64_t kStepMaxBatch = 65535;
+
+// Sum of v over the workgroup, known to every thread.
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* lds) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off);
+  __syncthreads();  // lds may still be read
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  int64_t s = 0;
+#pragma unroll
+  for (int w = 0; w < kStepWaves; ++w) s += lds[w];
+  return s;
+}
+
+// Number of flagged threads before this one in the workgroup; *total: all of them.
+__device__ __forceinline__ int block_rank(bool flag, int64_t* lds, int* total) {
+  const uint64_t m = __ballot(flag);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = __popcll(m);
+  __syncthreads();
+  int before = __popcll(m & ((1ull << (threadIdx.x & 63)) - 1)), all = 0;
+#pragma unroll
+  for (int w = 0; w < kStepWaves; ++w) {
+    if (w < (int)(threadIdx.x >> 6)) before += (int)lds[w];
+    all += (int)lds[w];
+  }
+  *total = all;
+  return before;
+}
+
+struct PlanParams {
+  int32_t* table;
+  const int32_t* lengths;
+  const int32_t* counts;
+  const int32_t* free_pages;
+  int64_t free_capacity;
+  int32_t* free_count;
+  const int32_t* parents;
+  int64_t batch, pps, page, rows, max_count;  // max_count: most new tokens per sequence that are placed
+  int words;
+  int32_t* starts;
+  int64_t* slots;
+  int32_t* positions;
+  uint64_t* masks;
+  int32_t* missing;
+  int32_t* need;  // workspace: pages that sequence b needs; at [batch] the free pages before the call
+};
+
+__device__ __forceinline__ int64_t plan_len(const PlanParams& p, int64_t b) {
+  const int64_t n = p.lengths[b];
+  return n < 0 ? 0 : n;
+}
+__device__ __forceinline__ int64_t plan_asked(const PlanParams& p, int64_t b) {
+  const int64_t c = p.counts[b];
+  return c < 0 ? 0 : c;
+}
+__device__ __forceinline__ int64_t plan_count(const PlanParams& p, int64_t b) {
+  const int64_t c = plan_asked(p, b);
+  return c < p.max_count ? c : p.max_count;
+}
+// New tokens of sequence b that have rows, where ``before`` rows belong to earlier ones.
+__device__ __forceinline__ int64_t plan_fit(const PlanParams& p, int64_t count, int64_t before) {
+  const int64_t left = p.rows - before;
+  return left <= 0 ? 0 : (count < left ? count : left);
+}
+// Page indexes [first, end) that the new tokens of sequence b lie in.
+__device__ __forceinline__ void plan_pages(const PlanParams& p, int64_t len, int64_t count, int64_t* first,
+                                           int64_t* end) {
+  *first = len / p.page;
+  const int64_t e = (len + count + p.page - 1) / p.page;
+  *end = count == 0 ? *first : (e < p.pps ? e : p.pps);
+}
+// Rows of the sequences before b.
+__device__ __forceinline__ int64_t plan_before(const PlanParams& p, int64_t b, int64_t* lds) {
+  int64_t s = 0;
+  for (int64_t i = threadIdx.x; i < b; i += kStepThreads) s += plan_count(p, i);
+  return block_sum(s, lds);
+}
+
+// Pages that each sequence needs: its unmapped entries under the new tokens.
+__global__ void __launch_bounds__(kStepThreads) plan_need_kernel(PlanParams p) {
+  __shared__ int64_t lds[kStepWaves];
+  const int64_t b = blockIdx.x;
+  const int64_t before = plan_before(p, b, lds);
+  int64_t first, end;
+  plan_pages(p, plan_len(p, b), plan_fit(p, plan_count(p, b), before), &first, &end);
+  int64_t n = 0;
+  for (int64_t e = first + threadIdx.x; e < end; e += kStepThreads) n += p.table[b * p.pps + e] < 0;
+  n = block_sum(n, lds);
+  if (threadIdx.x == 0) {
+    p.need[b] = (int32_t)n;
+    if (b == 0) {
+      p.missing[0] = 0;
+      const int64_t have = p.free_count[0];
+      p.need[p.batch] = (int32_t)(have < 0 ? 0 : (have < p.free_capacity ? have : p.free_capacity));
+    }
+  }
+}
+
+// Slot of the token at position t of sequence b, -1 without a page.
+__device__ __forceinline__ int64_t plan_slot(const PlanParams& p, int64_t b, int64_t t) {
+  const int64_t e = t / p.page;
+  if (e >= p.pps) return -1;
+  const int64_t pg = p.table[b * p.pps + e];
+  return pg < 0 ? -1 : pg * p.page + (t - e * p.page);
+}
+
+// Takes sequence b's pages from the stack; with a tree also its rows (at most
+// kMaxTree of them, one per thread): the ancestors by pointer doubling in LDS,
+// each round adds those 1, 2, 4, ... levels further up.
+__global__ void __launch_bounds__(kStepThreads) plan_take_kernel(PlanParams p) {
+  __shared__ int64_t lds[kStepWaves];
+  const int64_t b = blockIdx.x;
+  int64_t rows = 0, need = 0;
+  for (int64_t i = threadIdx.x; i < b; i += kStepThreads) {
+    rows += plan_count(p, i);
+    need += p.need[i];
+  }
+  const int64_t before = block_sum(rows, lds);
+  int64_t rank = block_sum(need, lds);  // pages that earlier sequences need
+  const int64_t have = p.need[p.batch];
+  const int64_t len = plan_len(p, b), count = plan_fit(p, plan_count(p, b), before);
+  int64_t first, end;
+  plan_pages(p, len, count, &first, &end);
+  for (int64_t e0 = first; e0 < end; e0 += kStepThreads) {
+    const int64_t e = e0 + threadIdx.x;
+    const bool want = e < end && p.table[b * p.pps + e] < 0;
+    int all;
+    const int64_t at = rank + block_rank(want, lds, &all);
+    if (want && at < have) p.table[b * p.pps + e] = p.free_pages[have - 1 - at];
+    rank += all;
+  }
+  const int64_t start = before < p.rows ? before : p.rows;
+  if (threadIdx.x == 0) {
+    p.starts[b] = (int32_t)start;
+    if (b == p.batch - 1) {
+      p.starts[p.batch] = (int32_t)(start + count);
+      p.free_count[0] = (int32_t)(have - (rank < have ? rank : have));
+    }
+  }
+  const int64_t lost = plan_asked(p, b) - count;
+  if (threadIdx.x == 0 && lost) atomicAdd(p.missing, (int32_t)(lost < (1 << 30) ? lost : 1 << 30));
+  if (!p.parents) return;
+  __shared__ uint64_t sees[kMaxTree][kMaxTree / 64];
+  __shared__ int up[kMaxTree], depth[kMaxTree];
+  const int j = threadIdx.x;
+  __syncthreads();  // the table entries above
+  if (j < count) {
+    const int64_t parent = p.parents[start + j];
+    up[j] = parent >= 0 && parent < j ? (int)parent : -1;
+    depth[j] = up[j] >= 0;
+    for (int w = 0; w < p.words; ++w) sees[j][w] = w == j >> 6 ? 1ull << (j & 63) : 0;
+  }
+  for (int64_t reach = 1; reach < count; reach *= 2) {
+    __syncthreads();
+    uint64_t more[kMaxTree / 64] = {};
+    int to = -1, deeper = 0;
+    if (j < count && up[j] >= 0) {
+      const int u = up[j];
+#pragma unroll
+      for (int w = 0; w < kMaxTree / 64; ++w)
+        if (w < p.words) more[w] = sees[u][w];
+      to = up[u];
+      deeper = depth[u];
+    }
+    __syncthreads();
+    if (j < count) {
+#pragma unroll
+      for (int w = 0; w < kMaxTree / 64; ++w)
+        if (w < p.words) sees[j][w] |= more[w];
+      depth[j] += deeper;
+      up[j] = to;
+    }
+  }
+  if (j < count) {
+    const int64_t slot = plan_slot(p, b, len + j), row = start + j;
+    p.slots[row] = slot;
+    p.positions[row] = (int32_t)(len + depth[j]);
+    for (int w = 0; w < p.words; ++w) p.masks[row * p.words + w] = sees[j][w];
+    if (slot < 0) atomicAdd(p.missing, 1);
+  }
+}
+
+// Rows of the ragged batch: slots and positions of the sequences' tokens (of
+// trees they are written above), and the rows behind the last sequence.
+__global__ void __launch_bounds__(kStepThreads) plan_rows_kernel(PlanParams p) {
+  const int64_t row = (int64_t)blockIdx.x * kStepThreads + threadIdx.x;
+  if (row >= p.rows) return;
+  const int64_t used = p.starts[p.batch];
+  if (row >= used) {
+    p.slots[row] = -1;
+    p.positions[row] = 0;
+    if (p.masks)
+      for (int w = 0; w < p.words; ++w) p.masks[row * p.words + w] = 0;
+    return;
+  }
+  if (p.parents) return;
+  int64_t b = 0, hi = p.batch - 1;  // the last sequence with starts[b] <= row
+  while (b < hi) {
+    const int64_t mid = (b + hi + 1) / 2;
+    if (p.starts[mid] <= row)
+      b = mid;
+    else
+      hi = mid - 1;
+  }
+  const int64_t t = plan_len(p, b) + row - p.starts[b];
+  const int64_t slot = plan_slot(p, b, t);
+  p.slots[row] = slot;
+  p.positions[row] = (int32_t)t;
+  if (slot < 0) atomicAdd(p.missing, 1);
+}
+
+struct ReleaseParams {
+  int32_t* table;
+  const int32_t* lengths;
+  int32_t* free_pages;
+  int64_t free_capacity;
+  int32_t* free_count;
+  int64_t batch, pps, page;
+  int32_t* back;  // workspace: pages that sequence b gives back; at [batch] the free pages before the call
+};
+
+__device__ __forceinline__ int64_t release_first(const ReleaseParams& p, int64_t b) {
+  const int64_t n = p.lengths[b];
+  return n <= 0 ? 0 : (n + p.page - 1) / p.page;
+}
+
+__global__ void __launch_bounds__(kStepThreads) release_count_kernel(ReleaseParams p) {
+  __shared__ int64_t lds[kStepWaves];
+  const int64_t b = blockIdx.x;
+  int64_t n = 0;
+  for (int64_t e = release_first(p, b) + threadIdx.x; e < p.pps; e += kStepThreads)
+    n += p.table[b * p.pps + e] >= 0;
+  n = block_sum(n, lds);
+  if (threadIdx.x == 0) {
+    p.back[b] = (int32_t)n;
+    if (b == 0) {
+      const int64_t have = p.free_count[0];
+      p.back[p.batch] = (int32_t)(have < 0 ? 0 : (have < p.free_capacity ? have : p.free_capacity));
+    }
+  }
+}
+
+// Page i of the ``total`` that go back lies at have + total - 1 - i, where taking
+// pages in the same order found it. Pages that the stack has no room for (the
+// first ones, then) stay mapped.
+__global__ void __launch_bounds__(kStepThreads) release_put_kernel(ReleaseParams p) {
+  __shared__ int64_t lds[kStepWaves];
+  const int64_t b = blockIdx.x;
+  int64_t mine = 0, all = 0;
+  for (int64_t i = threadIdx.x; i < p.batch; i += kStepThreads) {
+    const int64_t n = p.back[i];
+    mine += i < b ? n : 0;
+    all += n;
+  }
+  int64_t rank = block_sum(mine, lds);
+  const int64_t total = block_sum(all, lds);
+  const int64_t have = p.back[p.batch];
+  for (int64_t e0 = release_first(p, b); e0 < p.pps; e0 += kStepThreads) {
+    const int64_t e = e0 + threadIdx.x;
+    const int32_t pg = e < p.pps ? p.table[b * p.pps + e] : -1;
+    int n;
+    const int64_t at = have + total - 1 - (rank + block_rank(pg >= 0, lds, &n));
+    if (pg >= 0 && at < p.free_capacity) {
+      p.free_pages[at] = pg;
+      p.table[b * p.pps + e] = -1;
+    }
+    rank += n;
+  }
+  if (b == 0 && threadIdx.x == 0) {
+    const int64_t now = have + total;
+    p.free_count[0] = (int32_t)(now < p.free_capacity ? now : p.free_capacity);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Accepted tokens of a tree moved to the front of its places, in the caches of
+// all layers: row of position len + path[i] -> row of position len + i. A
+// workgroup takes one sequence, one pool and kKeepUnits units of its rows; every
+// thread holds what it moves in registers and all of a workgroup's reads come
+// before its writes, so a path may cross itself.
+// ---------------------------------------------------------------------------
+constexpr int kKeepPools = 128;  // pools per launch: their pointers are kernel arguments
+constexpr int kKeepUnits = 8;    // units (16, 4 or 1 bytes) of a row per workgroup
+constexpr int kKeepRows = 256;   // most accepted tokens of a sequence
+constexpr int kKeepTurns = kKeepRows * kKeepUnits / kStepThreads;
+
+struct KeepParams {
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* path;
+  const int32_t* accepted;
+  int64_t pps, page, pool_pages, most;
+  int64_t units;  // per row
+  void* pool[kKeepPools];
+};
+
+__device__ __forceinline__ int64_t keep_row(const KeepParams& p, int64_t b, int64_t t) {
+  if (t < 0 || t >= p.pps * p.page) return -1;
+  const int64_t pg = p.table[b * p.pps + t / p.page];
+  return pg < 0 || pg >= p.pool_pages ? -1 : pg * p.page + t % p.page;
+}
+
+template <typename Unit>
+__global__ void __launch_bounds__(kStepThreads) keep_kernel(KeepParams p) {
+  const int64_t b = blockIdx.y;
+  const int64_t asked = p.accepted[b];
+  const int n = (int)(asked < p.most ? asked : p.most);
+  if (n <= 0) return;
+  const int64_t u = (int64_t)blockIdx.x * kKeepUnits + threadIdx.x % kKeepUnits;
+  const int64_t len = p.lengths[b];
+  Unit* pool = reinterpret_cast<Unit*>(p.pool[blockIdx.z]);
+  Unit held[kKeepTurns];
+  int64_t to[kKeepTurns];
+#pragma unroll
+  for (int k = 0; k < kKeepTurns; ++k) {
+    const int i = k * (kStepThreads / kKeepUnits) + (int)threadIdx.x / kKeepUnits;
+    to[k] = -1;
+    if (i < n && u < p.units && len >= 0) {
+      const int64_t step = p.path[b * p.most + i];
+      const int64_t from = step < 0 ? -1 : keep_row(p, b, len + step);
+      to[k] = from < 0 || step == i ? -1 : keep_row(p, b, len + i);
+      if (to[k] >= 0) held[k] = pool[from * p.units + u];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kKeepTurns; ++k)
+    if (to[k] >= 0) pool[to[k] * p.units + u] = held[k];
+}
+
+template <typename Unit>
+static void keep_launch(KeepParams& p, int64_t bytes, int64_t batch, int pools, hipStream_t s) {
+  p.units = bytes / (int64_t)sizeof(Unit);
+  hipLaunchKernelGGL(keep_kernel<Unit>, dim3((unsigned)cdiv(p.units, kKeepUnits), (unsigned)batch, (unsigned)pools),
+                     dim3(kStepThreads), 0, s, p);
+}
+
+// Rows of ``bytes`` bytes in the pools at base[i] (every second pointer of the caller's list).
+static int keep_pools(KeepParams p, void* const* base, int64_t pools, int64_t bytes, int64_t batch, hipStream_t s) {
+  for (int64_t i0 = 0; i0 < pools; i0 += kKeepPools) {
+    const int n = (int)(pools - i0 < kKeepPools ? pools - i0 : kKeepPools);
+    int64_t a = bytes;
+    for (int i = 0; i < n; ++i) {
+      p.pool[i] = base[2 * (i0 + i)];
+      a |= (int64_t)reinterpret_cast<uintptr_t>(p.pool[i]);
+    }
+    if (a % 16 == 0)
+      keep_launch<u32x4>(p, bytes, batch, n, s);
+    else if (a % 4 == 0)
+      keep_launch<uint32_t>(p, bytes, batch, n, s);
+    else
+      keep_launch<uint8_t>(p, bytes, batch, n, s);
+    if (const int rc = check_launch("kv_keep")) return rc;
+  }
+  return Q6MOE_OK;
+}
+
+}  // namespace q6moe
+
+using namespace q6moe;
+
+extern "C" size_t q6moe_kv_plan_workspace_size(int64_t batch) { return batch < 1 ? 0 : (size_t)(batch + 1) * 4; }
+
+extern "C" int q6moe_kv_plan(const q6moe_kv_plan_args* a, void* stream) {
+  Q6MOE_REQUIRE(a, "kv_plan: null args");
+  Q6MOE_REQUIRE(a->page_table && a->lengths && a->counts && a->free_pages && a->free_count && a->starts && a->slots &&
+                    a->positions && a->missing && a->workspace,
+                "kv_plan: null pointer");
+  Q6MOE_REQUIRE(a->batch >= 1 && a->batch <= kStepMaxBatch && a->pages_per_seq >= 1 && a->page_size >= 1 &&
+                    a->free_capacity >= 1 && a->rows >= 1 && a->rows < (1ll << 31) && a->max_count >= 1,
+                "kv_plan: batch, pages_per_seq, page_size, free_capacity, rows and max_count must be positive "
+                "(batch at most 65535, rows below 2^31)");
+  Q6MOE_REQUIRE(a->pages_per_seq < (1ll << 31) && a->page_size < (1ll << 31) &&
+                    a->pages_per_seq * a->page_size < (1ll << 31) && a->free_capacity < (1ll << 31),
+                "kv_plan: a sequence's capacity and the free stack must be below 2^31");
+  if (a->parents) {
+    Q6MOE_REQUIRE(a->masks && a->max_count <= kMaxTree, "kv_plan: trees need masks and a max_count of at most 256");
+  } else {
+    Q6MOE_REQUIRE(!a->masks, "kv_plan: masks need parents");
+  }
+  if (a->workspace_bytes < q6moe_kv_plan_workspace_size(a->batch)) {
+    set_error("kv_plan: workspace too small (need " + std::to_string(q6moe_kv_plan_workspace_size(a->batch)) +
+              " bytes)");
+    return Q6MOE_ERR_INVALID;
+  }
+  PlanParams p;
+  p.table = a->page_table;
+  p.lengths = a->lengths;
+  p.counts = a->counts;
+  p.free_pages = a->free_pages;
+  p.free_capacity = a->free_capacity;
+  p.free_count = a->free_count;
+  p.parents = a->parents;
+  p.batch = a->batch;
+  p.pps = a->pages_per_seq;
+  p.page = a->page_size;
+  p.rows = a->rows;
+  p.max_count = a->max_count;
+  p.words = a->parents ? (int)cdiv(a->max_count, 64) : 0;
+  p.starts = a->starts;
+  p.slots = a->slots;
+  p.positions = a->positions;
+  p.masks = reinterpret_cast<uint64_t*>(a->masks);
+  p.missing = a->missing;
+  p.need = reinterpret_cast<int32_t*>(a->workspace);
+  hipStream_t s = (hipStream_t)stream;
+  hipLaunchKernelGGL(plan_need_kernel, dim3((unsigned)p.batch), dim3(kStepThreads), 0, s, p);
+  hipLaunchKernelGGL(plan_take_kernel, dim3((unsigned)p.batch), dim3(kStepThreads), 0, s, p);
+  hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)cdiv(p.rows, kStepThreads)), dim3(kStepThreads), 0, s, p);
+  return check_launch("kv_plan kernels");
+}
+
+extern "C" int q6moe_kv_release(int32_t* page_table, const int32_t* lengths, int32_t* free_pages,
+                                int64_t free_capacity, int32_t* free_count, int64_t batch, int64_t pages_per_seq,
+                                int64_t page_size, void* workspace, size_t workspace_bytes, void* stream) {
+  Q6MOE_REQUIRE(page_table && lengths && free_pages && free_count && workspace, "kv_release: null pointer");
+  Q6MOE_REQUIRE(batch >= 1 && batch <= kStepMaxBatch && pages_per_seq >= 1 && page_size >= 1 && free_capacity >= 1,
+                "kv_release: batch (at most 65535), pages_per_seq, page_size and free_capacity must be positive");
+  Q6MOE_REQUIRE(pages_per_seq < (1ll << 31) && page_size < (1ll << 31) && free_capacity < (1ll << 31),
+                "kv_release: sizes must be below 2^31");
+  if (workspace_bytes < q6moe_kv_plan_workspace_size(batch)) {
+    set_error("kv_release: workspace too small (need " + std::to_string(q6moe_kv_plan_workspace_size(batch)) +
+              " bytes)");
+    return Q6MOE_ERR_INVALID;
+  }
+  ReleaseParams p{page_table, lengths, free_pages, free_capacity, free_count, batch, pages_per_seq, page_size,
+                  reinterpret_cast<int32_t*>(workspace)};
+  hipStream_t s = (hipStream_t)stream;
+  hipLaunchKernelGGL(release_count_kernel, dim3((unsigned)batch), dim3(kStepThreads), 0, s, p);
+  hipLaunchKernelGGL(release_put_kernel, dim3((unsigned)batch), dim3(kStepThreads), 0, s, p);
+  return check_launch("kv_release kernels");
+}
+
+extern "C" int q6moe_kv_keep(const q6moe_kv_keep_args* a, void* stream) {
+  Q6MOE_REQUIRE(a, "kv_keep: null args");
+  Q6MOE_REQUIRE(a->pools && a->page_table && a->lengths && a->path && a->accepted, "kv_keep: null pointer");
+  Q6MOE_REQUIRE(a->count >= 1 && a->count <= (1 << 20) && a->batch >= 1 && a->batch <= kStepMaxBatch,
+                "kv_keep: count and batch (at most 65535) must be positive");
+  Q6MOE_REQUIRE(a->code_bytes >= 1 && a->scale_bytes >= 1 && a->code_bytes < (1 << 24) && a->scale_bytes < (1 << 24),
+                "kv_keep: row sizes must be positive and below 2^24 bytes");
+  Q6MOE_REQUIRE(a->pool_pages >= 1 && a->pages_per_seq >= 1 && a->page_size >= 1 && a->pool_pages < (1ll << 31) &&
+                    a->pages_per_seq < (1ll << 31) && a->page_size < (1ll << 31),
+                "kv_keep: pool_pages, pages_per_seq and page_size must be positive and below 2^31");
+  Q6MOE_REQUIRE(a->path_len >= 1 && a->path_len <= kKeepRows, "kv_keep: a path holds 1 to 256 tokens");
+  for (int64_t i = 0; i < 2 * a->count; ++i) Q6MOE_REQUIRE(a->pools[i], "kv_keep: null pool");
+  KeepParams p;
+  p.table = a->page_table;
+  p.lengths = a->lengths;
+  p.path = a->path;
+  p.accepted = a->accepted;
+  p.pps = a->pages_per_seq;
+  p.page = a->page_size;
+  p.pool_pages = a->pool_pages;
+  p.most = a->path_len;
+  hipStream_t s = (hipStream_t)stream;
+  if (const int rc = keep_pools(p, a->pools, a->count, a->code_bytes, a->batch, s)) return rc;
+  return keep_pools(p, a->pools + 1, a->count, a->scale_bytes, a->batch, s);
+}

@@ -13,6 +13,9 @@ operators of AhmadSaeedZaidi/data-synth-tpu:
 * ``quantize`` / ``write_quantized`` / ``gather_scale_plane`` /
   ``read_quantized`` (kaggle/qwen38_tpu/attention_cache.py), with the paged
   forms ``write_paged`` / ``read_paged`` and ``paged_decode_attention``
+* a step with several new tokens per sequence (prompt chunks, drafted trees):
+  ``plan_pages`` / ``release_pages``, ``write_tokens``, ``paged_tree_attention``
+  and ``keep_accepted`` (no counterpart in the reference)
 
 All device work runs in hand-written HIP kernels (libq6moe.so, gfx950).
 """
@@ -46,6 +49,10 @@ def __getattr__(name):
         from . import attention_cache
 
         return getattr(attention_cache, name)
+    if name in ("plan_pages", "release_pages", "write_tokens", "paged_tree_attention", "keep_accepted", "PagePlan"):
+        from . import step
+
+        return getattr(step, name)
     if name == "routes":
         from . import router
 

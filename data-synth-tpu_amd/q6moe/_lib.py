@@ -134,6 +134,98 @@ class KvWriteArgs(ctypes.Structure):
     ]
 
 
+class PlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("page_table", _vp),
+        ("lengths", _vp),
+        ("counts", _vp),
+        ("free_pages", _vp),
+        ("free_capacity", _i64),
+        ("free_count", _vp),
+        ("parents", _vp),
+        ("batch", _i64),
+        ("pages_per_seq", _i64),
+        ("page_size", _i64),
+        ("rows", _i64),
+        ("max_count", _i64),
+        ("starts", _vp),
+        ("slots", _vp),
+        ("positions", _vp),
+        ("masks", _vp),
+        ("missing", _vp),
+        ("workspace", _vp),
+        ("workspace_bytes", _size),
+    ]
+
+
+class KvWriteRowsArgs(ctypes.Structure):
+    _fields_ = [
+        ("key", _vp),
+        ("value", _vp),
+        ("key_stride", _i64),
+        ("value_stride", _i64),
+        ("x_dtype", _int),
+        ("k_codes", _vp),
+        ("v_codes", _vp),
+        ("k_scales", _vp),
+        ("v_scales", _vp),
+        ("scale_dtype", _int),
+        ("slots", _vp),
+        ("rows", _i64),
+        ("pool_rows", _i64),
+        ("kv_heads", _i64),
+        ("head_dim", _i64),
+        ("group", _i64),
+    ]
+
+
+class TreeAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp),
+        ("q_stride", _i64),
+        ("k_codes", _vp),
+        ("v_codes", _vp),
+        ("k_scales", _vp),
+        ("v_scales", _vp),
+        ("scale_dtype", _int),
+        ("page_table", _vp),
+        ("lengths", _vp),
+        ("starts", _vp),
+        ("masks", _vp),
+        ("mask_words", _i64),
+        ("batch", _i64),
+        ("rows", _i64),
+        ("max_count", _i64),
+        ("query_heads", _i64),
+        ("kv_heads", _i64),
+        ("head_dim", _i64),
+        ("pool_pages", _i64),
+        ("pages_per_seq", _i64),
+        ("page_size", _i64),
+        ("out", _vp),
+        ("workspace", _vp),
+        ("workspace_bytes", _size),
+    ]
+
+
+class KvKeepArgs(ctypes.Structure):
+    _fields_ = [
+        ("pools", ctypes.POINTER(_vp)),
+        ("count", _i64),
+        ("code_bytes", _i64),
+        ("scale_bytes", _i64),
+        ("page_table", _vp),
+        ("lengths", _vp),
+        ("path", _vp),
+        ("accepted", _vp),
+        ("batch", _i64),
+        ("path_len", _i64),
+        ("pool_pages", _i64),
+        ("pages_per_seq", _i64),
+        ("page_size", _i64),
+    ]
+
+
 # name -> (restype, argtypes); exactly the entry points of include/q6moe.h
 SIGNATURES = {
     "q6moe_version": (_int, []),
@@ -158,6 +250,13 @@ SIGNATURES = {
     "q6moe_attn_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64]),
     "q6moe_route_topk": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
     "q6moe_kv_decode_attention": (_int, [ctypes.POINTER(AttnArgs), _vp]),
+    "q6moe_kv_plan_workspace_size": (_size, [_i64]),
+    "q6moe_kv_plan": (_int, [ctypes.POINTER(PlanArgs), _vp]),
+    "q6moe_kv_release": (_int, [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _size, _vp]),
+    "q6moe_kv_write_rows": (_int, [ctypes.POINTER(KvWriteRowsArgs), _vp]),
+    "q6moe_tree_attn_workspace_size": (_size, [_i64] * 8),
+    "q6moe_kv_tree_attention": (_int, [ctypes.POINTER(TreeAttnArgs), _vp]),
+    "q6moe_kv_keep": (_int, [ctypes.POINTER(KvKeepArgs), _vp]),
 }
 
 _lib = None

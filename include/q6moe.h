@@ -360,6 +360,142 @@ size_t q6moe_attn_workspace_size(int64_t batch, int64_t query_heads, int64_t kv_
                                  int64_t page_size);
 int q6moe_kv_decode_attention(const q6moe_attn_args* args, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* A step with several new tokens per sequence over the paged INT8 cache:    */
+/* chunks of prompts, or trees of drafted tokens. No counterpart in the      */
+/* reference (its steps take one token per sequence).                        */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Common terms. Sequence b holds lengths[b] cached tokens (below 0 counts as 0). Its new
+ * tokens are rows starts[b] .. starts[b+1]-1 of a ragged batch of ``rows`` rows; new token
+ * j lies at position lengths[b] + j, pool row page_table[b, pos / page_size] * page_size +
+ * pos % page_size. Page-table entries below 0 are unmapped. Rows from starts[batch] on
+ * belong to no sequence (a batch padded for a captured graph).
+ */
+
+/*
+ * Pages and slots for the new tokens. counts[b] new tokens are asked for per sequence (below
+ * 0 counts as 0, more than max_count as max_count); starts is their running sum, cut off at
+ * ``rows``. Every unmapped page-table entry under the new tokens takes a page from the free
+ * stack free_pages[0 .. *free_count), from its end, in the order of (sequence, page), and
+ * *free_count goes down: a second call with the same arguments changes nothing.
+ * Results per row: slots (pool row, -1 without a page or past the table's width, and for
+ * rows behind the last sequence), positions (lengths[b] + j, or lengths[b] + the token's
+ * depth in its tree; 0 behind the last sequence) and, with ``parents``, masks: bit jj % 64
+ * of word jj / 64 is set where new token jj is an ancestor of the row's token or itself.
+ * parents[row] is the index (within the sequence) of the new token that the row's token
+ * follows; -1, and anything that is no earlier token, means the last cached one.
+ * *missing counts the asked-for tokens that got no slot.
+ */
+typedef struct q6moe_kv_plan_args {
+  int32_t* page_table;       /* [batch, pages_per_seq], updated in place */
+  const int32_t* lengths;    /* [batch] */
+  const int32_t* counts;     /* [batch] */
+  const int32_t* free_pages; /* [free_capacity]; the first *free_count are free */
+  int64_t free_capacity;
+  int32_t* free_count;       /* [1], updated in place */
+  const int32_t* parents;    /* [rows] or NULL: each new token follows the one before it */
+  int64_t batch, pages_per_seq, page_size, rows;
+  int64_t max_count;         /* most new tokens per sequence; at most 256 with parents */
+  int32_t* starts;           /* [batch + 1] */
+  int64_t* slots;            /* [rows] */
+  int32_t* positions;        /* [rows] */
+  int64_t* masks;            /* [rows, ceil(max_count / 64)] with parents, else NULL */
+  int32_t* missing;          /* [1] */
+  void* workspace;           /* q6moe_kv_plan_workspace_size(batch) bytes, 4-byte aligned */
+  size_t workspace_bytes;
+} q6moe_kv_plan_args;
+
+size_t q6moe_kv_plan_workspace_size(int64_t batch);
+int q6moe_kv_plan(const q6moe_kv_plan_args* args, void* stream);
+
+/*
+ * Pages past the cached tokens go back: every mapped entry of page index ceil(lengths[b] /
+ * page_size) on is unmapped and pushed on the free stack, in the order that undoes
+ * q6moe_kv_plan. Pages that the stack has no room for stay mapped. A page that two entries
+ * name is pushed twice: pages that sequences share are not released by this call.
+ * Workspace as q6moe_kv_plan.
+ */
+int q6moe_kv_release(int32_t* page_table, const int32_t* lengths, int32_t* free_pages, int64_t free_capacity,
+                     int32_t* free_count, int64_t batch, int64_t pages_per_seq, int64_t page_size, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/*
+ * Keys and values of a ragged batch quantised into their slots (codes and scales as
+ * q6moe_kv_quantize), K and V in one call. Rows whose slot is outside [0, pool_rows) are
+ * not written. The slots that are written must be distinct.
+ */
+typedef struct q6moe_kv_write_rows_args {
+  const void* key;           /* [rows, KVH*D], row r at key + r * key_stride values */
+  const void* value;
+  int64_t key_stride, value_stride;
+  int x_dtype;               /* Q6MOE_BF16 or Q6MOE_F32 */
+  int8_t* k_codes;           /* [pool_rows, KVH*D] */
+  int8_t* v_codes;
+  void* k_scales;            /* [pool_rows, KVH*D / group] */
+  void* v_scales;
+  int scale_dtype;           /* Q6MOE_BF16 or Q6MOE_F32 */
+  const int64_t* slots;      /* [rows] */
+  int64_t rows, pool_rows, kv_heads, head_dim, group;
+} q6moe_kv_write_rows_args;
+
+int q6moe_kv_write_rows(const q6moe_kv_write_rows_args* args, void* stream);
+
+/*
+ * Attention of the new tokens over the cached tokens of their sequence and over each other,
+ * whose keys and values are in the cache already. Row i = starts[b] + j sees the tokens at
+ * positions below lengths[b], and new token jj of its sequence where bit jj of its mask is
+ * set (masks NULL: where jj <= j), as far as the page table reaches. With k = code * scale
+ * and v = code * scale (unrounded), out = RNE_bf16(softmax(q . k / sqrt(D)) . v); a row that
+ * sees nothing gives 0; unmapped pages read as zero codes with zero scales. Rows behind the
+ * last sequence, and of a sequence those from max_count on, are left as they were in out.
+ * head_dim 64, 128 or 256; one scale per token and KV head.
+ */
+typedef struct q6moe_tree_attn_args {
+  const uint16_t* q;         /* BF16 [rows, Hq, D], row r at q + r * q_stride */
+  int64_t q_stride;
+  const int8_t* k_codes;     /* [pool_pages, page_size, KVH*D] */
+  const int8_t* v_codes;
+  const void* k_scales;      /* [pool_pages*page_size, KVH] */
+  const void* v_scales;
+  int scale_dtype;           /* Q6MOE_BF16 or Q6MOE_F32 */
+  const int32_t* page_table; /* [batch, pages_per_seq]; entries outside [0, pool_pages) read as 0 */
+  const int32_t* lengths;    /* [batch] cached tokens, without the new ones */
+  const int32_t* starts;     /* [batch + 1] */
+  const int64_t* masks;      /* [rows, mask_words], or NULL */
+  int64_t mask_words;        /* >= ceil(max_count / 64), at most 4 */
+  int64_t batch, rows, max_count, query_heads, kv_heads, head_dim, pool_pages, pages_per_seq, page_size;
+  uint16_t* out;             /* BF16 [rows, Hq, D] */
+  void* workspace;           /* >= q6moe_tree_attn_workspace_size(...) bytes, 256-byte aligned */
+  size_t workspace_bytes;
+} q6moe_tree_attn_args;
+
+size_t q6moe_tree_attn_workspace_size(int64_t batch, int64_t rows, int64_t max_count, int64_t query_heads,
+                                      int64_t kv_heads, int64_t head_dim, int64_t pages_per_seq, int64_t page_size);
+int q6moe_kv_tree_attention(const q6moe_tree_attn_args* args, void* stream);
+
+/*
+ * The accepted tokens of each tree moved to the front of its places: for i < accepted[b] (at
+ * most path_len) the cached row of position lengths[b] + path[b, i] is copied to position
+ * lengths[b] + i, codes and scales, in every pool of the list (the K and V caches of all
+ * layers, which share the page table). All of a pool's rows are read before any is written.
+ * A row whose source or place is negative, past the table or unmapped is left out.
+ */
+typedef struct q6moe_kv_keep_args {
+  void* const* pools;        /* HOST array of 2 * count device pointers: codes, scales of each pool */
+  int64_t count;
+  int64_t code_bytes;        /* bytes per pool row of the codes */
+  int64_t scale_bytes;       /* and of the scales */
+  const int32_t* page_table; /* [batch, pages_per_seq] */
+  const int32_t* lengths;    /* [batch] cached tokens, without the new ones */
+  const int32_t* path;       /* [batch, path_len] */
+  const int32_t* accepted;   /* [batch] */
+  int64_t batch, path_len, pool_pages, pages_per_seq, page_size;
+} q6moe_kv_keep_args;
+
+int q6moe_kv_keep(const q6moe_kv_keep_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
