@@ -6,13 +6,26 @@
 //   p_t = exp(s_t - max s)
 //
 // with the INT8 codes kc, vc and the FP32 scales ks, vs of (token, KV head).
+#include <atomic>
+#include <type_traits>
+
 #include "q6moe_api.h"
 #include "q6moe_device.h"
 
+#define LDS_PTR(p) ((__attribute__((address_space(3))) void*)(uint32_t)(uintptr_t)(p))
+
 namespace q6moe {
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTreeThreads = 256;
 constexpr int kTreeMaxHeads = 65535;
+constexpr float kTreeFloor = -0x1p126f;  // running maximum before the first seen key
+constexpr float kTreeSlack = 8.f;        // a score may pass the running maximum by 2^8 before that is raised
 
 struct TreeParams {
   const uint16_t* q;
@@ -27,95 +40,635 @@ struct TreeParams {
   const int32_t* starts;
   const uint64_t* masks;
   int words;
-  int64_t batch, rows, max_count;
+  int batch, rows, max_count;
   int kvh, hq, r;
-  int64_t pool_pages, pps, page, cap;
+  int pool_pages, pps, page, cap;
+  uint32_t page_magic;  // t / page = t * page_magic >> page_shift for 0 <= t < 2^31
+  int page_shift;
+  int slots;       // workgroups that the work is split for
+  int whole;       // no split over keys
+  float to_log2;   // log2(e) / sqrt(D)
+  float* part;     // [workgroup][row of the tile][D] partial sums
+  float* stat;     // [workgroup][row of the tile][2]: maximum (log2) and sum
+  int32_t* info;   // [batch + 1]: first workgroup of each sequence; at [batch] the keys per workgroup
   uint16_t* out;
+};
+
+template <int D, int RW>
+struct TreeCfg {
+  static constexpr int kRows = 32 * RW;          // (new token, head of the group) rows per workgroup
+  static constexpr int kGroups = 4 / RW;         // waves that share rows take different keys
+  static constexpr int kTile = RW == 1 ? 32 : 64;  // keys per tile of a group
+  static constexpr int kBlocks = kTile / 32;
+  static constexpr int kStep = kTile * kGroups;  // keys per turn of the workgroup
+  static constexpr int kStages = D == 256 && RW < 4 ? 2 : 3;
+  static constexpr int kHalf = kTile * D;        // bytes of a tile's keys, and of its values
+  static constexpr int kDma = kHalf / 1024 / RW;  // DMA instructions per wave for each
+  static constexpr int kChunks = D / 16;         // 16-byte chunks of a key
+  static constexpr int kRing = kGroups * kStages * 2 * kHalf;
+  static constexpr int kScale = 2 * 64 * 4 + 16;  // per wave and stage: key and value scales, value factor
+  static constexpr int kLds = kRing + 4 * kStages * kScale + 32;  // and four words of masks
+  static_assert(kHalf % (1024 * RW) == 0 && kLds <= 160 * 1024, "tile");
 };
 
 __device__ __forceinline__ float tree_scale(const TreeParams& p, const void* s, int64_t i) {
   return p.scale_bf16 ? bf16_to_float(reinterpret_cast<const uint16_t*>(s)[i]) : reinterpret_cast<const float*>(s)[i];
 }
 
-// One workgroup per (row, query head): 256 keys at a time, one per thread for
-// the scores, then one channel per thread (and key group) for the sum of values.
-template <int D>
-__global__ void __launch_bounds__(kTreeThreads) tree_attn_simple_kernel(TreeParams p) {
-  __shared__ float qs[D], pr[kTreeThreads], red[kTreeThreads];
-  __shared__ int64_t at[kTreeThreads];
-  const int64_t row = blockIdx.x;
-  const int h = blockIdx.y, kh = h / p.r, t = threadIdx.x;
-  int64_t b = 0, hi = p.batch - 1;  // the last sequence with starts[b] <= row
+template <int N>
+__device__ __forceinline__ void tree_wait_vm() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+  asm volatile("" ::: "memory");
+}
+
+// What the rows of a sequence need: cached tokens, new tokens with rows, keys in reach.
+struct TreeSeq {
+  int start, count, len, n;
+};
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b) {
+  TreeSeq s;
+  const int a = p.starts[b], e = p.starts[b + 1], n = p.len[b];
+  s.start = a < 0 ? 0 : (a < p.rows ? a : p.rows);
+  const int end = e < p.rows ? e : p.rows;
+  int c = end - s.start;
+  c = c < 0 ? 0 : c;
+  s.count = c < p.max_count ? c : p.max_count;
+  s.len = n < 0 ? 0 : (n < p.cap ? n : p.cap);
+  s.n = s.len + s.count < p.cap ? s.len + s.count : p.cap;
+  return s;
+}
+__device__ __forceinline__ int tree_tiles(const TreeParams& p, const TreeSeq& s, int rows) {
+  return (s.count * p.r + rows - 1) / rows;
+}
+__device__ __forceinline__ int tree_chunks(int n, int keys) { return n <= keys ? 1 : (n + keys - 1) / keys; }
+// Keys that the rows of one tile reach, and those that all of them see.
+__device__ __forceinline__ void tree_reach(const TreeParams& p, const TreeSeq& s, int tile, int rows, int* n,
+                                           int* all) {
+  if (p.masks) {
+    *n = s.n;
+    *all = s.len;
+    return;
+  }
+  const int first = tile * rows / p.r, last = (tile * rows + rows - 1) / p.r;
+  const int to = s.len + (last < s.count ? last + 1 : s.count), seen = s.len + first + 1;
+  *n = to < p.cap ? to : p.cap;
+  *all = seen < p.cap ? seen : p.cap;
+}
+
+struct TreeItem {
+  int b, tile, kh, chunk, keys;
+};
+
+// The workgroup's item. The call's work, sum over sequences of tiles x heads x
+// keys, is cut into chunks of an equal number of keys, one per slot, so that
+// ragged lengths fill the chip evenly; every workgroup derives the same cut from
+// the lengths, which only the GPU knows. Thread t takes the sequences [t, t + 1) * per.
+template <int ROWS, int STEP>
+__device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
+  __shared__ int64_t sums[4];
+  __shared__ int item[5];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int per = (p.batch + kTreeThreads - 1) / kTreeThreads;
+  const int b0 = t * per, b1 = b0 + per < p.batch ? b0 + per : p.batch;
+  int64_t cost = 0;
+  TreeSeq s{0, 0, 0, 0};
+  for (int b = b0; b < b1; ++b) {
+    s = tree_seq(p, b);
+    cost += (int64_t)tree_tiles(p, s, ROWS) * p.kvh * s.n;
+  }
+  if (t == 0) item[0] = -1;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) cost += __shfl_xor(cost, off);
+  if (lane == 0) sums[wave] = cost;
+  __syncthreads();
+  const int64_t total = sums[0] + sums[1] + sums[2] + sums[3];
+  int64_t keys = (total + p.slots - 1) / p.slots;
+  keys = (keys + STEP - 1) / STEP * STEP;
+  if (keys < STEP) keys = STEP;
+  if (p.whole || keys > (1 << 30)) keys = 1 << 30;
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    if (per > 1) s = tree_seq(p, b);
+    mine += (int64_t)tree_tiles(p, s, ROWS) * p.kvh * tree_chunks(s.n, (int)keys);
+  }
+  int64_t upto = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t v = __shfl_up(upto, off);
+    if (lane >= off) upto += v;
+  }
+  __syncthreads();
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) upto += sums[w];
+  int64_t first = upto - mine;
+  const int64_t id = blockIdx.x;
+  if (id >= first && id < upto)
+    for (int b = b0; b < b1; ++b) {
+      if (per > 1) s = tree_seq(p, b);
+      const int tiles = tree_tiles(p, s, ROWS);
+      const int64_t n = (int64_t)tiles * p.kvh * tree_chunks(s.n, (int)keys);
+      if (id >= first && id < first + n) {
+        const int at = (int)(id - first);
+        item[0] = b;
+        item[1] = at % tiles;
+        item[2] = at / tiles % p.kvh;
+        item[3] = at / tiles / p.kvh;
+        item[4] = (int)keys;
+        if (at == 0) p.info[b] = (int32_t)id;
+      }
+      first += n;
+    }
+  if (id == 0 && t == 0) p.info[p.batch] = (int32_t)keys;
+  __syncthreads();
+  it.b = __builtin_amdgcn_readfirstlane(item[0]);
+  it.tile = __builtin_amdgcn_readfirstlane(item[1]);
+  it.kh = __builtin_amdgcn_readfirstlane(item[2]);
+  it.chunk = __builtin_amdgcn_readfirstlane(item[3]);
+  it.keys = __builtin_amdgcn_readfirstlane(item[4]);
+  return it.b >= 0;
+}
+
+// Chunk c of key t lies in slot c ^ tree_swizzle(t) of its row, so that the 16
+// lanes that read one column of 16 keys meet 16 different bank groups.
+template <int CH>
+__device__ __forceinline__ int tree_swizzle(int key) {
+  return (key / (16 / CH)) & (CH - 1);
+}
+
+template <int D, int RW>
+__global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(TreeParams p) {
+  using C = TreeCfg<D, RW>;
+  constexpr int KS = D / 32;  // channel blocks of 32
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  TreeItem it;
+  if (!tree_item<C::kRows, C::kStep>(p, it)) return;  // uniform over the workgroup
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = wave / RW, rw = wave % RW;
+  const int col = lane & 31, h = lane >> 5;
+  const TreeSeq seq = tree_seq(p, it.b);
+  int n, n_all;
+  tree_reach(p, seq, it.tile, C::kRows, &n, &n_all);
+  const int c0 = it.chunk * it.keys;
+  if (c0 > 0 && c0 >= n) return;
+  const int c1 = n - c0 < it.keys ? n : c0 + it.keys;
+  const bool split = tree_chunks(n, it.keys) > 1;
+
+  // The lane's row of the tile: query (new token j, head hh of the group), held
+  // as 16-bit integers in two INT8 operands q = (256 hi + lo) 2^(e-14), e the
+  // exponent of the row's largest value: exact for values down to 2^-6 of it.
+  const int row = it.tile * C::kRows + rw * 32 + col;
+  const bool live = row < seq.count * p.r;
+  const int j = live ? row / p.r : 0, hh = live ? row - j * p.r : 0;
+  i32x4 qhi[KS], qlo[KS];
+  float qf;
+  {
+    const uint16_t* src = p.q + (int64_t)(seq.start + j) * p.q_stride + (int64_t)(it.kh * p.r + hh) * D + 16 * h;
+    u32x4 raw[KS][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        raw[s][e] = live ? *reinterpret_cast<const u32x4*>(src + 32 * s + 8 * e) : u32x4{0u, 0u, 0u, 0u};
+    uint32_t top = 0;  // the largest magnitude's bits
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t x = raw[s][e][w];
+          const uint32_t a = x & 0x7fffu, b = (x >> 16) & 0x7fffu;
+          top = top > a ? top : a;
+          top = top > b ? top : b;
+        }
+    const uint32_t other = __shfl_xor(top, 32);
+    top = top > other ? top : other;
+    int e = (int)(top >> 7) - 127;
+    e = e < -110 ? -110 : e;  // smaller queries lose bits: scores below 2^-90
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t hi = 0, lo = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x = raw[s][w >> 1][(2 * w + (i >> 1)) & 3];
+          const float f = __builtin_bit_cast(float, i & 1 ? x & 0xffff0000u : x << 16);
+          int v = (int)__builtin_rintf(__builtin_ldexpf(f, 14 - e));
+          v = v > 32639 ? 32639 : v;  // 32640 would need hi = 128
+          const int vh = (v + 128) >> 8;
+          hi |= ((uint32_t)vh & 0xffu) << (8 * i);
+          lo |= ((uint32_t)(v - 256 * vh) & 0xffu) << (8 * i);
+        }
+        qhi[s][w] = (int)hi;
+        qlo[s][w] = (int)lo;
+      }
+    qf = __builtin_ldexpf(p.to_log2, e - 14);
+    if (top >= 0x7f80u) qf = __builtin_nanf("");  // an infinite or NaN query: NaN scores
+  }
+
+  // ---- the stream of key and value tiles --------------------------------
+  uint8_t* ring = smem + group * (C::kStages * 2 * C::kHalf);
+  float* scales = reinterpret_cast<float*>(smem + C::kRing + wave * (C::kStages * C::kScale));
+  const int turns = (c1 - c0 + C::kStep - 1) / C::kStep;
+  const int64_t row_bytes = (int64_t)p.kvh * D;
+  const int8_t* kbase = p.kc + (int64_t)it.kh * D;
+  const int8_t* vbase = p.vc + (int64_t)it.kh * D;
+  const int32_t* trow = p.table + (int64_t)it.b * p.pps;
+  const int tkey = lane & (C::kTile - 1);  // the key of a tile that this lane looks up
+  auto tile_at = [&](int i) { return c0 + (group + C::kGroups * i) * C::kTile; };
+  auto page_of = [&](int t) { return (int)((uint64_t)(uint32_t)t * p.page_magic >> p.page_shift); };
+  // New tokens that some row of the sequence sees. What the cache holds at the
+  // others' places (they may never have been written) is not read.
+  uint64_t* wanted = reinterpret_cast<uint64_t*>(smem + C::kRing + 4 * C::kStages * C::kScale);
+  if (p.masks && c1 > seq.len) {
+    if (wave == 0)
+      for (int w = 0; w < p.words; ++w) {
+        uint64_t some = 0;
+        for (int i = lane; i < seq.count; i += 64) some |= p.masks[(int64_t)(seq.start + i) * p.words + w];
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) some |= __shfl_xor((unsigned long long)some, off);
+        if (lane == 0) wanted[w] = some;
+      }
+    __syncthreads();
+  }
+  auto entry = [&](int i) {  // page-table entry of the lane's key in turn i's tile
+    const int t = tile_at(i) + tkey, jj = t - seq.len;
+    bool on = t < c1;
+    if (p.masks && on && jj >= 0) on = wanted[jj >> 6] >> (jj & 63) & 1;
+    return on ? trow[page_of(t)] : -1;
+  };
+  int pg = entry(0);
+  float rk = 0.f, rv = 0.f;  // scales on their way
+  auto issue = [&](int i, int stage) {
+    const int t = tile_at(i) + tkey;
+    const bool on = t < c1 && pg >= 0 && pg < p.pool_pages;
+    const int r = on ? pg * p.page + (t - page_of(t) * p.page) : -1;
+    pg = entry(i + 1);
+    if (C::kTile == 32) {  // lanes 0-31 load key scales, the others value scales
+      rk = r >= 0 ? tree_scale(p, h ? p.vs : p.ks, (int64_t)r * p.kvh + it.kh) : 0.f;
+    } else {
+      rk = r >= 0 ? tree_scale(p, p.ks, (int64_t)r * p.kvh + it.kh) : 0.f;
+      rv = r >= 0 ? tree_scale(p, p.vs, (int64_t)r * p.kvh + it.kh) : 0.f;
+    }
+    uint8_t* st = ring + stage * 2 * C::kHalf;
+#pragma unroll
+    for (int d = 0; d < C::kDma; ++d) {
+      const int at = (rw * C::kDma + d) * 64;  // first 16-byte slot
+      const int key = (at + lane) / C::kChunks, slot = (at + lane) % C::kChunks;
+      const int rr = __shfl(r, key);
+      const int64_t off = (int64_t)(rr < 0 ? 0 : rr) * row_bytes + 16 * (slot ^ tree_swizzle<C::kChunks>(key));
+      __builtin_amdgcn_global_load_lds(kbase + off, LDS_PTR(st + at * 16), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(vbase + off, LDS_PTR(st + C::kHalf + at * 16), 16, 0, 0);
+    }
+  };
+
+  f32x16 acc[KS];
+#pragma unroll
+  for (int c = 0; c < KS; ++c)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[c][v] = 0.f;
+  float m = kTreeFloor, l = 0.f, psum = 0.f;
+  float vfac = 1.f, vfac_new = 1.f, vtop = -1.f;  // value factor in use, of the newest tile, and its limit
+
+  // Scales of the tile issued a turn ago into the wave's LDS. The value scales are
+  // brought to at most 2^6 by a power of two that falls as larger ones are met, so
+  // that probability x scale keeps its 11 bits in FP16.
+  auto put_scales = [&](int stage) {
+    float* sc = scales + stage * (C::kScale / 4);
+    const float v = C::kTile == 32 ? (h ? rk : 0.f) : rv;
+    const float a = fabsf(v) < __builtin_inff() ? fabsf(v) : 0.f;
+    if (__any(a > vtop)) {
+      float x = a;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) x = fmaxf(x, __shfl_xor(x, off));
+      int e = (int)(__builtin_bit_cast(uint32_t, x) >> 23) - 127;
+      e = e < -110 ? -110 : e;
+      vfac_new = __builtin_bit_cast(float, (uint32_t)(127 + 3 - e) << 23);  // 2^(3-e): at most 2^4 now
+      vtop = __builtin_bit_cast(float, (uint32_t)(127 + e + 3 > 254 ? 254 : 127 + e + 3) << 23);
+    }
+    if (C::kTile == 32) {
+      sc[lane] = h ? v * vfac_new : rk;
+    } else {
+      sc[lane] = rk;
+      sc[64 + lane] = v * vfac_new;
+    }
+    if (lane == 0) sc[128] = vfac_new;
+  };
+
+  auto compute = [&](auto slow, int t0, int stage) {
+    const uint8_t* kt = ring + stage * 2 * C::kHalf;
+    const uint8_t* vt = kt + C::kHalf;
+    const float* sc = scales + stage * (C::kScale / 4);
+    float t[C::kBlocks][16];
+    float top = -__builtin_inff();
+    uint32_t vis[C::kBlocks];
+#pragma unroll
+    for (int nb = 0; nb < C::kBlocks; ++nb) {
+      const int key = 32 * nb + col, sw = tree_swizzle<C::kChunks>(key);
+      i32x16 hi, lo;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) hi[v] = lo[v] = 0;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const i32x4 a = *reinterpret_cast<const i32x4*>(kt + key * D + 16 * ((2 * s + h) ^ sw));
+        hi = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qhi[s], hi, 0, 0, 0);
+        lo = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qlo[s], lo, 0, 0, 0);
+      }
+      if constexpr (slow) {
+        // bit v: the lane's row sees key 8 (v / 4) + 4 h + v % 4 of the block
+        vis[nb] = 0;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int kk = t0 + 32 * nb + 8 * (v >> 2) + 4 * h + (v & 3), jj = kk - seq.len;
+          bool on = live && kk < c1;
+          if (on && jj >= 0)
+            on = p.masks ? (p.masks[(int64_t)(seq.start + j) * p.words + (jj >> 6)] >> (jj & 63)) & 1 : jj <= j;
+          vis[nb] |= on ? 1u << v : 0u;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 ksv = *reinterpret_cast<const f32x4*>(sc + 32 * nb + 8 * g + 4 * h);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int v = 4 * g + u;
+          t[nb][v] = (float)((hi[v] << 8) + lo[v]) * ksv[u];
+          if constexpr (slow) t[nb][v] = vis[nb] >> v & 1 ? t[nb][v] : -__builtin_inff();
+          top = fmaxf(top, t[nb][v]);
+        }
+      }
+    }
+    top *= qf;
+    if (__any(top > m + kTreeSlack)) {
+      const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+      const float fade = __builtin_amdgcn_exp2f(m - to);
+      m = to;
+      l *= fade;
+      psum *= fade;
+#pragma unroll
+      for (int c = 0; c < KS; ++c)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[c][v] *= fade;
+    }
+    const float vf = sc[128];
+    if (vf != vfac) {  // uniform over the wave
+      const float fade = vf / vfac;
+      vfac = vf;
+      psum *= fade;
+#pragma unroll
+      for (int c = 0; c < KS; ++c)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[c][v] *= fade;
+    }
+#pragma unroll
+    for (int nb = 0; nb < C::kBlocks; ++nb)
+#pragma unroll
+      for (int mm = 0; mm < 2; ++mm) {  // 16 keys: 8 of each half wave
+        f16x8 pv;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const f32x4 vsv =
+              *reinterpret_cast<const f32x4*>(sc + (C::kTile == 32 ? 32 : 64) + 32 * nb + 16 * mm + 8 * g + 4 * h);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int v = 8 * mm + 4 * g + u;
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(t[nb][v], qf, -m));
+            float w = e * vsv[u];
+            if constexpr (slow) {
+              const bool on = vis[nb] >> v & 1;
+              l += on ? e : 0.f;
+              w = on ? w : 0.f;
+            } else {
+              l += e;
+            }
+            pv[4 * g + u] = (_Float16)w;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const f16x2 one = {(_Float16)1.f, (_Float16)1.f}, pair = {pv[2 * u], pv[2 * u + 1]};
+          psum = __builtin_amdgcn_fdot2(pair, one, psum, false);
+        }
+        // values: 8 rows of 16 bytes per 16 lanes, read transposed: the lane gets the
+        // bytes of its channel at its half wave's 8 keys
+        const int i16 = lane & 15, jr = i16 >> 1;
+        const int key = 32 * nb + 16 * mm + 8 * (jr >> 2) + 4 * h + (jr & 3);
+        const int sw = tree_swizzle<C::kChunks>(key);
+#pragma unroll
+        for (int c = 0; c < KS; ++c) {
+          const uint8_t* src = vt + key * D + 16 * ((2 * c + ((lane >> 4) & 1)) ^ sw) + 8 * (i16 & 1);
+          const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (__attribute__((address_space(3))) i32x2*)(uint32_t)(uintptr_t)src);
+          // code + 128 as an FP16 subnormal, (code + 128) 2^-24: the shift by 128 is
+          // taken back at the end with the sum of the rounded probabilities
+          const uint32_t w0 = (uint32_t)w[0] ^ 0x80808080u, w1 = (uint32_t)w[1] ^ 0x80808080u;
+          u32x4 a;
+          a[0] = __builtin_amdgcn_perm(w0, w0, 0x0c010c00u);
+          a[1] = __builtin_amdgcn_perm(w0, w0, 0x0c030c02u);
+          a[2] = __builtin_amdgcn_perm(w1, w1, 0x0c010c00u);
+          a[3] = __builtin_amdgcn_perm(w1, w1, 0x0c030c02u);
+          acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), pv, acc[c], 0, 0, 0);
+        }
+      }
+  };
+
+  // Turn i issues the tile of turn i + kStages - 1; its scales reach LDS a turn
+  // later. Waits count DMA instructions: those of the tiles after this one may
+  // still be in flight.
+#pragma unroll
+  for (int i = 0; i < C::kStages - 1; ++i) {
+    if (i > 0) put_scales(i - 1);
+    issue(i, i);
+  }
+  int stage = 0;
+  for (int i = 0; i < turns; ++i) {
+    tree_wait_vm<(C::kStages - 2) * 2 * C::kDma>();
+    // the wave's reads of the stage that is written next have returned
+    if (RW > 1)
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const int newest = (stage + C::kStages - 2) % C::kStages, next = (stage + C::kStages - 1) % C::kStages;
+    put_scales(newest);
+    issue(i + C::kStages - 1, next);
+    const int t0 = tile_at(i);
+    if (t0 + C::kTile <= n_all && t0 + C::kTile <= c1)
+      compute(std::false_type{}, t0, stage);
+    else if (t0 < c1)
+      compute(std::true_type{}, t0, stage);
+    stage = stage + 1 == C::kStages ? 0 : stage + 1;
+  }
+  tree_wait_vm<0>();
+
+  // ---- the row's result -------------------------------------------------
+  // Both half waves hold half of a row's keys in l and psum.
+  l += __shfl_xor(l, 32);
+  psum += __shfl_xor(psum, 32);
+  const float up = 0x1p24f / vfac, shift = 128.f * psum * 0x1p-24f;
+#pragma unroll
+  for (int c = 0; c < KS; ++c)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[c][v] = (acc[c][v] - shift) * up;
+  if constexpr (C::kGroups > 1) {
+    // the groups' sums meet in LDS, in group order
+    __syncthreads();
+    float* st = reinterpret_cast<float*>(smem);                    // [group][row]: maximum, sum
+    float* sum = st + 2 * C::kGroups * C::kRows;                   // [row][D], one group at a time
+    const int rr = rw * 32 + col;
+    if (h == 0) {
+      st[2 * (group * C::kRows + rr)] = m;
+      st[2 * (group * C::kRows + rr) + 1] = l;
+    }
+    __syncthreads();
+    float to = kTreeFloor, all = 0.f;
+#pragma unroll
+    for (int g = 0; g < C::kGroups; ++g) to = fmaxf(to, st[2 * (g * C::kRows + rr)]);
+#pragma unroll
+    for (int g = 0; g < C::kGroups; ++g)
+      all += st[2 * (g * C::kRows + rr) + 1] * __builtin_amdgcn_exp2f(st[2 * (g * C::kRows + rr)] - to);
+    const float fade = __builtin_amdgcn_exp2f(m - to);
+#pragma unroll
+    for (int g = C::kGroups - 1; g >= 0; --g) {
+      if (group == g) {
+#pragma unroll
+        for (int c = 0; c < KS; ++c)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            f32x4* at = reinterpret_cast<f32x4*>(sum + rr * (D + 4) + 32 * c + 8 * q + 4 * h);
+            f32x4 v = {acc[c][4 * q] * fade, acc[c][4 * q + 1] * fade, acc[c][4 * q + 2] * fade,
+                       acc[c][4 * q + 3] * fade};
+            if (g < C::kGroups - 1) v += *at;
+            if (g > 0) {
+              *at = v;
+            } else {
+#pragma unroll
+              for (int u = 0; u < 4; ++u) acc[c][4 * q + u] = v[u];
+            }
+          }
+      }
+      __syncthreads();
+    }
+    if (group > 0) return;
+    m = to;
+    l = all;
+  }
+  if (!live) return;
+  if (split) {
+    const int64_t at = (int64_t)blockIdx.x * C::kRows + rw * 32 + col;
+    float* dst = p.part + at * D;
+#pragma unroll
+    for (int c = 0; c < KS; ++c)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(dst + 32 * c + 8 * q + 4 * h) =
+            f32x4{acc[c][4 * q], acc[c][4 * q + 1], acc[c][4 * q + 2], acc[c][4 * q + 3]};
+    if (h == 0) *reinterpret_cast<f32x2*>(p.stat + 2 * at) = f32x2{m, l};
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* dst = p.out + ((int64_t)(seq.start + j) * p.hq + it.kh * p.r + hh) * D;
+#pragma unroll
+  for (int c = 0; c < KS; ++c)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<u32x2*>(dst + 32 * c + 8 * q + 4 * h) =
+          u32x2{pack_bf16x2(acc[c][4 * q] * inv, acc[c][4 * q + 1] * inv),
+                pack_bf16x2(acc[c][4 * q + 2] * inv, acc[c][4 * q + 3] * inv)};
+}
+
+// The chunks' sums of a row joined in chunk order: four channels per thread.
+__global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p, int dim, int tile_rows) {
+  const int row = blockIdx.x;
+  const int at = (blockIdx.y * kTreeThreads + threadIdx.x) * 4;  // within the row's heads
+  int b = 0, hi = p.batch - 1;  // the last sequence with starts[b] <= row
   while (b < hi) {
-    const int64_t mid = (b + hi + 1) / 2;
+    const int mid = (b + hi + 1) / 2;
     if (p.starts[mid] <= row)
       b = mid;
     else
       hi = mid - 1;
   }
-  const int64_t j = row - p.starts[b];
-  if (j < 0 || row >= p.starts[b + 1] || j >= p.max_count) return;
-  int64_t count = p.starts[b + 1] - p.starts[b];
-  count = count < p.max_count ? count : p.max_count;
-  const int64_t len = p.len[b] < 0 ? 0 : p.len[b];
-  const int64_t seen = p.masks ? count : j + 1;
-  const int64_t n = len + seen < p.cap ? len + seen : p.cap;
-  if (t < D) qs[t] = bf16_to_float(p.q[row * p.q_stride + (int64_t)h * D + t]);
-  float m = -__builtin_inff(), l = 0.f, acc = 0.f;
-  constexpr int kParts = kTreeThreads / D;  // key groups of the value sum
-  const int c = t % D, part = t / D;
-  const float inv = 1.f / sqrtf((float)D);
-  for (int64_t t0 = 0; t0 < n; t0 += kTreeThreads) {
-    __syncthreads();
-    const int64_t key = t0 + t;
-    bool on = key < n;
-    if (on && key >= len && p.masks) {
-      const int64_t jj = key - len;
-      on = (p.masks[row * p.words + (jj >> 6)] >> (jj & 63)) & 1;
-    }
-    int64_t r = -1;
-    if (on) {
-      const int64_t pg = p.table[b * p.pps + key / p.page];
-      if (pg >= 0 && pg < p.pool_pages) r = pg * p.page + key % p.page;
-    }
-    float s = -__builtin_inff();
-    if (on) {
-      float dot = 0.f;
-      if (r >= 0) {
-        const int8_t* k = p.kc + (r * p.kvh + kh) * D;
-        for (int d = 0; d < D; ++d) dot += qs[d] * (float)k[d];
-        dot *= tree_scale(p, p.ks, r * p.kvh + kh);
-      }
-      s = dot * inv;
-    }
-    red[t] = s;
-    at[t] = r;
-    __syncthreads();
-    float top = m;
-    for (int i = 0; i < kTreeThreads; ++i) top = fmaxf(top, red[i]);
-    const float shift = top == -__builtin_inff() ? 0.f : top;
-    const float e = on ? expf(s - shift) : 0.f;
-    pr[t] = e;
-    __syncthreads();
-    const float fade = expf(m - shift);
-    l *= fade;
-    acc *= fade;
-    for (int i = 0; i < kTreeThreads; ++i) l += pr[i];
-    for (int i = part; i < kTreeThreads; i += kParts) {
-      const int64_t rr = at[i];
-      if (pr[i] != 0.f && rr >= 0)
-        acc += pr[i] * tree_scale(p, p.vs, rr * p.kvh + kh) * (float)p.vc[(rr * p.kvh + kh) * D + c];
-    }
-    m = top;
+  const TreeSeq s = tree_seq(p, b);
+  const int j = row - s.start;
+  if (j < 0 || j >= s.count || at >= p.hq * dim) return;
+  const int head = at / dim, c = at - head * dim, kh = head / p.r, rr = j * p.r + head - kh * p.r;
+  const int tile = rr / tile_rows, tiles = tree_tiles(p, s, tile_rows), keys = p.info[p.batch];
+  int n, n_all;
+  tree_reach(p, s, tile, tile_rows, &n, &n_all);
+  const int chunks = tree_chunks(n, keys);
+  if (chunks == 1) return;
+  const int64_t first = p.info[b] + (int64_t)kh * tiles + tile, step = (int64_t)p.kvh * tiles;
+  const int in = rr - tile * tile_rows;
+  float m = kTreeFloor;
+  for (int i = 0; i < chunks; ++i) m = fmaxf(m, p.stat[2 * ((first + i * step) * tile_rows + in)]);
+  float l = 0.f;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < chunks; ++i) {
+    const int64_t slot = (first + i * step) * tile_rows + in;
+    const f32x2 st = *reinterpret_cast<const f32x2*>(p.stat + 2 * slot);
+    const float f = __builtin_amdgcn_exp2f(st[0] - m);
+    l += st[1] * f;
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + slot * dim + c);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = __builtin_fmaf(x[u], f, v[u]);
   }
-  __syncthreads();
-  red[t] = acc;
-  __syncthreads();
-  if (t < D) {
-    float v = 0.f;
-    for (int i = 0; i < kParts; ++i) v += red[i * D + t];
-    p.out[(row * p.hq + h) * D + t] = bf16_bits(l == 0.f ? 0.f : v / l);
-  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<u32x2*>(p.out + (int64_t)row * p.hq * dim + at) =
+      u32x2{pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv)};
+}
+
+constexpr int kTreeCus = 256;
+
+struct TreeLayout {
+  int row_waves;  // waves of a workgroup with rows of their own
+  int slots, whole;
+  int64_t grid;   // at most so many workgroups have work
+  size_t info, stat, part, total;
+};
+
+static size_t tree_align(size_t v) { return (v + 255) & ~(size_t)255; }
+
+static TreeLayout tree_layout(int64_t batch, int64_t rows, int64_t max_count, int64_t hq, int64_t kvh, int64_t dim) {
+  TreeLayout L;
+  const int64_t r = hq / kvh;
+  L.row_waves = max_count * r <= 32 ? 1 : (max_count * r <= 64 ? 2 : 4);
+  const int64_t tile = 32 * L.row_waves;
+  // row tiles of all sequences together: each ends with one that is not full
+  const int64_t by_batch = batch * cdiv(max_count * r, tile), by_rows = rows * r / tile + batch;
+  const int64_t units = kvh * (by_batch < by_rows ? by_batch : by_rows);
+  L.slots = kTreeCus * (L.row_waves == 4 && dim < 256 ? 2 : 1);
+  L.whole = units >= 4 * L.slots;
+  L.grid = units + (L.whole ? 0 : L.slots);
+  const int64_t parts = L.whole ? 0 : L.grid * tile;
+  L.info = 0;
+  L.stat = tree_align(L.info + (size_t)(batch + 1) * 4);
+  L.part = tree_align(L.stat + (size_t)parts * 8);
+  L.total = tree_align(L.part + (size_t)parts * dim * 4);
+  return L;
+}
+
+template <int D, int RW>
+static int tree_launch(const TreeParams& p, const TreeLayout& L, hipStream_t s) {
+  using C = TreeCfg<D, RW>;
+  static std::atomic<uint64_t> done{0};
+  once_per_device(done, [] {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&tree_attn_kernel<D, RW>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
+  });
+  hipLaunchKernelGGL((tree_attn_kernel<D, RW>), dim3((unsigned)L.grid), dim3(kTreeThreads), C::kLds, s, p);
+  if (!L.whole)
+    hipLaunchKernelGGL(tree_combine_kernel, dim3((unsigned)p.rows, (unsigned)cdiv(p.hq * D, 4 * kTreeThreads)),
+                       dim3(kTreeThreads), 0, s, p, D, C::kRows);
+  return check_launch("tree_attention");
+}
+
+template <int D>
+static int tree_launch(const TreeParams& p, const TreeLayout& L, hipStream_t s) {
+  return L.row_waves == 1 ? tree_launch<D, 1>(p, L, s)
+                          : (L.row_waves == 2 ? tree_launch<D, 2>(p, L, s) : tree_launch<D, 4>(p, L, s));
 }
 
 }  // namespace q6moe
@@ -127,7 +680,8 @@ extern "C" size_t q6moe_tree_attn_workspace_size(int64_t batch, int64_t rows, in
                                                  int64_t page_size) {
   if (batch < 1 || rows < 1 || max_count < 1 || query_heads < 1 || kv_heads < 1 || pages_per_seq < 1 || page_size < 1)
     return 0;
-  return 256;
+  if (query_heads % kv_heads || batch > 65535 || rows >= (1 << 24) || max_count >= (1 << 24)) return 0;
+  return tree_layout(batch, rows, max_count, query_heads, kv_heads, head_dim).total;
 }
 
 extern "C" int q6moe_kv_tree_attention(const q6moe_tree_attn_args* a, void* stream) {
@@ -144,9 +698,9 @@ extern "C" int q6moe_kv_tree_attention(const q6moe_tree_attn_args* a, void* stre
                 "tree_attention: rows and max_count must be positive and below 2^24");
   Q6MOE_REQUIRE(a->page_size >= 1 && a->pages_per_seq >= 1 && a->pool_pages >= 1 && a->page_size < (1 << 30) &&
                     a->pages_per_seq < (1 << 30) && a->pool_pages < (1ll << 31) &&
-                    a->pages_per_seq * a->page_size <= (1 << 30),
+                    a->pages_per_seq * a->page_size <= (1 << 30) && a->pool_pages * a->page_size < (1ll << 31),
                 "tree_attention: page_size, pages_per_seq and pool_pages must be positive, a sequence's capacity at "
-                "most 2^30");
+                "most 2^30 and the pool below 2^31 tokens");
   Q6MOE_REQUIRE(a->scale_dtype == Q6MOE_BF16 || a->scale_dtype == Q6MOE_F32, "tree_attention: scale dtype");
   Q6MOE_REQUIRE(!a->masks || (a->mask_words >= 1 && a->mask_words <= 4 && a->max_count <= 64 * a->mask_words),
                 "tree_attention: masks hold max_count bits in at most 4 words");
@@ -154,10 +708,11 @@ extern "C" int q6moe_kv_tree_attention(const q6moe_tree_attn_args* a, void* stre
   Q6MOE_REQUIRE(aligned(a->q, 16) && aligned(a->k_codes, 16) && aligned(a->v_codes, 16) && aligned(a->out, 16) &&
                     aligned(a->workspace, 256),
                 "tree_attention: q, codes and out need 16-byte and workspace 256-byte alignment");
-  const size_t need = q6moe_tree_attn_workspace_size(a->batch, a->rows, a->max_count, a->query_heads, a->kv_heads,
-                                                     a->head_dim, a->pages_per_seq, a->page_size);
-  if (a->workspace_bytes < need) {
-    set_error("tree_attention: workspace too small (need " + std::to_string(need) + " bytes)");
+  const TreeLayout L =
+      tree_layout(a->batch, a->rows, a->max_count, a->query_heads, a->kv_heads, a->head_dim);
+  Q6MOE_REQUIRE(L.grid < (1ll << 31), "tree_attention: too many rows");
+  if (a->workspace_bytes < L.total) {
+    set_error("tree_attention: workspace too small (need " + std::to_string(L.total) + " bytes)");
     return Q6MOE_ERR_INVALID;
   }
   TreeParams p;
@@ -173,24 +728,29 @@ extern "C" int q6moe_kv_tree_attention(const q6moe_tree_attn_args* a, void* stre
   p.starts = a->starts;
   p.masks = reinterpret_cast<const uint64_t*>(a->masks);
   p.words = (int)a->mask_words;
-  p.batch = a->batch;
-  p.rows = a->rows;
-  p.max_count = a->max_count;
+  p.batch = (int)a->batch;
+  p.rows = (int)a->rows;
+  p.max_count = (int)a->max_count;
   p.kvh = (int)a->kv_heads;
   p.hq = (int)a->query_heads;
   p.r = p.hq / p.kvh;
-  p.pool_pages = a->pool_pages;
-  p.pps = a->pages_per_seq;
-  p.page = a->page_size;
-  p.cap = a->pages_per_seq * a->page_size;
+  p.pool_pages = (int)a->pool_pages;
+  p.pps = (int)a->pages_per_seq;
+  p.page = (int)a->page_size;
+  p.cap = (int)(a->pages_per_seq * a->page_size);
+  int lg = 0;
+  while ((1ll << lg) < a->page_size) ++lg;
+  p.page_magic = (uint32_t)(((1ull << (31 + lg)) + a->page_size - 1) / a->page_size);
+  p.page_shift = 31 + lg;
+  p.slots = L.slots;
+  p.whole = L.whole;
+  p.to_log2 = 1.4426950408889634f / sqrtf((float)a->head_dim);
+  uint8_t* w = reinterpret_cast<uint8_t*>(a->workspace);
+  p.info = reinterpret_cast<int32_t*>(w + L.info);
+  p.stat = reinterpret_cast<float*>(w + L.stat);
+  p.part = reinterpret_cast<float*>(w + L.part);
   p.out = a->out;
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)p.rows, (unsigned)p.hq);
-  if (a->head_dim == 64)
-    hipLaunchKernelGGL(tree_attn_simple_kernel<64>, grid, dim3(kTreeThreads), 0, s, p);
-  else if (a->head_dim == 128)
-    hipLaunchKernelGGL(tree_attn_simple_kernel<128>, grid, dim3(kTreeThreads), 0, s, p);
-  else
-    hipLaunchKernelGGL(tree_attn_simple_kernel<256>, grid, dim3(kTreeThreads), 0, s, p);
-  return check_launch("tree_attention");
+  return a->head_dim == 64 ? tree_launch<64>(p, L, s)
+                           : (a->head_dim == 128 ? tree_launch<128>(p, L, s) : tree_launch<256>(p, L, s));
 }

@@ -288,8 +288,9 @@ def test_attention_garbage_where_nothing_looks(device):
     k[~held], v[~held] = -128, -128
     got = _attn(device, case, sees)
     np.testing.assert_array_equal(got, want)
-    vs[~held], ks[~held] = np.nan, -np.inf
-    np.testing.assert_array_equal(_attn(device, case, sees), want)
+    for bad in ((np.nan, -np.inf), (3e38, 3e38), (-3e38, 1e-38)):
+        vs[~held], ks[~held] = bad
+        np.testing.assert_array_equal(_attn(device, case, sees), want)
 
 
 def test_attention_scales_far_apart(device):
