@@ -16,7 +16,6 @@
 
 namespace q6moe {
 
-typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -70,10 +69,6 @@ struct TreeCfg {
   static constexpr int kLds = kRing + 4 * kStages * kScale + 32;  // and four words of masks
   static_assert(kHalf % (1024 * RW) == 0 && kLds <= 160 * 1024, "tile");
 };
-
-__device__ __forceinline__ float tree_scale(const TreeParams& p, const void* s, int64_t i) {
-  return p.scale_bf16 ? bf16_to_float(reinterpret_cast<const uint16_t*>(s)[i]) : reinterpret_cast<const float*>(s)[i];
-}
 
 template <int N>
 __device__ __forceinline__ void tree_wait_vm() {
@@ -190,15 +185,28 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
   return it.b >= 0;
 }
 
-// Chunk c of key t lies in slot c ^ tree_swizzle(t) of its row, so that the 16
-// lanes that read one column of 16 keys meet 16 different bank groups.
+// A tile's rows in LDS: key t lies in row tree_row(t), bits 0 and 2 of t exchanged,
+// so that the two half waves, which read the values of keys 4 apart, meet
+// different halves of the banks. Chunk c of a row's key lies in slot c ^
+// tree_swizzle(row), so that the 16 lanes that read one column of 16 keys meet 16
+// different bank groups; values, read by rows, lie as they are.
+__device__ __forceinline__ int tree_row(int key) { return (key & ~5) | (key & 1) << 2 | (key >> 2 & 1); }
 template <int CH>
-__device__ __forceinline__ int tree_swizzle(int key) {
-  return (key / (16 / CH)) & (CH - 1);
+__device__ __forceinline__ int tree_swizzle(int row) {
+  return (row / (16 / CH)) & (CH - 1);
+}
+
+// The channel of accumulator element v (of channel block c), for a lane of half
+// wave h: each lane's loads of D / 32 consecutive channels of a key serve all
+// blocks (for D = 64, of 4 channels, of which the upper 16 rows take the last two).
+template <int D>
+__device__ __forceinline__ int tree_channel(int c, int v, int h) {
+  const int i = 8 * (v >> 2) + 4 * h + (v & 3);
+  return D == 64 ? 4 * (i & 15) + 2 * (i >> 4) + c : D / 32 * i + c;
 }
 
 template <int D, int RW>
-__global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(TreeParams p) {
+__global__ void __launch_bounds__(kTreeThreads, D == 256 ? 1 : 2) tree_attn_kernel(TreeParams p) {
   using C = TreeCfg<D, RW>;
   constexpr int KS = D / 32;  // channel blocks of 32
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -215,75 +223,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(TreeParams p
   const int c1 = n - c0 < it.keys ? n : c0 + it.keys;
   const bool split = tree_chunks(n, it.keys) > 1;
 
-  // The lane's row of the tile: query (new token j, head hh of the group), held
-  // as 16-bit integers in two INT8 operands q = (256 hi + lo) 2^(e-14), e the
-  // exponent of the row's largest value: exact for values down to 2^-6 of it.
-  const int row = it.tile * C::kRows + rw * 32 + col;
-  const bool live = row < seq.count * p.r;
-  const int j = live ? row / p.r : 0, hh = live ? row - j * p.r : 0;
-  i32x4 qhi[KS], qlo[KS];
-  float qf;
-  {
-    const uint16_t* src = p.q + (int64_t)(seq.start + j) * p.q_stride + (int64_t)(it.kh * p.r + hh) * D + 16 * h;
-    u32x4 raw[KS][2];
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        raw[s][e] = live ? *reinterpret_cast<const u32x4*>(src + 32 * s + 8 * e) : u32x4{0u, 0u, 0u, 0u};
-    uint32_t top = 0;  // the largest magnitude's bits
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t x = raw[s][e][w];
-          const uint32_t a = x & 0x7fffu, b = (x >> 16) & 0x7fffu;
-          top = top > a ? top : a;
-          top = top > b ? top : b;
-        }
-    const uint32_t other = __shfl_xor(top, 32);
-    top = top > other ? top : other;
-    int e = (int)(top >> 7) - 127;
-    e = e < -110 ? -110 : e;  // smaller queries lose bits: scores below 2^-90
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t hi = 0, lo = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t x = raw[s][w >> 1][(2 * w + (i >> 1)) & 3];
-          const float f = __builtin_bit_cast(float, i & 1 ? x & 0xffff0000u : x << 16);
-          int v = (int)__builtin_rintf(__builtin_ldexpf(f, 14 - e));
-          v = v > 32639 ? 32639 : v;  // 32640 would need hi = 128
-          const int vh = (v + 128) >> 8;
-          hi |= ((uint32_t)vh & 0xffu) << (8 * i);
-          lo |= ((uint32_t)(v - 256 * vh) & 0xffu) << (8 * i);
-        }
-        qhi[s][w] = (int)hi;
-        qlo[s][w] = (int)lo;
-      }
-    qf = __builtin_ldexpf(p.to_log2, e - 14);
-    if (top >= 0x7f80u) qf = __builtin_nanf("");  // an infinite or NaN query: NaN scores
-  }
-
-  // ---- the stream of key and value tiles --------------------------------
-  uint8_t* ring = smem + group * (C::kStages * 2 * C::kHalf);
-  float* scales = reinterpret_cast<float*>(smem + C::kRing + wave * (C::kStages * C::kScale));
-  const int turns = (c1 - c0 + C::kStep - 1) / C::kStep;
-  const int64_t row_bytes = (int64_t)p.kvh * D;
-  const int8_t* kbase = p.kc + (int64_t)it.kh * D;
-  const int8_t* vbase = p.vc + (int64_t)it.kh * D;
-  const int32_t* trow = p.table + (int64_t)it.b * p.pps;
-  const int tkey = lane & (C::kTile - 1);  // the key of a tile that this lane looks up
-  auto tile_at = [&](int i) { return c0 + (group + C::kGroups * i) * C::kTile; };
-  auto page_of = [&](int t) { return (int)((uint64_t)(uint32_t)t * p.page_magic >> p.page_shift); };
   // New tokens that some row of the sequence sees. What the cache holds at the
   // others' places (they may never have been written) is not read.
   uint64_t* wanted = reinterpret_cast<uint64_t*>(smem + C::kRing + 4 * C::kStages * C::kScale);
-  if (p.masks && c1 > seq.len) {
+  const bool pick = p.masks && c1 > seq.len;
+  if (pick) {
     if (wave == 0)
       for (int w = 0; w < p.words; ++w) {
         uint64_t some = 0;
@@ -294,36 +238,112 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(TreeParams p
       }
     __syncthreads();
   }
+
+  // ---- the stream of key and value tiles --------------------------------
+  uint8_t* ring = smem + group * (C::kStages * 2 * C::kHalf);
+  float* scales = reinterpret_cast<float*>(smem + C::kRing + wave * (C::kStages * C::kScale));
+  const int turns = (c1 - c0 + C::kStep - 1) / C::kStep;
+  const int64_t row_bytes = (int64_t)p.kvh * D;
+  const int8_t* kbase = p.kc + (int64_t)it.kh * D;
+  const int8_t* vbase = p.vc + (int64_t)it.kh * D;
+  const int32_t* trow = p.table + (int64_t)it.b * p.pps;
+  const int last = c1 > c0 ? c1 - 1 : 0;
+  const int tkey = lane & (C::kTile - 1);  // the key of a tile that this lane looks up
+  auto tile_at = [&](int i) { return c0 + (group + C::kGroups * i) * C::kTile; };
+  auto page_of = [&](int t) { return (int)((uint64_t)(uint32_t)t * p.page_magic >> p.page_shift); };
   auto entry = [&](int i) {  // page-table entry of the lane's key in turn i's tile
-    const int t = tile_at(i) + tkey, jj = t - seq.len;
-    bool on = t < c1;
-    if (p.masks && on && jj >= 0) on = wanted[jj >> 6] >> (jj & 63) & 1;
-    return on ? trow[page_of(t)] : -1;
+    const int t = tile_at(i) + tkey;
+    return trow[page_of(t < c1 ? t : last)];
   };
   int pg = entry(0);
-  float rk = 0.f, rv = 0.f;  // scales on their way
+  uint32_t rk = 0, rv = 0;  // scales on their way, as they lie in the cache
+  bool ron = false;         // and whether there are any
+  auto scale_bits = [&](const void* s, int64_t i) {
+    return p.scale_bf16 ? (uint32_t)reinterpret_cast<const uint16_t*>(s)[i] : reinterpret_cast<const uint32_t*>(s)[i];
+  };
   auto issue = [&](int i, int stage) {
-    const int t = tile_at(i) + tkey;
-    const bool on = t < c1 && pg >= 0 && pg < p.pool_pages;
-    const int r = on ? pg * p.page + (t - page_of(t) * p.page) : -1;
+    const int t0 = tile_at(i), t = t0 + tkey;
+    ron = t < c1 && pg >= 0 && pg < p.pool_pages;
+    if (pick && t0 + C::kTile > seq.len) {  // uniform over the wave
+      const int jj = t - seq.len;
+      if (t < c1 && jj >= 0) ron = ron && (wanted[jj >> 6] >> (jj & 63) & 1);
+    }
+    const int tc = t < c1 ? t : last;
+    const int r = ron ? pg * p.page + (tc - page_of(tc) * p.page) : 0;
     pg = entry(i + 1);
+    const int64_t at = (int64_t)r * p.kvh + it.kh;
     if (C::kTile == 32) {  // lanes 0-31 load key scales, the others value scales
-      rk = r >= 0 ? tree_scale(p, h ? p.vs : p.ks, (int64_t)r * p.kvh + it.kh) : 0.f;
+      rk = scale_bits(h ? p.vs : p.ks, at);
     } else {
-      rk = r >= 0 ? tree_scale(p, p.ks, (int64_t)r * p.kvh + it.kh) : 0.f;
-      rv = r >= 0 ? tree_scale(p, p.vs, (int64_t)r * p.kvh + it.kh) : 0.f;
+      rk = scale_bits(p.ks, at);
+      rv = scale_bits(p.vs, at);
     }
     uint8_t* st = ring + stage * 2 * C::kHalf;
 #pragma unroll
     for (int d = 0; d < C::kDma; ++d) {
-      const int at = (rw * C::kDma + d) * 64;  // first 16-byte slot
-      const int key = (at + lane) / C::kChunks, slot = (at + lane) % C::kChunks;
-      const int rr = __shfl(r, key);
-      const int64_t off = (int64_t)(rr < 0 ? 0 : rr) * row_bytes + 16 * (slot ^ tree_swizzle<C::kChunks>(key));
-      __builtin_amdgcn_global_load_lds(kbase + off, LDS_PTR(st + at * 16), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(vbase + off, LDS_PTR(st + C::kHalf + at * 16), 16, 0, 0);
+      const int first = (rw * C::kDma + d) * 64;  // first 16-byte slot
+      const int line = (first + lane) / C::kChunks, slot = (first + lane) % C::kChunks;
+      const int64_t off = (int64_t)__shfl(r, tree_row(line)) * row_bytes;
+      const int8_t* k = kbase + off + 16 * (slot ^ tree_swizzle<C::kChunks>(line));
+      const int8_t* v = vbase + off + 16 * slot;
+      __builtin_amdgcn_global_load_lds(k, LDS_PTR(st + first * 16), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(v, LDS_PTR(st + C::kHalf + first * 16), 16, 0, 0);
     }
   };
+  issue(0, 0);
+
+  // The lane's row of the tile: query (new token j, head hh of the group), held
+  // as 16-bit integers in two INT8 operands q = (256 hi + lo) 2^(e-14), e the
+  // exponent of the row's largest value: exact for values down to 2^-6 of it.
+  const int row = it.tile * C::kRows + rw * 32 + col;
+  const bool live = row < seq.count * p.r;
+  const int j = live ? row / p.r : 0, hh = live ? row - j * p.r : 0;
+  i32x4 qhi[KS], qlo[KS];
+  float qf;
+  {
+    const uint16_t* src = p.q + (int64_t)(seq.start + j) * p.q_stride + (int64_t)(it.kh * p.r + hh) * D + 16 * h;
+    uint32_t top = 0;  // the largest magnitude's bits
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const u32x4 x = live ? *reinterpret_cast<const u32x4*>(src + 32 * s + 8 * e) : u32x4{0u, 0u, 0u, 0u};
+        i32x4& keep = e ? qlo[s] : qhi[s];
+        keep = __builtin_bit_cast(i32x4, x);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t a = x[w] & 0x7fffu, b = (x[w] >> 16) & 0x7fffu;
+          top = top > a ? top : a;
+          top = top > b ? top : b;
+        }
+      }
+    const uint32_t other = __shfl_xor(top, 32);
+    top = top > other ? top : other;
+    int e = (int)(top >> 7) - 127;
+    e = e < -110 ? -110 : e;  // smaller queries lose bits: scores below 2^-90
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const i32x4 raw[2] = {qhi[s], qlo[s]};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t hi = 0, lo = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x = (uint32_t)raw[w >> 1][(2 * w + (i >> 1)) & 3];
+          const float f = __builtin_bit_cast(float, i & 1 ? x & 0xffff0000u : x << 16);
+          int v = (int)__builtin_rintf(__builtin_ldexpf(f, 14 - e));
+          v = v > 32639 ? 32639 : v;  // 32640 would need hi = 128
+          const int vh = (v + 128) >> 8;
+          hi |= ((uint32_t)vh & 0xffu) << (8 * i);
+          lo |= ((uint32_t)(v - 256 * vh) & 0xffu) << (8 * i);
+        }
+        qhi[s][w] = (int)hi;
+        qlo[s][w] = (int)lo;
+      }
+    }
+    qf = __builtin_ldexpf(p.to_log2, e - 14);
+    if (top >= 0x7f80u) qf = __builtin_nanf("");  // an infinite or NaN query: NaN scores
+  }
 
   f32x16 acc[KS];
 #pragma unroll
@@ -338,8 +358,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(TreeParams p
   // that probability x scale keeps its 11 bits in FP16.
   auto put_scales = [&](int stage) {
     float* sc = scales + stage * (C::kScale / 4);
-    const float v = C::kTile == 32 ? (h ? rk : 0.f) : rv;
-    const float a = fabsf(v) < __builtin_inff() ? fabsf(v) : 0.f;
+    auto value = [&](uint32_t bits) {
+      return ron ? __builtin_bit_cast(float, p.scale_bf16 ? bits << 16 : bits) : 0.f;
+    };
+    const float k = value(rk), v = C::kTile == 32 ? k : value(rv);
+    const float a = (C::kTile == 64 || h) && fabsf(v) < __builtin_inff() ? fabsf(v) : 0.f;
     if (__any(a > vtop)) {
       float x = a;
 #pragma unroll
@@ -350,73 +373,80 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(TreeParams p
       vtop = __builtin_bit_cast(float, (uint32_t)(127 + e + 3 > 254 ? 254 : 127 + e + 3) << 23);
     }
     if (C::kTile == 32) {
-      sc[lane] = h ? v * vfac_new : rk;
+      sc[lane] = h ? v * vfac_new : k;
     } else {
-      sc[lane] = rk;
+      sc[lane] = k;
       sc[64 + lane] = v * vfac_new;
     }
     if (lane == 0) sc[128] = vfac_new;
   };
 
+  const int krow = tree_row(col);
+  const uint32_t koff = krow * D, ksw = tree_swizzle<C::kChunks>(krow);
+  const uint32_t voff = h * D + (D == 64 ? 4 * (col & 15) : D / 32 * col);
+  const uint32_t vsel = D == 64 ? (uint32_t)(col >> 4) * 0x00020002u : 0u;  // the lane's channels of its 4
   auto compute = [&](auto slow, int t0, int stage) {
     const uint8_t* kt = ring + stage * 2 * C::kHalf;
-    const uint8_t* vt = kt + C::kHalf;
-    const float* sc = scales + stage * (C::kScale / 4);
+    const uint8_t* vt = kt + C::kHalf + voff;
+    const float* sc = scales + stage * (C::kScale / 4) + 4 * h;
     float t[C::kBlocks][16];
     float top = -__builtin_inff();
     uint32_t vis[C::kBlocks];
 #pragma unroll
     for (int nb = 0; nb < C::kBlocks; ++nb) {
-      const int key = 32 * nb + col, sw = tree_swizzle<C::kChunks>(key);
       i32x16 hi, lo;
 #pragma unroll
       for (int v = 0; v < 16; ++v) hi[v] = lo[v] = 0;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const i32x4 a = *reinterpret_cast<const i32x4*>(kt + key * D + 16 * ((2 * s + h) ^ sw));
+        const i32x4 a = *reinterpret_cast<const i32x4*>(kt + 32 * nb * D + koff + 16 * ((2 * s + h) ^ ksw));
         hi = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qhi[s], hi, 0, 0, 0);
         lo = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qlo[s], lo, 0, 0, 0);
       }
       if constexpr (slow) {
-        // bit v: the lane's row sees key 8 (v / 4) + 4 h + v % 4 of the block
-        vis[nb] = 0;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int kk = t0 + 32 * nb + 8 * (v >> 2) + 4 * h + (v & 3), jj = kk - seq.len;
-          bool on = live && kk < c1;
-          if (on && jj >= 0)
-            on = p.masks ? (p.masks[(int64_t)(seq.start + j) * p.words + (jj >> 6)] >> (jj & 63)) & 1 : jj <= j;
-          vis[nb] |= on ? 1u << v : 0u;
+        // bit i: the lane's row sees key t0 + 32 nb + i; then moved to the half wave's keys
+        const int k0 = t0 + 32 * nb, jj = k0 - seq.len;
+        uint32_t on = 0;
+        if (p.masks) {
+          const uint64_t* w = p.masks + (int64_t)(seq.start + j) * p.words;
+          if (jj >= 0) {
+            const int at = jj >> 6, sh = jj & 63;
+            const uint64_t a = at < p.words ? w[at] : 0, b = at + 1 < p.words ? w[at + 1] : 0;
+            on = (uint32_t)(a >> sh | (b << 1) << (63 - sh));
+          } else if (jj > -32) {
+            on = (uint32_t)(w[0] << -jj) | ((1u << -jj) - 1);
+          } else {
+            on = ~0u;
+          }
+        } else {
+          const int seen = j + 1 - jj;  // keys of the block up to the row's own
+          on = seen >= 32 ? ~0u : (seen <= 0 ? 0u : (1u << seen) - 1);
         }
+        const int left = c1 - k0;
+        if (left < 32) on &= left <= 0 ? 0u : (1u << left) - 1;
+        vis[nb] = live ? on >> (4 * h) : 0u;
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const f32x4 ksv = *reinterpret_cast<const f32x4*>(sc + 32 * nb + 8 * g + 4 * h);
+        const f32x4 ksv = *reinterpret_cast<const f32x4*>(sc + 32 * nb + 8 * g);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int v = 4 * g + u;
           t[nb][v] = (float)((hi[v] << 8) + lo[v]) * ksv[u];
-          if constexpr (slow) t[nb][v] = vis[nb] >> v & 1 ? t[nb][v] : -__builtin_inff();
+          if constexpr (slow) t[nb][v] = vis[nb] >> (8 * g + u) & 1 ? t[nb][v] : -__builtin_inff();
           top = fmaxf(top, t[nb][v]);
         }
       }
     }
     top *= qf;
-    if (__any(top > m + kTreeSlack)) {
+    const float vf = __builtin_bit_cast(
+        float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sc[128 - 4 * h])));
+    if (__any(top > m + kTreeSlack) || vf != vfac) {  // uniform over the wave
       const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
-      const float fade = __builtin_amdgcn_exp2f(m - to);
-      m = to;
-      l *= fade;
-      psum *= fade;
-#pragma unroll
-      for (int c = 0; c < KS; ++c)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) acc[c][v] *= fade;
-    }
-    const float vf = sc[128];
-    if (vf != vfac) {  // uniform over the wave
-      const float fade = vf / vfac;
+      const float fade_l = __builtin_amdgcn_exp2f(m - to), fade = fade_l * (vf / vfac);
       vfac = vf;
+      m = to;
+      l *= fade_l;
       psum *= fade;
 #pragma unroll
       for (int c = 0; c < KS; ++c)
@@ -430,15 +460,14 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(TreeParams p
         f16x8 pv;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const f32x4 vsv =
-              *reinterpret_cast<const f32x4*>(sc + (C::kTile == 32 ? 32 : 64) + 32 * nb + 16 * mm + 8 * g + 4 * h);
+          const f32x4 vsv = *reinterpret_cast<const f32x4*>(sc + (C::kTile == 32 ? 32 : 64) + 32 * nb + 16 * mm + 8 * g);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int v = 8 * mm + 4 * g + u;
             const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(t[nb][v], qf, -m));
             float w = e * vsv[u];
             if constexpr (slow) {
-              const bool on = vis[nb] >> v & 1;
+              const bool on = vis[nb] >> (16 * mm + 8 * g + u) & 1;
               l += on ? e : 0.f;
               w = on ? w : 0.f;
             } else {
@@ -452,24 +481,30 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(TreeParams p
           const f16x2 one = {(_Float16)1.f, (_Float16)1.f}, pair = {pv[2 * u], pv[2 * u + 1]};
           psum = __builtin_amdgcn_fdot2(pair, one, psum, false);
         }
-        // values: 8 rows of 16 bytes per 16 lanes, read transposed: the lane gets the
-        // bytes of its channel at its half wave's 8 keys
-        const int i16 = lane & 15, jr = i16 >> 1;
-        const int key = 32 * nb + 16 * mm + 8 * (jr >> 2) + 4 * h + (jr & 3);
-        const int sw = tree_swizzle<C::kChunks>(key);
+        // Values: the lane's channels of its half wave's 8 keys; byte b of two keys
+        // makes one operand word. Code + 128 enters as an FP16 subnormal, (code + 128)
+        // 2^-24: the 128 is taken back at the end with the sum of the rounded
+        // probabilities.
+        constexpr int W = D == 256 ? 2 : 1;
+        uint32_t x[8][W];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint8_t* src = vt + (32 * nb + 16 * mm + tree_row(8 * (i >> 2) + (i & 3))) * D;
+          if constexpr (W == 2) {
+            const u32x2 y = *reinterpret_cast<const u32x2*>(src);
+            x[i][0] = y[0] ^ 0x80808080u;
+            x[i][1] = y[1] ^ 0x80808080u;
+          } else {
+            x[i][0] = *reinterpret_cast<const uint32_t*>(src) ^ 0x80808080u;
+          }
+        }
 #pragma unroll
         for (int c = 0; c < KS; ++c) {
-          const uint8_t* src = vt + key * D + 16 * ((2 * c + ((lane >> 4) & 1)) ^ sw) + 8 * (i16 & 1);
-          const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-              (__attribute__((address_space(3))) i32x2*)(uint32_t)(uintptr_t)src);
-          // code + 128 as an FP16 subnormal, (code + 128) 2^-24: the shift by 128 is
-          // taken back at the end with the sum of the rounded probabilities
-          const uint32_t w0 = (uint32_t)w[0] ^ 0x80808080u, w1 = (uint32_t)w[1] ^ 0x80808080u;
           u32x4 a;
-          a[0] = __builtin_amdgcn_perm(w0, w0, 0x0c010c00u);
-          a[1] = __builtin_amdgcn_perm(w0, w0, 0x0c030c02u);
-          a[2] = __builtin_amdgcn_perm(w1, w1, 0x0c010c00u);
-          a[3] = __builtin_amdgcn_perm(w1, w1, 0x0c030c02u);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            a[q] = __builtin_amdgcn_perm(x[2 * q + 1][c >> 2], x[2 * q][c >> 2],
+                                         0x0c040c00u + (uint32_t)(c & 3) * 0x00010001u + vsel);
           acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), pv, acc[c], 0, 0, 0);
         }
       }
@@ -479,26 +514,35 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(TreeParams p
   // later. Waits count DMA instructions: those of the tiles after this one may
   // still be in flight.
 #pragma unroll
-  for (int i = 0; i < C::kStages - 1; ++i) {
-    if (i > 0) put_scales(i - 1);
+  for (int i = 1; i < C::kStages - 1; ++i) {
+    put_scales(i - 1);
     issue(i, i);
   }
   int stage = 0;
-  for (int i = 0; i < turns; ++i) {
+  auto advance = [&](int i) {
     tree_wait_vm<(C::kStages - 2) * 2 * C::kDma>();
     // the wave's reads of the stage that is written next have returned
     if (RW > 1)
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     else
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    const int newest = (stage + C::kStages - 2) % C::kStages, next = (stage + C::kStages - 1) % C::kStages;
-    put_scales(newest);
+    const int next = stage == 0 ? C::kStages - 1 : stage - 1;
+    put_scales(C::kStages == 2 ? stage : (stage + 1 == C::kStages ? 0 : stage + 1));
     issue(i + C::kStages - 1, next);
-    const int t0 = tile_at(i);
-    if (t0 + C::kTile <= n_all && t0 + C::kTile <= c1)
-      compute(std::false_type{}, t0, stage);
-    else if (t0 < c1)
-      compute(std::true_type{}, t0, stage);
+  };
+  // first the turns whose tile every row sees whole
+  const int open = (n_all < c1 ? n_all : c1) - tile_at(0);
+  int fast = open / C::kTile > 0 ? (open / C::kTile - 1) / C::kGroups + 1 : 0;
+  fast = fast < turns ? fast : turns;
+  int i = 0;
+  for (; i < fast; ++i) {
+    advance(i);
+    compute(std::false_type{}, 0, stage);
+    stage = stage + 1 == C::kStages ? 0 : stage + 1;
+  }
+  for (; i < turns; ++i) {
+    advance(i);
+    compute(std::true_type{}, tile_at(i), stage);
     stage = stage + 1 == C::kStages ? 0 : stage + 1;
   }
   tree_wait_vm<0>();
@@ -512,11 +556,21 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(TreeParams p
   for (int c = 0; c < KS; ++c)
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[c][v] = (acc[c][v] - shift) * up;
+  // Channels q * kRun + [0, kRun) of a lane's sums lie together.
+  constexpr int kRun = D == 64 ? 4 : KS, kRuns = KS * 16 / kRun;
+  auto at_run = [&](int q) { return tree_channel<D>(0, q, h); };
+  auto of_run = [&](int q, int u) { return D == 64 ? acc[u & 1][q + 8 * (u >> 1)] : acc[D == 64 ? 0 : u][q]; };
+  auto set_run = [&](int q, int u, float v) {
+    if constexpr (D == 64)
+      acc[u & 1][q + 8 * (u >> 1)] = v;
+    else
+      acc[u][q] = v;
+  };
   if constexpr (C::kGroups > 1) {
     // the groups' sums meet in LDS, in group order
     __syncthreads();
-    float* st = reinterpret_cast<float*>(smem);                    // [group][row]: maximum, sum
-    float* sum = st + 2 * C::kGroups * C::kRows;                   // [row][D], one group at a time
+    float* st = reinterpret_cast<float*>(smem);   // [group][row]: maximum, sum
+    float* sum = st + 2 * C::kGroups * C::kRows;  // [row][D], one group at a time
     const int rr = rw * 32 + col;
     if (h == 0) {
       st[2 * (group * C::kRows + rr)] = m;
@@ -531,27 +585,32 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(TreeParams p
       all += st[2 * (g * C::kRows + rr) + 1] * __builtin_amdgcn_exp2f(st[2 * (g * C::kRows + rr)] - to);
     const float fade = __builtin_amdgcn_exp2f(m - to);
 #pragma unroll
+    for (int c = 0; c < KS; ++c)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[c][v] *= fade;
     for (int g = C::kGroups - 1; g >= 0; --g) {
       if (group == g) {
 #pragma unroll
-        for (int c = 0; c < KS; ++c)
+        for (int q = 0; q < kRuns; ++q)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            f32x4* at = reinterpret_cast<f32x4*>(sum + rr * (D + 4) + 32 * c + 8 * q + 4 * h);
-            f32x4 v = {acc[c][4 * q] * fade, acc[c][4 * q + 1] * fade, acc[c][4 * q + 2] * fade,
-                       acc[c][4 * q + 3] * fade};
+          for (int u = 0; u < kRun; u += 4) {
+            f32x4* at = reinterpret_cast<f32x4*>(sum + rr * (D + 4) + at_run(q) + u);
+            f32x4 v = {of_run(q, u), of_run(q, u + 1), of_run(q, u + 2), of_run(q, u + 3)};
             if (g < C::kGroups - 1) v += *at;
-            if (g > 0) {
-              *at = v;
-            } else {
-#pragma unroll
-              for (int u = 0; u < 4; ++u) acc[c][4 * q + u] = v[u];
-            }
+            *at = v;
           }
       }
       __syncthreads();
     }
     if (group > 0) return;
+#pragma unroll
+    for (int q = 0; q < kRuns; ++q)
+#pragma unroll
+      for (int u = 0; u < kRun; u += 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(sum + rr * (D + 4) + at_run(q) + u);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) set_run(q, u + w, v[w]);
+      }
     m = to;
     l = all;
   }
@@ -560,23 +619,23 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(TreeParams p
     const int64_t at = (int64_t)blockIdx.x * C::kRows + rw * 32 + col;
     float* dst = p.part + at * D;
 #pragma unroll
-    for (int c = 0; c < KS; ++c)
+    for (int q = 0; q < kRuns; ++q)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f32x4*>(dst + 32 * c + 8 * q + 4 * h) =
-            f32x4{acc[c][4 * q], acc[c][4 * q + 1], acc[c][4 * q + 2], acc[c][4 * q + 3]};
+      for (int u = 0; u < kRun; u += 4)
+        *reinterpret_cast<f32x4*>(dst + at_run(q) + u) =
+            f32x4{of_run(q, u), of_run(q, u + 1), of_run(q, u + 2), of_run(q, u + 3)};
     if (h == 0) *reinterpret_cast<f32x2*>(p.stat + 2 * at) = f32x2{m, l};
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* dst = p.out + ((int64_t)(seq.start + j) * p.hq + it.kh * p.r + hh) * D;
 #pragma unroll
-  for (int c = 0; c < KS; ++c)
+  for (int q = 0; q < kRuns; ++q)
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<u32x2*>(dst + 32 * c + 8 * q + 4 * h) =
-          u32x2{pack_bf16x2(acc[c][4 * q] * inv, acc[c][4 * q + 1] * inv),
-                pack_bf16x2(acc[c][4 * q + 2] * inv, acc[c][4 * q + 3] * inv)};
+    for (int u = 0; u < kRun; u += 4)
+      *reinterpret_cast<u32x2*>(dst + at_run(q) + u) =
+          u32x2{pack_bf16x2(of_run(q, u) * inv, of_run(q, u + 1) * inv),
+                pack_bf16x2(of_run(q, u + 2) * inv, of_run(q, u + 3) * inv)};
 }
 
 // The chunks' sums of a row joined in chunk order: four channels per thread.
