@@ -60,14 +60,16 @@ struct TreeCfg {
   static constexpr int kTile = RW == 1 ? 32 : 64;  // keys per tile of a group
   static constexpr int kBlocks = kTile / 32;
   static constexpr int kStep = kTile * kGroups;  // keys per turn of the workgroup
-  static constexpr int kStages = D == 256 && RW < 4 ? 2 : 3;
+  // Stages: two workgroups share a CU's LDS, one of 256-channel heads
+  static constexpr int kStages = D > 64 && RW < 4 ? 2 : 3;
+  static constexpr int kPerCu = D == 256 ? 1 : 2;  // workgroups per CU
   static constexpr int kHalf = kTile * D;        // bytes of a tile's keys, and of its values
   static constexpr int kDma = kHalf / 1024 / RW;  // DMA instructions per wave for each
   static constexpr int kChunks = D / 16;         // 16-byte chunks of a key
   static constexpr int kRing = kGroups * kStages * 2 * kHalf;
   static constexpr int kScale = 2 * 64 * 4 + 16;  // per wave and stage: key and value scales, value factor
   static constexpr int kLds = kRing + 4 * kStages * kScale + 32;  // and four words of masks
-  static_assert(kHalf % (1024 * RW) == 0 && kLds <= 160 * 1024, "tile");
+  static_assert(kHalf % (1024 * RW) == 0 && kPerCu * kLds <= 160 * 1024, "tile");
 };
 
 template <int N>
@@ -113,75 +115,93 @@ __device__ __forceinline__ void tree_reach(const TreeParams& p, const TreeSeq& s
 
 struct TreeItem {
   int b, tile, kh, chunk, keys;
+  TreeSeq seq;
 };
 
-// The workgroup's item. The call's work, sum over sequences of tiles x heads x
-// keys, is cut into chunks of an equal number of keys, one per slot, so that
-// ragged lengths fill the chip evenly; every workgroup derives the same cut from
-// the lengths, which only the GPU knows. Thread t takes the sequences [t, t + 1) * per.
+template <typename T, typename F>
+__device__ __forceinline__ T tree_wave_reduce(T v, F f) {
+  const auto step = [&](auto ctrl) {
+    const int w = __builtin_bit_cast(int, v);
+    v = f(v, __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(w, w, decltype(ctrl)::value, 0xf, 0xf, true)));
+  };
+  step(std::integral_constant<int, 0xb1>{});   // quad_perm [1,0,3,2]
+  step(std::integral_constant<int, 0x4e>{});   // quad_perm [2,3,0,1]
+  step(std::integral_constant<int, 0x124>{});  // row_ror:4
+  step(std::integral_constant<int, 0x128>{});  // row_ror:8
+  v = f(v, __shfl_xor(v, 16));
+  return f(v, __shfl_xor(v, 32));
+}
+
+// The workgroup's item, found by each wave for itself (lane t takes the sequences
+// t, t + 64, ..). The call's work, sum over sequences of tiles x heads x keys, is
+// cut into chunks of at most ``keys`` keys: the least number that gives no more
+// chunks than the chip holds workgroups, so that all run at once and, whatever the
+// lengths, end together. Only the GPU knows the lengths. (Cut at the mean instead,
+// 64-token trees made 640 chunks for 512 places: 321 us against 236.) Where the
+// tiles themselves fill half of the places or more, the chunks are half as long as
+// the mean share and run in turns.
 template <int ROWS, int STEP>
 __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
-  __shared__ int64_t sums[4];
-  __shared__ int item[5];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int per = (p.batch + kTreeThreads - 1) / kTreeThreads;
-  const int b0 = t * per, b1 = b0 + per < p.batch ? b0 + per : p.batch;
-  int64_t cost = 0;
-  TreeSeq s{0, 0, 0, 0};
-  for (int b = b0; b < b1; ++b) {
-    s = tree_seq(p, b);
-    cost += (int64_t)tree_tiles(p, s, ROWS) * p.kvh * s.n;
-  }
-  if (t == 0) item[0] = -1;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) cost += __shfl_xor(cost, off);
-  if (lane == 0) sums[wave] = cost;
-  __syncthreads();
-  const int64_t total = sums[0] + sums[1] + sums[2] + sums[3];
-  int64_t keys = (total + p.slots - 1) / p.slots;
-  keys = (keys + STEP - 1) / STEP * STEP;
-  if (keys < STEP) keys = STEP;
-  if (p.whole || keys > (1 << 30)) keys = 1 << 30;
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    if (per > 1) s = tree_seq(p, b);
-    mine += (int64_t)tree_tiles(p, s, ROWS) * p.kvh * tree_chunks(s.n, (int)keys);
-  }
-  int64_t upto = mine;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t v = __shfl_up(upto, off);
-    if (lane >= off) upto += v;
-  }
-  __syncthreads();
-  if (lane == 63) sums[wave] = upto;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) upto += sums[w];
-  int64_t first = upto - mine;
-  const int64_t id = blockIdx.x;
-  if (id >= first && id < upto)
-    for (int b = b0; b < b1; ++b) {
-      if (per > 1) s = tree_seq(p, b);
-      const int tiles = tree_tiles(p, s, ROWS);
-      const int64_t n = (int64_t)tiles * p.kvh * tree_chunks(s.n, (int)keys);
-      if (id >= first && id < first + n) {
-        const int at = (int)(id - first);
-        item[0] = b;
-        item[1] = at % tiles;
-        item[2] = at / tiles % p.kvh;
-        item[3] = at / tiles / p.kvh;
-        item[4] = (int)keys;
-        if (at == 0) p.info[b] = (int32_t)id;
+  const int lane = threadIdx.x & 63;
+  const TreeSeq none{0, 0, 0, 0}, mine = lane < p.batch ? tree_seq(p, lane) : none;
+  const auto units = [&](const TreeSeq& s) { return tree_tiles(p, s, ROWS) * p.kvh; };
+  const auto sum = [&](auto zero, auto of) {
+    auto v = lane < p.batch ? of(mine) : zero;
+    for (int b = lane + 64; b < p.batch; b += 64) v += of(tree_seq(p, b));
+    return tree_wave_reduce(v, [](auto x, auto y) { return x + y; });
+  };
+  int keys = 1 << 30;
+  if (!p.whole) {
+    const float total = sum(0.f, [&](const TreeSeq& s) { return (float)units(s) * (float)s.n; });
+    const int tiles = sum(0, units);
+    const bool once = 2 * tiles <= p.slots;
+    int lo = (int)(total / (float)(once ? p.slots : 2 * p.slots) * (1.f / STEP));
+    lo = lo < 1 ? 1 : (lo < (1 << 30) / STEP / 2 - 1 ? lo : (1 << 30) / STEP / 2 - 1);
+    int hi = once ? 2 * lo + 2 : lo + 1;  // in steps; hi gives few enough chunks
+    if (once && p.batch <= 256)
+      for (int i = 0; i < 5 && lo < hi; ++i) {
+        const int mid = (lo + hi) >> 1;
+        const int n = sum(0, [&](const TreeSeq& s) { return units(s) * tree_chunks(s.n, mid * STEP); });
+        if (n <= p.slots)
+          hi = mid;
+        else
+          lo = mid + 1;
       }
-      first += n;
+    keys = hi * STEP;
+  }
+  const int id = blockIdx.x;
+  int base = 0;
+  it.b = -1;
+  it.keys = keys;
+  for (int b0 = 0; b0 < p.batch; b0 += 64) {  // 64 sequences at a time
+    const TreeSeq s = b0 == 0 ? mine : (b0 + lane < p.batch ? tree_seq(p, b0 + lane) : none);
+    const int n = units(s) * tree_chunks(s.n, keys);
+    int upto = n;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int v = __shfl_up(upto, off);
+      if (lane >= off) upto += v;
     }
-  if (id == 0 && t == 0) p.info[p.batch] = (int32_t)keys;
-  __syncthreads();
-  it.b = __builtin_amdgcn_readfirstlane(item[0]);
-  it.tile = __builtin_amdgcn_readfirstlane(item[1]);
-  it.kh = __builtin_amdgcn_readfirstlane(item[2]);
-  it.chunk = __builtin_amdgcn_readfirstlane(item[3]);
-  it.keys = __builtin_amdgcn_readfirstlane(item[4]);
+    upto += base;
+    const uint64_t has = __ballot(id < upto);
+    if (has) {
+      const int at = __builtin_ctzll(has);
+      it.b = b0 + at;
+      it.seq.start = __builtin_amdgcn_readlane(s.start, at);
+      it.seq.count = __builtin_amdgcn_readlane(s.count, at);
+      it.seq.len = __builtin_amdgcn_readlane(s.len, at);
+      it.seq.n = __builtin_amdgcn_readlane(s.n, at);
+      const int first = __builtin_amdgcn_readlane(upto - n, at), in = id - first;
+      const int tiles = tree_tiles(p, it.seq, ROWS), row = in / tiles;
+      it.tile = in - row * tiles;
+      it.chunk = row / p.kvh;
+      it.kh = row - it.chunk * p.kvh;
+      if (threadIdx.x == 0 && in == 0) p.info[it.b] = first;
+      break;
+    }
+    base = __builtin_amdgcn_readlane(upto, 63);
+  }
+  if (threadIdx.x == 0 && id == 0) p.info[p.batch] = keys;
   return it.b >= 0;
 }
 
@@ -215,7 +235,7 @@ __global__ void __launch_bounds__(kTreeThreads, D == 256 ? 1 : 2) tree_attn_kern
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = wave / RW, rw = wave % RW;
   const int col = lane & 31, h = lane >> 5;
-  const TreeSeq seq = tree_seq(p, it.b);
+  const TreeSeq seq = it.seq;
   int n, n_all;
   tree_reach(p, seq, it.tile, C::kRows, &n, &n_all);
   const int c0 = it.chunk * it.keys;
@@ -319,26 +339,29 @@ __global__ void __launch_bounds__(kTreeThreads, D == 256 ? 1 : 2) tree_attn_kern
       }
     const uint32_t other = __shfl_xor(top, 32);
     top = top > other ? top : other;
-    int e = (int)(top >> 7) - 127;
+    int e = (int)(top >> 7) - 127 + ((top & 0x7f) == 0x7f);  // the largest stays below 127 * 256 + 128
     e = e < -110 ? -110 : e;  // smaller queries lose bits: scores below 2^-90
+    // v = q 2^(14-e) rounded into the low bits of 1.5 * 2^23 + v; its low byte is lo,
+    // the second byte of v + 128 is hi
+    const float up = __builtin_ldexpf(1.f, 14 - e);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const i32x4 raw[2] = {qhi[s], qlo[s]};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        uint32_t hi = 0, lo = 0;
+        uint32_t v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t x = (uint32_t)raw[w >> 1][(2 * w + (i >> 1)) & 3];
           const float f = __builtin_bit_cast(float, i & 1 ? x & 0xffff0000u : x << 16);
-          int v = (int)__builtin_rintf(__builtin_ldexpf(f, 14 - e));
-          v = v > 32639 ? 32639 : v;  // 32640 would need hi = 128
-          const int vh = (v + 128) >> 8;
-          hi |= ((uint32_t)vh & 0xffu) << (8 * i);
-          lo |= ((uint32_t)(v - 256 * vh) & 0xffu) << (8 * i);
+          v[i] = __builtin_bit_cast(uint32_t, __builtin_fmaf(f, up, 12582912.f));
         }
-        qhi[s][w] = (int)hi;
-        qlo[s][w] = (int)lo;
+        const uint32_t l01 = __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0400u);
+        const uint32_t l23 = __builtin_amdgcn_perm(v[3], v[2], 0x04000c0cu);
+        const uint32_t h01 = __builtin_amdgcn_perm(v[1] + 128, v[0] + 128, 0x0c0c0501u);
+        const uint32_t h23 = __builtin_amdgcn_perm(v[3] + 128, v[2] + 128, 0x05010c0cu);
+        qhi[s][w] = (int)(h01 | h23);
+        qlo[s][w] = (int)(l01 | l23);
       }
     }
     qf = __builtin_ldexpf(p.to_log2, e - 14);
@@ -638,44 +661,70 @@ __global__ void __launch_bounds__(kTreeThreads, D == 256 ? 1 : 2) tree_attn_kern
                 pack_bf16x2(of_run(q, u + 2) * inv, of_run(q, u + 3) * inv)};
 }
 
-// The chunks' sums of a row joined in chunk order: four channels per thread.
-__global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p, int dim, int tile_rows) {
-  const int row = blockIdx.x;
+// The chunks' sums of a row and head joined in chunk order, D / 4 lanes of four
+// channels each. Eight chunks' sums are loaded at a time; lane i of the head holds
+// the weight of chunk i.
+template <int D>
+__global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p, int tile_rows) {
+  constexpr int W = D / 4;  // lanes per head
+  const int row = blockIdx.x, lane = threadIdx.x & 63;
   const int at = (blockIdx.y * kTreeThreads + threadIdx.x) * 4;  // within the row's heads
-  int b = 0, hi = p.batch - 1;  // the last sequence with starts[b] <= row
-  while (b < hi) {
-    const int mid = (b + hi + 1) / 2;
-    if (p.starts[mid] <= row)
-      b = mid;
-    else
-      hi = mid - 1;
+  int b = 0;  // the sequences that end before the row
+  for (int b0 = 0; b0 < p.batch; b0 += 64) {
+    const uint64_t before = __ballot(b0 + lane < p.batch && p.starts[b0 + lane + 1] <= row);
+    b += __popcll(before);
+    if (!(before >> 63)) break;
   }
+  if (b >= p.batch) return;
   const TreeSeq s = tree_seq(p, b);
+  const int keys = p.info[p.batch], from = p.info[b];
   const int j = row - s.start;
-  if (j < 0 || j >= s.count || at >= p.hq * dim) return;
-  const int head = at / dim, c = at - head * dim, kh = head / p.r, rr = j * p.r + head - kh * p.r;
-  const int tile = rr / tile_rows, tiles = tree_tiles(p, s, tile_rows), keys = p.info[p.batch];
+  if (j < 0 || j >= s.count || at >= p.hq * D) return;  // whole heads
+  const int head = at / D, c = at - head * D, kh = head / p.r, rr = j * p.r + head - kh * p.r;
+  const int tile = rr / tile_rows, tiles = tree_tiles(p, s, tile_rows);
   int n, n_all;
   tree_reach(p, s, tile, tile_rows, &n, &n_all);
   const int chunks = tree_chunks(n, keys);
   if (chunks == 1) return;
-  const int64_t first = p.info[b] + (int64_t)kh * tiles + tile, step = (int64_t)p.kvh * tiles;
-  const int in = rr - tile * tile_rows;
-  float m = kTreeFloor;
-  for (int i = 0; i < chunks; ++i) m = fmaxf(m, p.stat[2 * ((first + i * step) * tile_rows + in)]);
-  float l = 0.f;
+  const int64_t first = ((int64_t)from + (int64_t)kh * tiles + tile) * tile_rows + rr - tile * tile_rows;
+  const int64_t step = (int64_t)p.kvh * tiles * tile_rows;
+  const int in = lane & (W - 1);
+  float m = kTreeFloor, l = 0.f;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < chunks; ++i) {
-    const int64_t slot = (first + i * step) * tile_rows + in;
-    const f32x2 st = *reinterpret_cast<const f32x2*>(p.stat + 2 * slot);
-    const float f = __builtin_amdgcn_exp2f(st[0] - m);
-    l += st[1] * f;
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + slot * dim + c);
+  for (int i0 = 0; i0 < chunks; i0 += W) {
+    const bool on = i0 + in < chunks;
+    const f32x2 st = on ? *reinterpret_cast<const f32x2*>(p.stat + 2 * (first + (i0 + in) * step)) : f32x2{kTreeFloor, 0.f};
+    float to = st[0];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = __builtin_fmaf(x[u], f, v[u]);
+    for (int off = 1; off < W; off <<= 1) to = fmaxf(to, __shfl_xor(to, off));
+    to = fmaxf(to, m);
+    const float fade = __builtin_amdgcn_exp2f(m - to), weight = __builtin_amdgcn_exp2f(st[0] - to);
+    m = to;
+    float some = st[1] * weight;
+#pragma unroll
+    for (int off = 1; off < W; off <<= 1) some += __shfl_xor(some, off);
+    l = l * fade + some;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] *= fade;
+    const int end = chunks - i0 < W ? chunks - i0 : W;
+    for (int i = 0; i < end; i += 8) {
+      f32x4 x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int ii = i + k < end ? i + k : end - 1;
+        x[k] = *reinterpret_cast<const f32x4*>(p.part + (first + (i0 + ii) * step) * D + c);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float f = __shfl(weight, i + k, W);
+        if (i + k < end)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) v[u] = __builtin_fmaf(x[k][u], f, v[u]);
+      }
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<u32x2*>(p.out + (int64_t)row * p.hq * dim + at) =
+  *reinterpret_cast<u32x2*>(p.out + (int64_t)row * p.hq * D + at) =
       u32x2{pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv)};
 }
 
@@ -698,9 +747,9 @@ static TreeLayout tree_layout(int64_t batch, int64_t rows, int64_t max_count, in
   // row tiles of all sequences together: each ends with one that is not full
   const int64_t by_batch = batch * cdiv(max_count * r, tile), by_rows = rows * r / tile + batch;
   const int64_t units = kvh * (by_batch < by_rows ? by_batch : by_rows);
-  L.slots = kTreeCus * (L.row_waves == 4 && dim < 256 ? 2 : 1);
+  L.slots = kTreeCus * (dim == 256 ? TreeCfg<256, 1>::kPerCu : TreeCfg<128, 1>::kPerCu);
   L.whole = units >= 4 * L.slots;
-  L.grid = units + (L.whole ? 0 : L.slots);
+  L.grid = L.whole ? units : (2 * units <= L.slots ? L.slots : units + 2 * L.slots);
   const int64_t parts = L.whole ? 0 : L.grid * tile;
   L.info = 0;
   L.stat = tree_align(L.info + (size_t)(batch + 1) * 4);
@@ -719,8 +768,8 @@ static int tree_launch(const TreeParams& p, const TreeLayout& L, hipStream_t s) 
   });
   hipLaunchKernelGGL((tree_attn_kernel<D, RW>), dim3((unsigned)L.grid), dim3(kTreeThreads), C::kLds, s, p);
   if (!L.whole)
-    hipLaunchKernelGGL(tree_combine_kernel, dim3((unsigned)p.rows, (unsigned)cdiv(p.hq * D, 4 * kTreeThreads)),
-                       dim3(kTreeThreads), 0, s, p, D, C::kRows);
+    hipLaunchKernelGGL(tree_combine_kernel<D>, dim3((unsigned)p.rows, (unsigned)cdiv(p.hq * D, 4 * kTreeThreads)),
+                       dim3(kTreeThreads), 0, s, p, C::kRows);
   return check_launch("tree_attention");
 }
 
