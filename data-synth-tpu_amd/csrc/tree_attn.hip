@@ -53,23 +53,34 @@ struct TreeParams {
   uint16_t* out;
 };
 
-template <int D, int RW>
-struct TreeCfg {
-  static constexpr int kRows = 32 * RW;          // (new token, head of the group) rows per workgroup
-  static constexpr int kGroups = 4 / RW;         // waves that share rows take different keys
-  static constexpr int kTile = RW == 1 ? 32 : 64;  // keys per tile of a group
-  static constexpr int kBlocks = kTile / 32;
-  static constexpr int kStep = kTile * kGroups;  // keys per turn of the workgroup
-  // Stages: two workgroups share a CU's LDS, one of 256-channel heads
-  static constexpr int kStages = D > 64 && RW < 4 ? 2 : 3;
-  static constexpr int kPerCu = D == 256 ? 1 : 2;  // workgroups per CU
-  static constexpr int kHalf = kTile * D;        // bytes of a tile's keys, and of its values
-  static constexpr int kDma = kHalf / 1024 / RW;  // DMA instructions per wave for each
-  static constexpr int kChunks = D / 16;         // 16-byte chunks of a key
-  static constexpr int kRing = kGroups * kStages * 2 * kHalf;
-  static constexpr int kScale = 2 * 64 * 4 + 16;  // per wave and stage: key and value scales, value factor
+// Calls of few rows per KV head: 32 rows per workgroup, every wave all of them
+// with keys of its own. Bound by memory.
+template <int D>
+struct TreeThin {
+  static constexpr int kRows = 32;    // (new token, head of the group) rows per workgroup
+  static constexpr int kTile = 32;    // keys per tile of a wave
+  static constexpr int kStep = 128;   // keys per turn of the workgroup
+  static constexpr int kStages = D > 64 ? 2 : 3;
+  static constexpr int kPerCu = D > 128 ? 1 : 2;  // workgroups per CU
+  static constexpr int kHalf = kTile * D;         // bytes of a tile's keys, and of its values
+  static constexpr int kScale = 2 * 32 * 4 + 16;  // per wave and stage: key and value scales, value factor
+  static constexpr int kRing = 4 * kStages * 2 * kHalf;
   static constexpr int kLds = kRing + 4 * kStages * kScale + 32;  // and four words of masks
-  static_assert(kHalf % (1024 * RW) == 0 && kPerCu * kLds <= 160 * 1024, "tile");
+  static_assert(kPerCu * kLds <= 160 * 1024, "tile");
+};
+
+// Calls of many rows: 128 rows per workgroup, 32 per wave, which share the keys.
+// Bound by the vector ALU.
+template <int D>
+struct TreeWide {
+  static constexpr int kRows = 128;
+  static constexpr int kTile = D == 256 ? 32 : 64;
+  static constexpr int kStep = kTile;
+  static constexpr int kPerCu = D == 64 ? 3 : 2;
+  static constexpr int kHalf = kTile * D;
+  static constexpr int kScale = 2 * kTile * 4 + 16;
+  static constexpr int kLds = 2 * kHalf + 4 * kHalf + 4 * kScale + 32;  // a tile's codes, the same in FP16
+  static_assert(kPerCu * kLds <= 160 * 1024, "tile");
 };
 
 template <int N>
@@ -114,7 +125,7 @@ __device__ __forceinline__ void tree_reach(const TreeParams& p, const TreeSeq& s
 }
 
 struct TreeItem {
-  int b, tile, kh, chunk, keys;
+  int id, b, tile, kh, chunk, keys;
   TreeSeq seq;
 };
 
@@ -148,7 +159,8 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
   const auto sum = [&](auto zero, auto of) {
     auto v = lane < p.batch ? of(mine) : zero;
     for (int b = lane + 64; b < p.batch; b += 64) v += of(tree_seq(p, b));
-    return tree_wave_reduce(v, [](auto x, auto y) { return x + y; });
+    v = tree_wave_reduce(v, [](auto x, auto y) { return x + y; });
+    return __builtin_bit_cast(decltype(v), __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
   };
   int keys = 1 << 30;
   if (!p.whole) {
@@ -169,7 +181,10 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
       }
     keys = hi * STEP;
   }
-  const int id = blockIdx.x;
+  // Workgroup i runs on XCD i % 8: each XCD takes a contiguous run of items, so
+  // that the tiles that share a chunk's keys share its L2
+  const int id = (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3));
+  it.id = id;
   int base = 0;
   it.b = -1;
   it.keys = keys;
@@ -211,12 +226,13 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
 // tree_swizzle(row), so that the 16 lanes that read one column of 16 keys meet 16
 // different bank groups; values, read by rows, lie as they are.
 __device__ __forceinline__ int tree_row(int key) { return (key & ~5) | (key & 1) << 2 | (key >> 2 & 1); }
-template <int CH>
+template <int D>
 __device__ __forceinline__ int tree_swizzle(int row) {
+  constexpr int CH = D / 16;
   return (row / (16 / CH)) & (CH - 1);
 }
 
-// The channel of accumulator element v (of channel block c), for a lane of half
+// The channel of accumulator element v of channel block c, for a lane of half
 // wave h: each lane's loads of D / 32 consecutive channels of a key serve all
 // blocks (for D = 64, of 4 channels, of which the upper 16 rows take the last two).
 template <int D>
@@ -225,15 +241,237 @@ __device__ __forceinline__ int tree_channel(int c, int v, int h) {
   return D == 64 ? 4 * (i & 15) + 2 * (i >> 4) + c : D / 32 * i + c;
 }
 
-template <int D, int RW>
-__global__ void __launch_bounds__(kTreeThreads, D == 256 ? 1 : 2) tree_attn_kernel(TreeParams p) {
-  using C = TreeCfg<D, RW>;
+// New tokens that some row of the sequence sees. What the cache holds at the
+// others' places (they may never have been written) is not read. One wave's work.
+__device__ __forceinline__ void tree_wanted(const TreeParams& p, const TreeSeq& s, uint64_t* wanted) {
+  const int lane = threadIdx.x & 63;
+  for (int w = 0; w < p.words; ++w) {
+    uint64_t some = 0;
+    for (int i = lane; i < s.count; i += 64) some |= p.masks[(int64_t)(s.start + i) * p.words + w];
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) some |= __shfl_xor((unsigned long long)some, off);
+    if (lane == 0) wanted[w] = some;
+  }
+}
+
+// Bit i: a row's token j sees key k0 + i; moved to the keys of half wave h.
+__device__ __forceinline__ uint32_t tree_visible(const TreeParams& p, const TreeSeq& s, int j, int k0, int c1, int h) {
+  const int jj = k0 - s.len;
+  uint32_t on;
+  if (p.masks) {
+    const uint64_t* w = p.masks + (int64_t)(s.start + j) * p.words;
+    if (jj >= 0) {
+      const int at = jj >> 6, sh = jj & 63;
+      const uint64_t a = at < p.words ? w[at] : 0, b = at + 1 < p.words ? w[at + 1] : 0;
+      on = (uint32_t)(a >> sh | (b << 1) << (63 - sh));
+    } else if (jj > -32) {
+      on = (uint32_t)(w[0] << -jj) | ((1u << -jj) - 1);
+    } else {
+      on = ~0u;
+    }
+  } else {
+    const int seen = j + 1 - jj;  // keys of the block up to the row's own
+    on = seen >= 32 ? ~0u : (seen <= 0 ? 0u : (1u << seen) - 1);
+  }
+  const int left = c1 - k0;
+  if (left < 32) on &= left <= 0 ? 0u : (1u << left) - 1;
+  return on >> (4 * h);
+}
+
+// The way from a tile's keys to the cache: the lane looks up key ``lane`` of the
+// tile (of 32: lanes 0-31 for its key scale, the others for its value scale).
+template <int T>
+struct TreeLookup {
+  const int32_t* table;
+  const uint64_t* wanted;
+  int c1, len, kh, lane;
+  bool pick;
+  int entry;        // page-table entry of the next tile's key
+  uint32_t rk, rv;  // scales on their way, as they lie in the cache
+  bool on;          // and whether there are any
+
+  __device__ __forceinline__ int page_of(const TreeParams& p, int t) const {
+    return (int)((uint64_t)(uint32_t)t * p.page_magic >> p.page_shift);
+  }
+  __device__ __forceinline__ int clamp(int t) const { return t < c1 ? t : (c1 > 0 ? c1 - 1 : 0); }
+  __device__ __forceinline__ void ask(const TreeParams& p, int t0) {
+    entry = table[page_of(p, clamp(t0 + (lane & (T - 1))))];
+  }
+  static __device__ __forceinline__ uint32_t bits(const TreeParams& p, const void* s, int64_t i) {
+    return p.scale_bf16 ? (uint32_t)reinterpret_cast<const uint16_t*>(s)[i] : reinterpret_cast<const uint32_t*>(s)[i];
+  }
+  // Pool row of the lane's key of the tile at t0 (0 where nothing is read), its
+  // scales' loads, and the entry for the tile at t1.
+  __device__ __forceinline__ int row(const TreeParams& p, int t0, int t1) {
+    const int t = t0 + (lane & (T - 1)), tc = clamp(t);
+    on = t < c1 && entry >= 0 && entry < p.pool_pages;
+    if (pick && t0 + T > len) {  // uniform over the wave
+      const int jj = t - len;
+      if (t < c1 && jj >= 0) on = on && (wanted[jj >> 6] >> (jj & 63) & 1);
+    }
+    const int r = on ? entry * p.page + (tc - page_of(p, tc) * p.page) : 0;
+    ask(p, t1);
+    const int64_t at = (int64_t)r * p.kvh + kh;
+    if (T == 32) {
+      rk = bits(p, lane < 32 ? p.ks : p.vs, at);
+    } else {
+      rk = bits(p, p.ks, at);
+      rv = bits(p, p.vs, at);
+    }
+    return r;
+  }
+};
+
+// Scales of a tile into the wave's LDS. The value scales are brought to at most
+// 2^6 by a power of two that falls as larger ones are met, so that probability x
+// scale keeps its 11 bits in FP16.
+template <int T>
+struct TreeScales {
+  float factor = 1.f, limit = -1.f;  // of the newest tile
+  __device__ __forceinline__ void put(const TreeParams& p, const TreeLookup<T>& at, float* sc) {
+    const auto value = [&](uint32_t bits) {
+      return at.on ? __builtin_bit_cast(float, p.scale_bf16 ? bits << 16 : bits) : 0.f;
+    };
+    const float k = value(at.rk), v = T == 32 ? k : value(at.rv);
+    const float a = (T == 64 || at.lane >= 32) && fabsf(v) < __builtin_inff() ? fabsf(v) : 0.f;
+    if (__any(a > limit)) {
+      const float x = tree_wave_reduce(a, [](float c, float d) { return fmaxf(c, d); });
+      int e = (int)(__builtin_bit_cast(uint32_t, x) >> 23) - 127;
+      e = e < -110 ? -110 : e;
+      factor = __builtin_bit_cast(float, (uint32_t)(127 + 3 - e) << 23);  // 2^(3-e): at most 2^4 now
+      limit = __builtin_bit_cast(float, (uint32_t)(127 + e + 3 > 254 ? 254 : 127 + e + 3) << 23);
+    }
+    if (T == 32) {
+      sc[at.lane] = at.lane < 32 ? k : v * factor;
+    } else {
+      sc[at.lane] = k;
+      sc[T + at.lane] = v * factor;
+    }
+    if (at.lane == 0) sc[2 * T] = factor;
+  }
+};
+
+// A row's softmax so far: maximum (log2), sum over the lane's keys, value factor.
+struct TreeState {
+  float m = kTreeFloor, l = 0.f, factor = 1.f;
+};
+
+// The maximum of 32 keys' scores, ``top``, and their value factor, taken into the
+// state; calls fade(f) where what was summed up to now is to be multiplied by f.
+// The maximum is raised only where a score passes it by 2^8, for the whole wave.
+template <typename F>
+__device__ __forceinline__ void tree_raise(TreeState& st, float top, float factor, F&& fade) {
+  factor = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, factor)));
+  if (__any(top > st.m + kTreeSlack) || factor != st.factor) {  // uniform over the wave
+    const float to = fmaxf(st.m, fmaxf(top, __shfl_xor(top, 32)));
+    const float f = __builtin_amdgcn_exp2f(st.m - to);
+    fade(f * (factor / st.factor));
+    st.factor = factor;
+    st.m = to;
+    st.l *= f;
+  }
+}
+
+// The rows of a workgroup: which query, and the bits of its channels.
+template <int D>
+struct TreeRow {
+  bool live;
+  int j, hh;
+  int e;      // exponent of the row's largest magnitude
+  bool bad;   // an infinite or NaN query: NaN scores
+  u32x4 raw[D / 32][2];
+  // Channels 32 s + 16 h + [0, 16) in raw[s] of half wave h, with ``kHalves`` 8 h' +
+  // [0, 8) of 16 channels in raw: the operands' order.
+  template <bool kBytes>
+  __device__ __forceinline__ void load(const TreeParams& p, const TreeItem& it, int row, int h) {
+    live = row < it.seq.count * p.r;
+    j = live ? row / p.r : 0;
+    hh = live ? row - j * p.r : 0;
+    const uint16_t* src = p.q + (int64_t)(it.seq.start + j) * p.q_stride + (int64_t)(it.kh * p.r + hh) * D;
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = kBytes ? 32 * s + 16 * h + 8 * i : 32 * s + 16 * i + 8 * h;
+        raw[s][i] = live ? *reinterpret_cast<const u32x4*>(src + c) : u32x4{0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t a = raw[s][i][w] & 0x7fffu, b = (raw[s][i][w] >> 16) & 0x7fffu;
+          top = top > a ? top : a;
+          top = top > b ? top : b;
+        }
+    const uint32_t other = __shfl_xor(top, 32);
+    top = top > other ? top : other;
+    bad = top >= 0x7f80u;
+    // the largest stays below 127 * 256 + 128 in steps of 2^(e-14)
+    e = (int)(top >> 7) - 127 + ((top & 0x7f) == 0x7f);
+    e = e < -110 ? -110 : e;  // smaller queries lose bits: scores below 2^-90
+  }
+  __device__ __forceinline__ float value(int s, int i, int k) const {  // k of 8
+    const uint32_t x = raw[s][i][k >> 1];
+    return __builtin_bit_cast(float, k & 1 ? x & 0xffff0000u : x << 16);
+  }
+};
+
+// Runs of a lane's sums whose channels lie together: each four become f(first channel, them).
+template <int D, typename A, typename F>
+__device__ __forceinline__ void tree_runs(A& acc, int h, F&& f) {
+  constexpr int kRun = D == 64 ? 4 : D / 32, kRuns = D / 2 / kRun;
+#pragma unroll
+  for (int q = 0; q < kRuns; ++q)
+#pragma unroll
+    for (int u = 0; u < kRun; u += 4) {
+      const int c = tree_channel<D>(0, q, h) + u;
+      if constexpr (D == 64) {
+        const f32x4 v = f(c, f32x4{acc[0][q], acc[1][q], acc[0][q + 8], acc[1][q + 8]});
+        acc[0][q] = v[0], acc[1][q] = v[1], acc[0][q + 8] = v[2], acc[1][q + 8] = v[3];
+      } else {
+        const f32x4 v = f(c, f32x4{acc[u][q], acc[u + 1][q], acc[u + 2][q], acc[u + 3][q]});
+        acc[u][q] = v[0], acc[u + 1][q] = v[1], acc[u + 2][q] = v[2], acc[u + 3][q] = v[3];
+      }
+    }
+}
+
+// A row's sums (of the values times the state's factor) to the workspace, or its output.
+template <int D, typename A>
+__device__ __forceinline__ void tree_result(const TreeParams& p, const TreeItem& it, A& acc, bool split, float m,
+                                            float l, int j, int hh, int place, int h) {
+  if (split) {
+    float* dst = p.part + (int64_t)place * D;
+    tree_runs<D>(acc, h, [&](int c, f32x4 v) { return *reinterpret_cast<f32x4*>(dst + c) = v; });
+    if (h == 0) *reinterpret_cast<f32x2*>(p.stat + 2 * (int64_t)place) = f32x2{m, l};
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* dst = p.out + ((int64_t)(it.seq.start + j) * p.hq + it.kh * p.r + hh) * D;
+  tree_runs<D>(acc, h, [&](int c, f32x4 v) {
+    *reinterpret_cast<u32x2*>(dst + c) = u32x2{pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv)};
+    return v;
+  });
+}
+
+// ---------------------------------------------------------------------------
+// Few rows. Queries are 16-bit integers in two INT8 operands, q = (256 hi + lo)
+// 2^(e-14): exact for values down to 2^-6 of the row's largest. So the INT8 codes
+// of the keys are matrix operands as they lie, and the sums are exact. The values'
+// codes + 128 enter the second product as FP16 subnormals, (code + 128) 2^-24, one
+// byte permutation per two of them; the 128 is taken back at the end with the sum
+// of the rounded probabilities.
+// ---------------------------------------------------------------------------
+template <int D>
+__global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_kernel(TreeParams p) {
+  using C = TreeThin<D>;
   constexpr int KS = D / 32;  // channel blocks of 32
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   TreeItem it;
   if (!tree_item<C::kRows, C::kStep>(p, it)) return;  // uniform over the workgroup
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int group = wave / RW, rw = wave % RW;
   const int col = lane & 31, h = lane >> 5;
   const TreeSeq seq = it.seq;
   int n, n_all;
@@ -241,121 +479,53 @@ __global__ void __launch_bounds__(kTreeThreads, D == 256 ? 1 : 2) tree_attn_kern
   const int c0 = it.chunk * it.keys;
   if (c0 > 0 && c0 >= n) return;
   const int c1 = n - c0 < it.keys ? n : c0 + it.keys;
-  const bool split = tree_chunks(n, it.keys) > 1;
+  const int turns = (c1 - c0 + C::kStep - 1) / C::kStep;
 
-  // New tokens that some row of the sequence sees. What the cache holds at the
-  // others' places (they may never have been written) is not read.
+  uint8_t* ring = smem + wave * (C::kStages * 2 * C::kHalf);
+  float* scales = reinterpret_cast<float*>(smem + C::kRing + wave * (C::kStages * C::kScale));
   uint64_t* wanted = reinterpret_cast<uint64_t*>(smem + C::kRing + 4 * C::kStages * C::kScale);
-  const bool pick = p.masks && c1 > seq.len;
-  if (pick) {
-    if (wave == 0)
-      for (int w = 0; w < p.words; ++w) {
-        uint64_t some = 0;
-        for (int i = lane; i < seq.count; i += 64) some |= p.masks[(int64_t)(seq.start + i) * p.words + w];
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) some |= __shfl_xor((unsigned long long)some, off);
-        if (lane == 0) wanted[w] = some;
-      }
+  TreeLookup<C::kTile> keys{p.table + (int64_t)it.b * p.pps, wanted, c1, seq.len, it.kh, lane,
+                            p.masks && c1 > seq.len, 0, 0, 0, false};
+  TreeScales<C::kTile> put;
+  const auto tile_at = [&](int i) { return c0 + (wave + 4 * i) * C::kTile; };
+  keys.ask(p, tile_at(0));
+  if (keys.pick) {
+    if (wave == 0) tree_wanted(p, seq, wanted);
     __syncthreads();
   }
-
-  // ---- the stream of key and value tiles --------------------------------
-  uint8_t* ring = smem + group * (C::kStages * 2 * C::kHalf);
-  float* scales = reinterpret_cast<float*>(smem + C::kRing + wave * (C::kStages * C::kScale));
-  const int turns = (c1 - c0 + C::kStep - 1) / C::kStep;
   const int64_t row_bytes = (int64_t)p.kvh * D;
   const int8_t* kbase = p.kc + (int64_t)it.kh * D;
   const int8_t* vbase = p.vc + (int64_t)it.kh * D;
-  const int32_t* trow = p.table + (int64_t)it.b * p.pps;
-  const int last = c1 > c0 ? c1 - 1 : 0;
-  const int tkey = lane & (C::kTile - 1);  // the key of a tile that this lane looks up
-  auto tile_at = [&](int i) { return c0 + (group + C::kGroups * i) * C::kTile; };
-  auto page_of = [&](int t) { return (int)((uint64_t)(uint32_t)t * p.page_magic >> p.page_shift); };
-  auto entry = [&](int i) {  // page-table entry of the lane's key in turn i's tile
-    const int t = tile_at(i) + tkey;
-    return trow[page_of(t < c1 ? t : last)];
-  };
-  int pg = entry(0);
-  uint32_t rk = 0, rv = 0;  // scales on their way, as they lie in the cache
-  bool ron = false;         // and whether there are any
-  auto scale_bits = [&](const void* s, int64_t i) {
-    return p.scale_bf16 ? (uint32_t)reinterpret_cast<const uint16_t*>(s)[i] : reinterpret_cast<const uint32_t*>(s)[i];
-  };
-  auto issue = [&](int i, int stage) {
-    const int t0 = tile_at(i), t = t0 + tkey;
-    ron = t < c1 && pg >= 0 && pg < p.pool_pages;
-    if (pick && t0 + C::kTile > seq.len) {  // uniform over the wave
-      const int jj = t - seq.len;
-      if (t < c1 && jj >= 0) ron = ron && (wanted[jj >> 6] >> (jj & 63) & 1);
-    }
-    const int tc = t < c1 ? t : last;
-    const int r = ron ? pg * p.page + (tc - page_of(tc) * p.page) : 0;
-    pg = entry(i + 1);
-    const int64_t at = (int64_t)r * p.kvh + it.kh;
-    if (C::kTile == 32) {  // lanes 0-31 load key scales, the others value scales
-      rk = scale_bits(h ? p.vs : p.ks, at);
-    } else {
-      rk = scale_bits(p.ks, at);
-      rv = scale_bits(p.vs, at);
-    }
+  const auto issue = [&](int i, int stage) {
+    const int r = keys.row(p, tile_at(i), tile_at(i + 1));
     uint8_t* st = ring + stage * 2 * C::kHalf;
 #pragma unroll
-    for (int d = 0; d < C::kDma; ++d) {
-      const int first = (rw * C::kDma + d) * 64;  // first 16-byte slot
-      const int line = (first + lane) / C::kChunks, slot = (first + lane) % C::kChunks;
+    for (int d = 0; d < KS; ++d) {  // 64 chunks of 16 bytes each
+      const int line = (64 * d + lane) / (D / 16), slot = (64 * d + lane) % (D / 16);
       const int64_t off = (int64_t)__shfl(r, tree_row(line)) * row_bytes;
-      const int8_t* k = kbase + off + 16 * (slot ^ tree_swizzle<C::kChunks>(line));
+      const int8_t* k = kbase + off + 16 * (slot ^ tree_swizzle<D>(line));
       const int8_t* v = vbase + off + 16 * slot;
-      __builtin_amdgcn_global_load_lds(k, LDS_PTR(st + first * 16), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(v, LDS_PTR(st + C::kHalf + first * 16), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(k, LDS_PTR(st + 1024 * d), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(v, LDS_PTR(st + C::kHalf + 1024 * d), 16, 0, 0);
     }
   };
   issue(0, 0);
 
-  // The lane's row of the tile: query (new token j, head hh of the group), held
-  // as 16-bit integers in two INT8 operands q = (256 hi + lo) 2^(e-14), e the
-  // exponent of the row's largest value: exact for values down to 2^-6 of it.
-  const int row = it.tile * C::kRows + rw * 32 + col;
-  const bool live = row < seq.count * p.r;
-  const int j = live ? row / p.r : 0, hh = live ? row - j * p.r : 0;
+  TreeRow<D> row;
+  row.template load<true>(p, it, it.tile * C::kRows + col, h);
   i32x4 qhi[KS], qlo[KS];
-  float qf;
   {
-    const uint16_t* src = p.q + (int64_t)(seq.start + j) * p.q_stride + (int64_t)(it.kh * p.r + hh) * D + 16 * h;
-    uint32_t top = 0;  // the largest magnitude's bits
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const u32x4 x = live ? *reinterpret_cast<const u32x4*>(src + 32 * s + 8 * e) : u32x4{0u, 0u, 0u, 0u};
-        i32x4& keep = e ? qlo[s] : qhi[s];
-        keep = __builtin_bit_cast(i32x4, x);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t a = x[w] & 0x7fffu, b = (x[w] >> 16) & 0x7fffu;
-          top = top > a ? top : a;
-          top = top > b ? top : b;
-        }
-      }
-    const uint32_t other = __shfl_xor(top, 32);
-    top = top > other ? top : other;
-    int e = (int)(top >> 7) - 127 + ((top & 0x7f) == 0x7f);  // the largest stays below 127 * 256 + 128
-    e = e < -110 ? -110 : e;  // smaller queries lose bits: scores below 2^-90
     // v = q 2^(14-e) rounded into the low bits of 1.5 * 2^23 + v; its low byte is lo,
     // the second byte of v + 128 is hi
-    const float up = __builtin_ldexpf(1.f, 14 - e);
+    const float up = __builtin_ldexpf(1.f, 14 - row.e);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const i32x4 raw[2] = {qhi[s], qlo[s]};
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         uint32_t v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t x = (uint32_t)raw[w >> 1][(2 * w + (i >> 1)) & 3];
-          const float f = __builtin_bit_cast(float, i & 1 ? x & 0xffff0000u : x << 16);
-          v[i] = __builtin_bit_cast(uint32_t, __builtin_fmaf(f, up, 12582912.f));
-        }
+        for (int i = 0; i < 4; ++i)
+          v[i] = __builtin_bit_cast(uint32_t, __builtin_fmaf(row.value(s, w >> 1, 4 * (w & 1) + i), up, 12582912.f));
         const uint32_t l01 = __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0400u);
         const uint32_t l23 = __builtin_amdgcn_perm(v[3], v[2], 0x04000c0cu);
         const uint32_t h01 = __builtin_amdgcn_perm(v[1] + 128, v[0] + 128, 0x0c0c0501u);
@@ -363,302 +533,397 @@ __global__ void __launch_bounds__(kTreeThreads, D == 256 ? 1 : 2) tree_attn_kern
         qhi[s][w] = (int)(h01 | h23);
         qlo[s][w] = (int)(l01 | l23);
       }
-    }
-    qf = __builtin_ldexpf(p.to_log2, e - 14);
-    if (top >= 0x7f80u) qf = __builtin_nanf("");  // an infinite or NaN query: NaN scores
   }
+  const float qf = row.bad ? __builtin_nanf("") : __builtin_ldexpf(p.to_log2, row.e - 14);
 
   f32x16 acc[KS];
 #pragma unroll
   for (int c = 0; c < KS; ++c)
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[c][v] = 0.f;
-  float m = kTreeFloor, l = 0.f, psum = 0.f;
-  float vfac = 1.f, vfac_new = 1.f, vtop = -1.f;  // value factor in use, of the newest tile, and its limit
-
-  // Scales of the tile issued a turn ago into the wave's LDS. The value scales are
-  // brought to at most 2^6 by a power of two that falls as larger ones are met, so
-  // that probability x scale keeps its 11 bits in FP16.
-  auto put_scales = [&](int stage) {
-    float* sc = scales + stage * (C::kScale / 4);
-    auto value = [&](uint32_t bits) {
-      return ron ? __builtin_bit_cast(float, p.scale_bf16 ? bits << 16 : bits) : 0.f;
-    };
-    const float k = value(rk), v = C::kTile == 32 ? k : value(rv);
-    const float a = (C::kTile == 64 || h) && fabsf(v) < __builtin_inff() ? fabsf(v) : 0.f;
-    if (__any(a > vtop)) {
-      float x = a;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) x = fmaxf(x, __shfl_xor(x, off));
-      int e = (int)(__builtin_bit_cast(uint32_t, x) >> 23) - 127;
-      e = e < -110 ? -110 : e;
-      vfac_new = __builtin_bit_cast(float, (uint32_t)(127 + 3 - e) << 23);  // 2^(3-e): at most 2^4 now
-      vtop = __builtin_bit_cast(float, (uint32_t)(127 + e + 3 > 254 ? 254 : 127 + e + 3) << 23);
-    }
-    if (C::kTile == 32) {
-      sc[lane] = h ? v * vfac_new : k;
-    } else {
-      sc[lane] = k;
-      sc[64 + lane] = v * vfac_new;
-    }
-    if (lane == 0) sc[128] = vfac_new;
-  };
+  TreeState st;
+  float psum = 0.f;  // of the rounded probabilities times the value scales
 
   const int krow = tree_row(col);
-  const uint32_t koff = krow * D, ksw = tree_swizzle<C::kChunks>(krow);
+  const uint32_t koff = krow * D, ksw = tree_swizzle<D>(krow);
   const uint32_t voff = h * D + (D == 64 ? 4 * (col & 15) : D / 32 * col);
   const uint32_t vsel = D == 64 ? (uint32_t)(col >> 4) * 0x00020002u : 0u;  // the lane's channels of its 4
-  auto compute = [&](auto slow, int t0, int stage) {
-    const uint8_t* kt = ring + stage * 2 * C::kHalf;
-    const uint8_t* vt = kt + C::kHalf + voff;
+  // The wave's 32 keys of a turn: scores, probabilities, values.
+  const auto compute = [&](auto slow, int t0, int stage) {
+    const uint8_t* kt = ring + stage * 2 * C::kHalf + koff;
+    const uint8_t* vt = ring + stage * 2 * C::kHalf + C::kHalf + voff;
     const float* sc = scales + stage * (C::kScale / 4) + 4 * h;
-    float t[C::kBlocks][16];
-    float top = -__builtin_inff();
-    uint32_t vis[C::kBlocks];
+    i32x16 hi, lo;
 #pragma unroll
-    for (int nb = 0; nb < C::kBlocks; ++nb) {
-      i32x16 hi, lo;
+    for (int v = 0; v < 16; ++v) hi[v] = lo[v] = 0;
 #pragma unroll
-      for (int v = 0; v < 16; ++v) hi[v] = lo[v] = 0;
+    for (int s = 0; s < KS; ++s) {
+      const i32x4 a = *reinterpret_cast<const i32x4*>(kt + 16 * ((2 * s + h) ^ ksw));
+      hi = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qhi[s], hi, 0, 0, 0);
+      lo = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qlo[s], lo, 0, 0, 0);
+    }
+    uint32_t vis = 0;
+    if constexpr (slow) vis = row.live ? tree_visible(p, seq, row.j, t0, c1, h) : 0u;
+    float t[16], top = -__builtin_inff();
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const i32x4 a = *reinterpret_cast<const i32x4*>(kt + 32 * nb * D + koff + 16 * ((2 * s + h) ^ ksw));
-        hi = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qhi[s], hi, 0, 0, 0);
-        lo = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qlo[s], lo, 0, 0, 0);
-      }
-      if constexpr (slow) {
-        // bit i: the lane's row sees key t0 + 32 nb + i; then moved to the half wave's keys
-        const int k0 = t0 + 32 * nb, jj = k0 - seq.len;
-        uint32_t on = 0;
-        if (p.masks) {
-          const uint64_t* w = p.masks + (int64_t)(seq.start + j) * p.words;
-          if (jj >= 0) {
-            const int at = jj >> 6, sh = jj & 63;
-            const uint64_t a = at < p.words ? w[at] : 0, b = at + 1 < p.words ? w[at + 1] : 0;
-            on = (uint32_t)(a >> sh | (b << 1) << (63 - sh));
-          } else if (jj > -32) {
-            on = (uint32_t)(w[0] << -jj) | ((1u << -jj) - 1);
-          } else {
-            on = ~0u;
-          }
-        } else {
-          const int seen = j + 1 - jj;  // keys of the block up to the row's own
-          on = seen >= 32 ? ~0u : (seen <= 0 ? 0u : (1u << seen) - 1);
-        }
-        const int left = c1 - k0;
-        if (left < 32) on &= left <= 0 ? 0u : (1u << left) - 1;
-        vis[nb] = live ? on >> (4 * h) : 0u;
-      }
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 ksv = *reinterpret_cast<const f32x4*>(sc + 8 * g);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 ksv = *reinterpret_cast<const f32x4*>(sc + 32 * nb + 8 * g);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int v = 4 * g + u;
-          t[nb][v] = (float)((hi[v] << 8) + lo[v]) * ksv[u];
-          if constexpr (slow) t[nb][v] = vis[nb] >> (8 * g + u) & 1 ? t[nb][v] : -__builtin_inff();
-          top = fmaxf(top, t[nb][v]);
-        }
+      for (int u = 0; u < 4; ++u) {
+        const int v = 4 * g + u;
+        t[v] = (float)((hi[v] << 8) + lo[v]) * ksv[u];
+        if constexpr (slow) t[v] = vis >> (8 * g + u) & 1 ? t[v] : -__builtin_inff();
+        top = fmaxf(top, t[v]);
       }
     }
-    top *= qf;
-    const float vf = __builtin_bit_cast(
-        float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sc[128 - 4 * h])));
-    if (__any(top > m + kTreeSlack) || vf != vfac) {  // uniform over the wave
-      const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
-      const float fade_l = __builtin_amdgcn_exp2f(m - to), fade = fade_l * (vf / vfac);
-      vfac = vf;
-      m = to;
-      l *= fade_l;
-      psum *= fade;
+    tree_raise(st, top * qf, sc[64 - 4 * h], [&](float f) {
+      psum *= f;
 #pragma unroll
       for (int c = 0; c < KS; ++c)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) acc[c][v] *= fade;
-    }
+        for (int v = 0; v < 16; ++v) acc[c][v] *= f;
+    });
 #pragma unroll
-    for (int nb = 0; nb < C::kBlocks; ++nb)
+    for (int mm = 0; mm < 2; ++mm) {  // 16 keys: 8 of each half wave
+      f16x8 pv;
 #pragma unroll
-      for (int mm = 0; mm < 2; ++mm) {  // 16 keys: 8 of each half wave
-        f16x8 pv;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const f32x4 vsv = *reinterpret_cast<const f32x4*>(sc + (C::kTile == 32 ? 32 : 64) + 32 * nb + 16 * mm + 8 * g);
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int v = 8 * mm + 4 * g + u;
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(t[nb][v], qf, -m));
-            float w = e * vsv[u];
-            if constexpr (slow) {
-              const bool on = vis[nb] >> (16 * mm + 8 * g + u) & 1;
-              l += on ? e : 0.f;
-              w = on ? w : 0.f;
-            } else {
-              l += e;
-            }
-            pv[4 * g + u] = (_Float16)w;
-          }
-        }
+      for (int g = 0; g < 2; ++g) {
+        const f32x4 vsv = *reinterpret_cast<const f32x4*>(sc + 32 + 16 * mm + 8 * g);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const f16x2 one = {(_Float16)1.f, (_Float16)1.f}, pair = {pv[2 * u], pv[2 * u + 1]};
-          psum = __builtin_amdgcn_fdot2(pair, one, psum, false);
-        }
-        // Values: the lane's channels of its half wave's 8 keys; byte b of two keys
-        // makes one operand word. Code + 128 enters as an FP16 subnormal, (code + 128)
-        // 2^-24: the 128 is taken back at the end with the sum of the rounded
-        // probabilities.
-        constexpr int W = D == 256 ? 2 : 1;
-        uint32_t x[8][W];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint8_t* src = vt + (32 * nb + 16 * mm + tree_row(8 * (i >> 2) + (i & 3))) * D;
-          if constexpr (W == 2) {
-            const u32x2 y = *reinterpret_cast<const u32x2*>(src);
-            x[i][0] = y[0] ^ 0x80808080u;
-            x[i][1] = y[1] ^ 0x80808080u;
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(t[8 * mm + 4 * g + u], qf, -st.m));
+          float w = e * vsv[u];
+          if constexpr (slow) {
+            const bool on = vis >> (16 * mm + 8 * g + u) & 1;
+            st.l += on ? e : 0.f;
+            w = on ? w : 0.f;
           } else {
-            x[i][0] = *reinterpret_cast<const uint32_t*>(src) ^ 0x80808080u;
+            st.l += e;
           }
-        }
-#pragma unroll
-        for (int c = 0; c < KS; ++c) {
-          u32x4 a;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            a[q] = __builtin_amdgcn_perm(x[2 * q + 1][c >> 2], x[2 * q][c >> 2],
-                                         0x0c040c00u + (uint32_t)(c & 3) * 0x00010001u + vsel);
-          acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), pv, acc[c], 0, 0, 0);
+          pv[4 * g + u] = (_Float16)w;
         }
       }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const f16x2 one = {(_Float16)1.f, (_Float16)1.f}, pair = {pv[2 * u], pv[2 * u + 1]};
+        psum = __builtin_amdgcn_fdot2(pair, one, psum, false);
+      }
+      // the lane's channels of its half wave's 8 keys; byte b of two keys makes one
+      // operand word
+      constexpr int W = D == 256 ? 2 : 1;
+      uint32_t x[8][W];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint8_t* src = vt + (16 * mm + tree_row(8 * (i >> 2) + (i & 3))) * D;
+        if constexpr (W == 2) {
+          const u32x2 y = *reinterpret_cast<const u32x2*>(src);
+          x[i][0] = y[0] ^ 0x80808080u;
+          x[i][1] = y[1] ^ 0x80808080u;
+        } else {
+          x[i][0] = *reinterpret_cast<const uint32_t*>(src) ^ 0x80808080u;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < KS; ++c) {
+        u32x4 a;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          a[q] = __builtin_amdgcn_perm(x[2 * q + 1][c >> 2], x[2 * q][c >> 2],
+                                       0x0c040c00u + (uint32_t)(c & 3) * 0x00010001u + vsel);
+        acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), pv, acc[c], 0, 0, 0);
+      }
+    }
   };
 
   // Turn i issues the tile of turn i + kStages - 1; its scales reach LDS a turn
   // later. Waits count DMA instructions: those of the tiles after this one may
-  // still be in flight.
+  // still be in flight. The waves work apart.
 #pragma unroll
   for (int i = 1; i < C::kStages - 1; ++i) {
-    put_scales(i - 1);
+    put.put(p, keys, scales + (i - 1) * (C::kScale / 4));
     issue(i, i);
   }
   int stage = 0;
-  auto advance = [&](int i) {
-    tree_wait_vm<(C::kStages - 2) * 2 * C::kDma>();
-    // the wave's reads of the stage that is written next have returned
-    if (RW > 1)
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    else
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    const int next = stage == 0 ? C::kStages - 1 : stage - 1;
-    put_scales(C::kStages == 2 ? stage : (stage + 1 == C::kStages ? 0 : stage + 1));
-    issue(i + C::kStages - 1, next);
+  const auto advance = [&](int i) {
+    tree_wait_vm<(C::kStages - 2) * 2 * KS>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // reads of the stage that is written next
+    put.put(p, keys, scales + (C::kStages == 2 ? stage : (stage + 1) % C::kStages) * (C::kScale / 4));
+    issue(i + C::kStages - 1, (stage + C::kStages - 1) % C::kStages);
   };
   // first the turns whose tile every row sees whole
   const int open = (n_all < c1 ? n_all : c1) - tile_at(0);
-  int fast = open / C::kTile > 0 ? (open / C::kTile - 1) / C::kGroups + 1 : 0;
+  int fast = open >= C::kTile ? (open / C::kTile - 1) / 4 + 1 : 0;
   fast = fast < turns ? fast : turns;
   int i = 0;
   for (; i < fast; ++i) {
     advance(i);
     compute(std::false_type{}, 0, stage);
-    stage = stage + 1 == C::kStages ? 0 : stage + 1;
+    stage = (stage + 1) % C::kStages;
   }
   for (; i < turns; ++i) {
     advance(i);
     compute(std::true_type{}, tile_at(i), stage);
-    stage = stage + 1 == C::kStages ? 0 : stage + 1;
+    stage = (stage + 1) % C::kStages;
   }
   tree_wait_vm<0>();
 
-  // ---- the row's result -------------------------------------------------
   // Both half waves hold half of a row's keys in l and psum.
-  l += __shfl_xor(l, 32);
+  float l = st.l + __shfl_xor(st.l, 32), m = st.m;
   psum += __shfl_xor(psum, 32);
-  const float up = 0x1p24f / vfac, shift = 128.f * psum * 0x1p-24f;
+  // The waves' sums meet in LDS: each brings its own to the common maximum.
+  __syncthreads();
+  float* stats = reinterpret_cast<float*>(smem);  // [wave][row]: maximum, sum
+  float* sum = stats + 2 * 4 * C::kRows;          // [row][D + 4], one wave at a time
+  if (h == 0) {
+    stats[2 * (wave * C::kRows + col)] = m;
+    stats[2 * (wave * C::kRows + col) + 1] = l;
+  }
+  __syncthreads();
+  float to = kTreeFloor, all = 0.f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) to = fmaxf(to, stats[2 * (g * C::kRows + col)]);
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    all += stats[2 * (g * C::kRows + col) + 1] * __builtin_amdgcn_exp2f(stats[2 * (g * C::kRows + col)] - to);
+  const float up = __builtin_amdgcn_exp2f(m - to) * (0x1p24f / st.factor), shift = 128.f * psum * 0x1p-24f;
 #pragma unroll
   for (int c = 0; c < KS; ++c)
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[c][v] = (acc[c][v] - shift) * up;
-  // Channels q * kRun + [0, kRun) of a lane's sums lie together.
-  constexpr int kRun = D == 64 ? 4 : KS, kRuns = KS * 16 / kRun;
-  auto at_run = [&](int q) { return tree_channel<D>(0, q, h); };
-  auto of_run = [&](int q, int u) { return D == 64 ? acc[u & 1][q + 8 * (u >> 1)] : acc[D == 64 ? 0 : u][q]; };
-  auto set_run = [&](int q, int u, float v) {
-    if constexpr (D == 64)
-      acc[u & 1][q + 8 * (u >> 1)] = v;
-    else
-      acc[u][q] = v;
+  for (int g = 3; g >= 0; --g) {
+    if (wave == g)
+      tree_runs<D>(acc, h, [&](int c, f32x4 v) {
+        f32x4* at = reinterpret_cast<f32x4*>(sum + col * (D + 4) + c);
+        if (g < 3) v += *at;
+        return *at = v;
+      });
+    __syncthreads();
+  }
+  if (wave == 0 && row.live)
+    tree_result<D>(p, it, acc, tree_chunks(n, it.keys) > 1, to, all, row.j, row.hh, it.id * C::kRows + col, h);
+}
+
+// ---------------------------------------------------------------------------
+// Many rows. The four waves bring a tile's codes to FP16 together, (code) 2^-24,
+// exact, in the order of the matrix operands; each then works on its 32 rows.
+// Queries are FP16 too, scaled by a power of two: exact for values down to 2^-28
+// of the row's largest. A conversion by each wave for itself took a third of the
+// vector instructions; with it two workgroups shared a CU, now three.
+// ---------------------------------------------------------------------------
+template <int D>
+__global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_kernel(TreeParams p) {
+  using C = TreeWide<D>;
+  constexpr int KS = D / 32, T = C::kTile;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  TreeItem it;
+  if (!tree_item<C::kRows, C::kStep>(p, it)) return;  // uniform over the workgroup
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  const TreeSeq seq = it.seq;
+  int n, n_all;
+  tree_reach(p, seq, it.tile, C::kRows, &n, &n_all);
+  const int c0 = it.chunk * it.keys;
+  if (c0 > 0 && c0 >= n) return;
+  const int c1 = n - c0 < it.keys ? n : c0 + it.keys;
+  const int turns = (c1 - c0 + T - 1) / T;
+
+  uint8_t* kr = smem;                  // the codes as they lie in the cache
+  uint8_t* vr = kr + C::kHalf;
+  uint8_t* kf = vr + C::kHalf;         // [16-channel step][half][key] x 8 channels
+  uint8_t* vf = kf + 2 * C::kHalf;     // [16 keys][half][channel block][row] x 8 keys
+  float* scales = reinterpret_cast<float*>(vf + 2 * C::kHalf + wave * C::kScale);
+  uint64_t* wanted = reinterpret_cast<uint64_t*>(vf + 2 * C::kHalf + 4 * C::kScale);
+  TreeLookup<T> keys{p.table + (int64_t)it.b * p.pps, wanted, c1, seq.len, it.kh, lane, p.masks && c1 > seq.len,
+                     0, 0, 0, false};
+  TreeScales<T> put;
+  const auto tile_at = [&](int i) { return c0 + i * T; };
+  keys.ask(p, tile_at(0));
+  if (keys.pick) {
+    if (wave == 0) tree_wanted(p, seq, wanted);
+    __syncthreads();
+  }
+  const int64_t row_bytes = (int64_t)p.kvh * D;
+  const int8_t* kbase = p.kc + (int64_t)it.kh * D;
+  const int8_t* vbase = p.vc + (int64_t)it.kh * D;
+  constexpr int kDma = C::kHalf / 4096;  // DMA instructions per wave for keys, and for values
+  const auto issue = [&](int i) {
+    const int r = keys.row(p, tile_at(i), tile_at(i + 1));
+#pragma unroll
+    for (int d = 0; d < kDma; ++d) {
+      const int first = 64 * (wave * kDma + d);  // chunks of 16 bytes
+      const int line = (first + lane) / (D / 16), slot = (first + lane) % (D / 16);
+      const int64_t off = (int64_t)__shfl(r, tree_row(line)) * row_bytes;
+      const int8_t* k = kbase + off + 16 * (slot ^ tree_swizzle<D>(line));
+      const int8_t* v = vbase + off + 16 * slot;
+      __builtin_amdgcn_global_load_lds(k, LDS_PTR(kr + 16 * first), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(v, LDS_PTR(vr + 16 * first), 16, 0, 0);
+    }
   };
-  if constexpr (C::kGroups > 1) {
-    // the groups' sums meet in LDS, in group order
-    __syncthreads();
-    float* st = reinterpret_cast<float*>(smem);   // [group][row]: maximum, sum
-    float* sum = st + 2 * C::kGroups * C::kRows;  // [row][D], one group at a time
-    const int rr = rw * 32 + col;
-    if (h == 0) {
-      st[2 * (group * C::kRows + rr)] = m;
-      st[2 * (group * C::kRows + rr) + 1] = l;
+  issue(0);
+
+  TreeRow<D> row;
+  row.template load<false>(p, it, it.tile * C::kRows + wave * 32 + col, h);
+  f16x8 q[KS][2];
+  {
+    const float up = __builtin_ldexpf(1.f, 14 - row.e);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) q[s][i][k] = (_Float16)(row.value(s, i, k) * up);
+  }
+  const float qf = row.bad ? __builtin_nanf("") : __builtin_ldexpf(p.to_log2, row.e + 10);
+  const bool rows = it.tile * C::kRows + wave * 32 < seq.count * p.r;  // the wave has any
+
+  f32x16 acc[KS];
+#pragma unroll
+  for (int c = 0; c < KS; ++c)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[c][v] = 0.f;
+  TreeState st;
+
+  // The tile's codes into FP16: a key's 16 channels per thread and turn, then four
+  // keys' D / 32 channels (of D = 64: 4). Code + 128 as a subnormal, less 128.
+  const f16x2 bias = __builtin_bit_cast(f16x2, 0x80808080u);  // -128 2^-24 each
+  const auto half2 = [&](uint32_t hi, uint32_t lo, uint32_t sel) {
+    return __builtin_bit_cast(uint32_t, (f16x2)(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(hi, lo, sel)) + bias));
+  };
+  const int tid = threadIdx.x;
+  const auto convert = [&]() {
+#pragma unroll
+    for (int i = 0; i < C::kHalf / 4096; ++i) {
+      const int key = tid % T, chunk = tid / T + i * (kTreeThreads / T);
+      const int line = tree_row(key);
+      u32x4 x = *reinterpret_cast<const u32x4*>(kr + line * D + 16 * (chunk ^ tree_swizzle<D>(line)));
+      u32x4 y[2];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t u = x[w] ^ 0x80808080u;
+        y[w >> 1][2 * (w & 1)] = half2(u, u, 0x0c010c00u);
+        y[w >> 1][2 * (w & 1) + 1] = half2(u, u, 0x0c030c02u);
+      }
+      *reinterpret_cast<u32x4*>(kf + 16 * ((2 * chunk) * T + key)) = y[0];
+      *reinterpret_cast<u32x4*>(kf + 16 * ((2 * chunk + 1) * T + key)) = y[1];
     }
-    __syncthreads();
-    float to = kTreeFloor, all = 0.f;
+    constexpr int kLanes = D == 64 ? 16 : 32, W = D == 256 ? 2 : 1;
+    const int quad = tid % kLanes;
 #pragma unroll
-    for (int g = 0; g < C::kGroups; ++g) to = fmaxf(to, st[2 * (g * C::kRows + rr)]);
+    for (int k = 0; k < T / 4 * kLanes / kTreeThreads; ++k) {
+    const int four = tid / kLanes + k * (kTreeThreads / kLanes);  // keys 4 four + [0, 4)
+    uint32_t x[4][W];
 #pragma unroll
-    for (int g = 0; g < C::kGroups; ++g)
-      all += st[2 * (g * C::kRows + rr) + 1] * __builtin_amdgcn_exp2f(st[2 * (g * C::kRows + rr)] - to);
-    const float fade = __builtin_amdgcn_exp2f(m - to);
+    for (int i = 0; i < 4; ++i) {
+      const uint8_t* src = vr + tree_row(4 * four + i) * D + 4 * W * quad;
+      if constexpr (W == 2) {
+        const u32x2 y = *reinterpret_cast<const u32x2*>(src);
+        x[i][0] = y[0] ^ 0x80808080u;
+        x[i][1] = y[1] ^ 0x80808080u;
+      } else {
+        x[i][0] = *reinterpret_cast<const uint32_t*>(src) ^ 0x80808080u;
+      }
+    }
+    // keys 4 four + i: 16 keys' block four / 4, half wave four & 1, operand place 4 (four / 2 & 1) + i
+    uint8_t* dst = vf + 16 * ((four >> 2) * 2 + (four & 1)) * KS * 32 + 8 * (four >> 1 & 1);
 #pragma unroll
-    for (int c = 0; c < KS; ++c)
+    for (int b = 0; b < 4 * W; ++b) {
+      const uint32_t sel = 0x0c040c00u + (uint32_t)(b & 3) * 0x00010001u;
+      const u32x2 y = {half2(x[1][b >> 2], x[0][b >> 2], sel), half2(x[3][b >> 2], x[2][b >> 2], sel)};
+      const int c = D == 64 ? b & 1 : b, r = D == 64 ? quad + 16 * (b >> 1) : quad;
+      *reinterpret_cast<u32x2*>(dst + 16 * (c * 32 + r)) = y;
+    }
+    }
+  };
+  const auto compute = [&](auto slow, int t0) {
+    const uint8_t* kt = kf + 16 * (h * T + col);
+    const uint8_t* vt = vf + 16 * (h * KS * 32 + col);
+    const float* sc = scales + 4 * h;
 #pragma unroll
-      for (int v = 0; v < 16; ++v) acc[c][v] *= fade;
-    for (int g = C::kGroups - 1; g >= 0; --g) {
-      if (group == g) {
+    for (int nb = 0; nb < T / 32; ++nb) {
+      f32x16 s;
 #pragma unroll
-        for (int q = 0; q < kRuns; ++q)
+      for (int v = 0; v < 16; ++v) s[v] = 0.f;
 #pragma unroll
-          for (int u = 0; u < kRun; u += 4) {
-            f32x4* at = reinterpret_cast<f32x4*>(sum + rr * (D + 4) + at_run(q) + u);
-            f32x4 v = {of_run(q, u), of_run(q, u + 1), of_run(q, u + 2), of_run(q, u + 3)};
-            if (g < C::kGroups - 1) v += *at;
-            *at = v;
+      for (int k = 0; k < 2 * KS; ++k)
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(kt + 16 * (2 * k * T + 32 * nb)),
+                                                   q[k >> 1][k & 1], s, 0, 0, 0);
+      uint32_t vis = 0;
+      if constexpr (slow) vis = row.live ? tree_visible(p, seq, row.j, t0 + 32 * nb, c1, h) : 0u;
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 ksv = *reinterpret_cast<const f32x4*>(sc + 32 * nb + 8 * g);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          s[4 * g + u] *= ksv[u];
+          if constexpr (slow) s[4 * g + u] = vis >> (8 * g + u) & 1 ? s[4 * g + u] : -__builtin_inff();
+          top = fmaxf(top, s[4 * g + u]);
+        }
+      }
+      tree_raise(st, top * qf, sc[2 * T - 4 * h], [&](float f) {
+#pragma unroll
+        for (int c = 0; c < KS; ++c)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) acc[c][v] *= f;
+      });
+#pragma unroll
+      for (int mm = 0; mm < 2; ++mm) {
+        f16x8 pv;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const f32x4 vsv = *reinterpret_cast<const f32x4*>(sc + T + 32 * nb + 16 * mm + 8 * g);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * mm + 4 * g + u], qf, -st.m));
+            float w = e * vsv[u];
+            if constexpr (slow) {
+              const bool on = vis >> (16 * mm + 8 * g + u) & 1;
+              st.l += on ? e : 0.f;
+              w = on ? w : 0.f;
+            } else {
+              st.l += e;
+            }
+            pv[4 * g + u] = (_Float16)w;
           }
+        }
+#pragma unroll
+        for (int c = 0; c < KS; ++c)
+          acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+              *reinterpret_cast<const f16x8*>(vt + 16 * (((2 * nb + mm) * 2 * KS + c) * 32)), pv, acc[c], 0, 0, 0);
       }
-      __syncthreads();
     }
-    if (group > 0) return;
-#pragma unroll
-    for (int q = 0; q < kRuns; ++q)
-#pragma unroll
-      for (int u = 0; u < kRun; u += 4) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(sum + rr * (D + 4) + at_run(q) + u);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) set_run(q, u + w, v[w]);
-      }
-    m = to;
-    l = all;
+  };
+
+  // Turn i: the tile's DMA has landed; all waves convert it, issue the next tile
+  // into its place, and compute.
+  const auto advance = [&](int i) {
+    tree_wait_vm<0>();
+    put.put(p, keys, scales);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    convert();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    issue(i + 1);
+  };
+  const int open = (n_all < c1 ? n_all : c1) - c0;
+  const int fast = open >= T ? (open / T < turns ? open / T : turns) : 0;
+  int i = 0;
+  for (; i < fast; ++i) {
+    advance(i);
+    if (rows) compute(std::false_type{}, 0);
   }
-  if (!live) return;
-  if (split) {
-    const int64_t at = (int64_t)blockIdx.x * C::kRows + rw * 32 + col;
-    float* dst = p.part + at * D;
-#pragma unroll
-    for (int q = 0; q < kRuns; ++q)
-#pragma unroll
-      for (int u = 0; u < kRun; u += 4)
-        *reinterpret_cast<f32x4*>(dst + at_run(q) + u) =
-            f32x4{of_run(q, u), of_run(q, u + 1), of_run(q, u + 2), of_run(q, u + 3)};
-    if (h == 0) *reinterpret_cast<f32x2*>(p.stat + 2 * at) = f32x2{m, l};
-    return;
+  for (; i < turns; ++i) {
+    advance(i);
+    if (rows) compute(std::true_type{}, tile_at(i));
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t* dst = p.out + ((int64_t)(seq.start + j) * p.hq + it.kh * p.r + hh) * D;
+  tree_wait_vm<0>();
+  const float l = st.l + __shfl_xor(st.l, 32), up = 0x1p24f / st.factor;
 #pragma unroll
-  for (int q = 0; q < kRuns; ++q)
+  for (int c = 0; c < KS; ++c)
 #pragma unroll
-    for (int u = 0; u < kRun; u += 4)
-      *reinterpret_cast<u32x2*>(dst + at_run(q) + u) =
-          u32x2{pack_bf16x2(of_run(q, u) * inv, of_run(q, u + 1) * inv),
-                pack_bf16x2(of_run(q, u + 2) * inv, of_run(q, u + 3) * inv)};
+    for (int v = 0; v < 16; ++v) acc[c][v] *= up;
+  if (row.live)
+    tree_result<D>(p, it, acc, tree_chunks(n, it.keys) > 1, st.m, l, row.j, row.hh,
+                   it.id * C::kRows + wave * 32 + col, h);
 }
 
 // The chunks' sums of a row and head joined in chunk order, D / 4 lanes of four
@@ -731,25 +996,29 @@ __global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p
 constexpr int kTreeCus = 256;
 
 struct TreeLayout {
-  int row_waves;  // waves of a workgroup with rows of their own
+  int wide;
   int slots, whole;
-  int64_t grid;   // at most so many workgroups have work
+  int64_t grid;  // at most so many workgroups have work
   size_t info, stat, part, total;
 };
 
 static size_t tree_align(size_t v) { return (v + 255) & ~(size_t)255; }
 
+template <int D>
+static int tree_per_cu(bool wide) { return wide ? TreeWide<D>::kPerCu : TreeThin<D>::kPerCu; }
+
 static TreeLayout tree_layout(int64_t batch, int64_t rows, int64_t max_count, int64_t hq, int64_t kvh, int64_t dim) {
   TreeLayout L;
   const int64_t r = hq / kvh;
-  L.row_waves = max_count * r <= 32 ? 1 : (max_count * r <= 64 ? 2 : 4);
-  const int64_t tile = 32 * L.row_waves;
+  L.wide = max_count * r > TreeThin<128>::kRows;
+  const int64_t tile = L.wide ? TreeWide<128>::kRows : TreeThin<128>::kRows;
   // row tiles of all sequences together: each ends with one that is not full
   const int64_t by_batch = batch * cdiv(max_count * r, tile), by_rows = rows * r / tile + batch;
   const int64_t units = kvh * (by_batch < by_rows ? by_batch : by_rows);
-  L.slots = kTreeCus * (dim == 256 ? TreeCfg<256, 1>::kPerCu : TreeCfg<128, 1>::kPerCu);
+  L.slots = kTreeCus * (dim == 64 ? tree_per_cu<64>(L.wide) : (dim == 128 ? tree_per_cu<128>(L.wide) : tree_per_cu<256>(L.wide)));
   L.whole = units >= 4 * L.slots;
   L.grid = L.whole ? units : (2 * units <= L.slots ? L.slots : units + 2 * L.slots);
+  L.grid = cdiv(L.grid, 8) * 8;  // whole runs per XCD
   const int64_t parts = L.whole ? 0 : L.grid * tile;
   L.info = 0;
   L.stat = tree_align(L.info + (size_t)(batch + 1) * 4);
@@ -758,25 +1027,26 @@ static TreeLayout tree_layout(int64_t batch, int64_t rows, int64_t max_count, in
   return L;
 }
 
-template <int D, int RW>
-static int tree_launch(const TreeParams& p, const TreeLayout& L, hipStream_t s) {
-  using C = TreeCfg<D, RW>;
-  static std::atomic<uint64_t> done{0};
-  once_per_device(done, [] {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&tree_attn_kernel<D, RW>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
+template <typename C, typename K>
+static void tree_run(K kernel, std::atomic<uint64_t>& done, const TreeParams& p, const TreeLayout& L, hipStream_t s) {
+  once_per_device(done, [&] {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                              C::kLds);
   });
-  hipLaunchKernelGGL((tree_attn_kernel<D, RW>), dim3((unsigned)L.grid), dim3(kTreeThreads), C::kLds, s, p);
-  if (!L.whole)
-    hipLaunchKernelGGL(tree_combine_kernel<D>, dim3((unsigned)p.rows, (unsigned)cdiv(p.hq * D, 4 * kTreeThreads)),
-                       dim3(kTreeThreads), 0, s, p, C::kRows);
-  return check_launch("tree_attention");
+  hipLaunchKernelGGL(kernel, dim3((unsigned)L.grid), dim3(kTreeThreads), C::kLds, s, p);
 }
 
 template <int D>
 static int tree_launch(const TreeParams& p, const TreeLayout& L, hipStream_t s) {
-  return L.row_waves == 1 ? tree_launch<D, 1>(p, L, s)
-                          : (L.row_waves == 2 ? tree_launch<D, 2>(p, L, s) : tree_launch<D, 4>(p, L, s));
+  static std::atomic<uint64_t> thin{0}, wide{0};
+  if (L.wide)
+    tree_run<TreeWide<D>>(tree_wide_kernel<D>, wide, p, L, s);
+  else
+    tree_run<TreeThin<D>>(tree_thin_kernel<D>, thin, p, L, s);
+  if (!L.whole)
+    hipLaunchKernelGGL(tree_combine_kernel<D>, dim3((unsigned)p.rows, (unsigned)cdiv(p.hq * D, 4 * kTreeThreads)),
+                       dim3(kTreeThreads), 0, s, p, L.wide ? TreeWide<D>::kRows : TreeThin<D>::kRows);
+  return check_launch("tree_attention");
 }
 
 }  // namespace q6moe
