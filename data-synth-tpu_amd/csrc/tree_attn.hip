@@ -76,7 +76,7 @@ struct TreeWide {
   static constexpr int kRows = 128;
   static constexpr int kTile = D == 256 ? 32 : 64;
   static constexpr int kStep = kTile;
-  static constexpr int kPerCu = D == 64 ? 3 : 2;
+  static constexpr int kPerCu = D == 64 ? 4 : (D == 128 ? 3 : 2);
   static constexpr int kHalf = kTile * D;
   static constexpr int kScale = 2 * kTile * 4 + 16;
   static constexpr int kLds = 2 * kHalf + 4 * kHalf + 4 * kScale + 32;  // a tile's codes, the same in FP16
@@ -88,6 +88,13 @@ __device__ __forceinline__ void tree_wait_vm() {
   static_assert(N >= 0 && N < 64, "vmcnt range");
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
   asm volatile("" ::: "memory");
+}
+
+// A value that the compiler knows nothing of: what is formed from it in a loop is
+// formed anew each time, instead of being held in registers across the loop.
+__device__ __forceinline__ uint32_t tree_opaque(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 // What the rows of a sequence need: cached tokens, new tokens with rows, keys in reach.
@@ -225,10 +232,10 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
 // different halves of the banks. Chunk c of a row's key lies in slot c ^
 // tree_swizzle(row), so that the 16 lanes that read one column of 16 keys meet 16
 // different bank groups; values, read by rows, lie as they are.
-__device__ __forceinline__ int tree_row(int key) { return (key & ~5) | (key & 1) << 2 | (key >> 2 & 1); }
+__device__ __forceinline__ uint32_t tree_row(uint32_t key) { return (key & ~5u) | (key & 1) << 2 | (key >> 2 & 1); }
 template <int D>
-__device__ __forceinline__ int tree_swizzle(int row) {
-  constexpr int CH = D / 16;
+__device__ __forceinline__ uint32_t tree_swizzle(uint32_t row) {
+  constexpr uint32_t CH = D / 16;
   return (row / (16 / CH)) & (CH - 1);
 }
 
@@ -493,7 +500,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
     if (wave == 0) tree_wanted(p, seq, wanted);
     __syncthreads();
   }
-  const int64_t row_bytes = (int64_t)p.kvh * D;
+  const uint32_t row_bytes = (uint32_t)p.kvh * D;
   const int8_t* kbase = p.kc + (int64_t)it.kh * D;
   const int8_t* vbase = p.vc + (int64_t)it.kh * D;
   const auto issue = [&](int i, int stage) {
@@ -501,10 +508,10 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
     uint8_t* st = ring + stage * 2 * C::kHalf;
 #pragma unroll
     for (int d = 0; d < KS; ++d) {  // 64 chunks of 16 bytes each
-      const int line = (64 * d + lane) / (D / 16), slot = (64 * d + lane) % (D / 16);
-      const int64_t off = (int64_t)__shfl(r, tree_row(line)) * row_bytes;
-      const int8_t* k = kbase + off + 16 * (slot ^ tree_swizzle<D>(line));
-      const int8_t* v = vbase + off + 16 * slot;
+      const uint32_t line = 64 * d / (D / 16) + (uint32_t)lane / (D / 16), slot = (uint32_t)lane % (D / 16);
+      const uint32_t rr = __builtin_amdgcn_ds_bpermute(4 * tree_row(line), r);
+      const int8_t* k = kbase + (uint64_t)rr * row_bytes + 16 * (slot ^ tree_swizzle<D>(line));
+      const int8_t* v = vbase + (uint64_t)rr * row_bytes + 16 * slot;
       __builtin_amdgcn_global_load_lds(k, LDS_PTR(st + 1024 * d), 16, 0, 0);
       __builtin_amdgcn_global_load_lds(v, LDS_PTR(st + C::kHalf + 1024 * d), 16, 0, 0);
     }
@@ -742,19 +749,20 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
     if (wave == 0) tree_wanted(p, seq, wanted);
     __syncthreads();
   }
-  const int64_t row_bytes = (int64_t)p.kvh * D;
+  const uint32_t row_bytes = (uint32_t)p.kvh * D;
   const int8_t* kbase = p.kc + (int64_t)it.kh * D;
   const int8_t* vbase = p.vc + (int64_t)it.kh * D;
   constexpr int kDma = C::kHalf / 4096;  // DMA instructions per wave for keys, and for values
   const auto issue = [&](int i) {
     const int r = keys.row(p, tile_at(i), tile_at(i + 1));
+    const uint32_t at = tree_opaque(lane);
 #pragma unroll
     for (int d = 0; d < kDma; ++d) {
-      const int first = 64 * (wave * kDma + d);  // chunks of 16 bytes
-      const int line = (first + lane) / (D / 16), slot = (first + lane) % (D / 16);
-      const int64_t off = (int64_t)__shfl(r, tree_row(line)) * row_bytes;
-      const int8_t* k = kbase + off + 16 * (slot ^ tree_swizzle<D>(line));
-      const int8_t* v = vbase + off + 16 * slot;
+      const uint32_t first = 64 * (wave * kDma + d);  // chunks of 16 bytes
+      const uint32_t line = first / (D / 16) + at / (D / 16), slot = at % (D / 16);
+      const uint32_t rr = __builtin_amdgcn_ds_bpermute(4 * tree_row(line), r);
+      const int8_t* k = kbase + (uint64_t)rr * row_bytes + 16 * (slot ^ tree_swizzle<D>(line));
+      const int8_t* v = vbase + (uint64_t)rr * row_bytes + 16 * slot;
       __builtin_amdgcn_global_load_lds(k, LDS_PTR(kr + 16 * first), 16, 0, 0);
       __builtin_amdgcn_global_load_lds(v, LDS_PTR(vr + 16 * first), 16, 0, 0);
     }
@@ -789,12 +797,11 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   const auto half2 = [&](uint32_t hi, uint32_t lo, uint32_t sel) {
     return __builtin_bit_cast(uint32_t, (f16x2)(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(hi, lo, sel)) + bias));
   };
-  const int tid = threadIdx.x;
   const auto convert = [&]() {
+    const uint32_t tid = tree_opaque(threadIdx.x);
 #pragma unroll
     for (int i = 0; i < C::kHalf / 4096; ++i) {
-      const int key = tid % T, chunk = tid / T + i * (kTreeThreads / T);
-      const int line = tree_row(key);
+      const uint32_t key = tid % T, chunk = tid / T + i * (kTreeThreads / T), line = tree_row(key);
       u32x4 x = *reinterpret_cast<const u32x4*>(kr + line * D + 16 * (chunk ^ tree_swizzle<D>(line)));
       u32x4 y[2];
 #pragma unroll
@@ -807,10 +814,10 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
       *reinterpret_cast<u32x4*>(kf + 16 * ((2 * chunk + 1) * T + key)) = y[1];
     }
     constexpr int kLanes = D == 64 ? 16 : 32, W = D == 256 ? 2 : 1;
-    const int quad = tid % kLanes;
+    const uint32_t quad = tid % kLanes;
 #pragma unroll
     for (int k = 0; k < T / 4 * kLanes / kTreeThreads; ++k) {
-    const int four = tid / kLanes + k * (kTreeThreads / kLanes);  // keys 4 four + [0, 4)
+    const uint32_t four = tid / kLanes + k * (kTreeThreads / kLanes);  // keys 4 four + [0, 4)
     uint32_t x[4][W];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -829,7 +836,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
     for (int b = 0; b < 4 * W; ++b) {
       const uint32_t sel = 0x0c040c00u + (uint32_t)(b & 3) * 0x00010001u;
       const u32x2 y = {half2(x[1][b >> 2], x[0][b >> 2], sel), half2(x[3][b >> 2], x[2][b >> 2], sel)};
-      const int c = D == 64 ? b & 1 : b, r = D == 64 ? quad + 16 * (b >> 1) : quad;
+      const uint32_t c = D == 64 ? b & 1 : b, r = D == 64 ? quad + 16 * (b >> 1) : quad;
       *reinterpret_cast<u32x2*>(dst + 16 * (c * 32 + r)) = y;
     }
     }
