@@ -30,6 +30,8 @@ import torch
 
 own = False
 
+PACKAGE = str(Path(__file__).resolve().parents[1] / "data-synth-tpu_amd")
+
 MOST_TREE = 256  # new tokens of a sequence that masks tell apart
 
 
@@ -390,9 +392,8 @@ def run(s):
 
 
 def _run_own(s):
-    package = str(Path(__file__).resolve().parents[1] / "data-synth-tpu_amd")
-    if package not in sys.path:
-        sys.path.insert(0, package)
+    if PACKAGE not in sys.path:
+        sys.path.insert(0, PACKAGE)
     import q6moe
 
     if s["kind"] == "plan":
