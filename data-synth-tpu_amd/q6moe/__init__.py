@@ -52,7 +52,8 @@ def __getattr__(name):
     if name in ("plan_pages", "release_pages", "write_tokens", "paged_tree_attention", "keep_accepted", "PagePlan"):
         from . import step
 
-        return getattr(step, name)
+        globals()[name] = found = getattr(step, name)  # a step's calls are short: the next one finds it at once
+        return found
     if name == "routes":
         from . import router
 

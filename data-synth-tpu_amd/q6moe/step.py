@@ -136,16 +136,13 @@ def plan_pages(page_table, lengths, counts, free_pages, free_count, *, page_size
         elif out.masks is not None:
             raise ValueError("out.masks must be None without parents")
     work = torch.empty(batch + 1, dtype=torch.int32, device=device)
-    a = _lib.PlanArgs()
-    a.page_table, a.lengths, a.counts = page_table.data_ptr(), lens.data_ptr(), want.data_ptr()
-    a.free_pages, a.free_capacity, a.free_count = free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr()
-    a.parents = parents.data_ptr() if words else None
-    a.batch, a.pages_per_seq, a.page_size, a.rows = batch, pps, page_size, rows
-    a.max_count = rows if max_count is None else max_count
-    a.starts, a.slots, a.positions = out.starts.data_ptr(), out.slots.data_ptr(), out.positions.data_ptr()
-    a.masks = out.masks.data_ptr() if words else None
-    a.missing = out.missing.data_ptr()
-    a.workspace, a.workspace_bytes = work.data_ptr(), 4 * (batch + 1)
+    # positionally, in the order of q6moe_kv_plan_args: a field assigned by name costs as much as a check
+    a = _lib.PlanArgs(
+        page_table.data_ptr(), lens.data_ptr(), want.data_ptr(), free_pages.data_ptr(), free_pages.shape[0],
+        free_count.data_ptr(), parents.data_ptr() if words else None, batch, pps, page_size, rows,
+        rows if max_count is None else max_count, out.starts.data_ptr(), out.slots.data_ptr(),
+        out.positions.data_ptr(), out.masks.data_ptr() if words else None, out.missing.data_ptr(), work.data_ptr(),
+        4 * (batch + 1))
     _launch.run("kv_plan", _lib.load().q6moe_kv_plan, device, ctypes.byref(a))
     return out
 
@@ -222,13 +219,10 @@ def write_tokens(k_pool, k_scales, v_pool, v_scales, key, value, slots, *, kv_he
         raise ValueError("key and value must have the same type")
     if rows == 0 or n == 0:
         return
-    a = _lib.KvWriteRowsArgs()
-    a.key, a.value, a.key_stride, a.value_stride = key.data_ptr(), value.data_ptr(), key_stride, value_stride
-    a.x_dtype = _dtype_code(key.dtype)
-    a.k_codes, a.v_codes, a.k_scales, a.v_scales = (t.data_ptr() for t in (k_pool, v_pool, k_scales, v_scales))
-    a.scale_dtype = _dtype_code(k_scales.dtype)
-    a.slots = slots.data_ptr()
-    a.rows, a.pool_rows, a.kv_heads, a.head_dim, a.group = rows, n, kv_heads, head_dim, group
+    a = _lib.KvWriteRowsArgs(
+        key.data_ptr(), value.data_ptr(), key_stride, value_stride, _dtype_code(key.dtype), k_pool.data_ptr(),
+        v_pool.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), _dtype_code(k_scales.dtype), slots.data_ptr(),
+        rows, n, kv_heads, head_dim, group)
     _launch.run("kv_write_rows", _lib.load().q6moe_kv_write_rows, device, ctypes.byref(a))
 
 
@@ -297,17 +291,11 @@ def paged_tree_attention(q, k_pool, k_scales, v_pool, v_scales, page_table, leng
     elif (not isinstance(workspace, torch.Tensor) or workspace.dtype is not torch.uint8 or workspace.device != device
           or not workspace.is_contiguous() or workspace.numel() < need):
         raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on {device}")
-    a = _lib.TreeAttnArgs()
-    a.q, a.q_stride = q.data_ptr(), q.stride(0)
-    a.k_codes, a.v_codes, a.k_scales, a.v_scales = (t.data_ptr() for t in (k_pool, v_pool, k_scales, v_scales))
-    a.scale_dtype = _dtype_code(k_scales.dtype)
-    a.page_table, a.lengths, a.starts = table.data_ptr(), lens.data_ptr(), first.data_ptr()
-    a.masks, a.mask_words = masks.data_ptr() if words else None, words
-    a.batch, a.rows, a.max_count = batch, rows, max_count
-    a.query_heads, a.kv_heads, a.head_dim = hq, kv_heads, dim
-    a.pool_pages, a.pages_per_seq, a.page_size = k_pool.shape[0], pps, page_size
-    a.out = out.data_ptr()
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    a = _lib.TreeAttnArgs(
+        q.data_ptr(), q.stride(0), k_pool.data_ptr(), v_pool.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+        _dtype_code(k_scales.dtype), table.data_ptr(), lens.data_ptr(), first.data_ptr(),
+        masks.data_ptr() if words else None, words, batch, rows, max_count, hq, kv_heads, dim, k_pool.shape[0], pps,
+        page_size, out.data_ptr(), workspace.data_ptr(), workspace.numel())
     _launch.run("kv_tree_attention", _lib.load().q6moe_kv_tree_attention, device, ctypes.byref(a))
     return out
 
@@ -353,15 +341,14 @@ def keep_accepted(caches, page_table, lengths, path, accepted, *, page_size):
         code_bytes, scale_bytes = sizes[0] * page_size * sizes[1], sizes[0] * page_size * sizes[2]
         base, scale_base = codes.data_ptr(), scales.data_ptr()
         for i in range(stacked):
-            pointers += (base + i * code_bytes, scale_base + i * scale_bytes)
+            pointers.append(base + i * code_bytes)
+            pointers.append(scale_base + i * scale_bytes)
     if len(set(pointers)) != len(pointers):
         raise ValueError("a cache may be listed only once")
     if not pointers:
         return
-    a = _lib.KvKeepArgs()
-    a.pools, a.count = (ctypes.c_void_p * len(pointers))(*pointers), len(pointers) // 2
-    a.code_bytes, a.scale_bytes = row[1], row[2]
-    a.page_table, a.lengths, a.path, a.accepted = (t.data_ptr() for t in (table, lens, path, taken))
-    a.batch, a.path_len = path.shape
-    a.pool_pages, a.pages_per_seq, a.page_size = row[0], table.shape[1], page_size
+    a = _lib.KvKeepArgs(
+        (ctypes.c_void_p * len(pointers))(*pointers), len(pointers) // 2, row[1], row[2], table.data_ptr(),
+        lens.data_ptr(), path.data_ptr(), taken.data_ptr(), path.shape[0], path.shape[1], row[0], table.shape[1],
+        page_size)
     _launch.run("kv_keep", _lib.load().q6moe_kv_keep, device, ctypes.byref(a))
