@@ -146,8 +146,10 @@ __device__ __forceinline__ T tree_wave_reduce(T v, F f) {
   step(std::integral_constant<int, 0x4e>{});   // quad_perm [2,3,0,1]
   step(std::integral_constant<int, 0x124>{});  // row_ror:4
   step(std::integral_constant<int, 0x128>{});  // row_ror:8
-  v = f(v, __shfl_xor(v, 16));
-  return f(v, __shfl_xor(v, 32));
+  const auto swap = [&](auto r) { v = f(__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1])); };
+  swap(__builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false));
+  swap(__builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false));
+  return v;
 }
 
 // The workgroup's item, found by each wave for itself (lane t takes the sequences
@@ -180,7 +182,9 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
     if (once && p.batch <= 256)
       for (int i = 0; i < 5 && lo < hi; ++i) {
         const int mid = (lo + hi) >> 1;
-        const int n = sum(0, [&](const TreeSeq& s) { return units(s) * tree_chunks(s.n, mid * STEP); });
+        // at least the number of chunks: a rounded quotient, raised by 2^-20
+        const float per = 1.000001f / (float)(mid * STEP);
+        const int n = sum(0, [&](const TreeSeq& s) { return units(s) * ((int)((float)s.n * per) + 1); });
         if (n <= p.slots)
           hi = mid;
         else
@@ -677,37 +681,58 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   // Both half waves hold half of a row's keys in l and psum.
   float l = st.l + __shfl_xor(st.l, 32), m = st.m;
   psum += __shfl_xor(psum, 32);
-  // The waves' sums meet in LDS: each brings its own to the common maximum.
+  // The waves' sums meet in LDS, each brought to the common maximum; then every
+  // thread adds four channels of a row in wave order. A row's 16-byte runs are
+  // swizzled by the row, so that the 32 rows of a store meet all banks.
+  float* sum = reinterpret_cast<float*>(smem);  // [wave][row][D]
+  float* stats = reinterpret_cast<float*>(smem + 4 * C::kRows * D * 4);  // [wave][row]: maximum, sum
+  static_assert(4 * C::kRows * (D * 4 + 8) <= C::kLds, "merge");
   __syncthreads();
-  float* stats = reinterpret_cast<float*>(smem);  // [wave][row]: maximum, sum
-  float* sum = stats + 2 * 4 * C::kRows;          // [row][D + 4], one wave at a time
-  if (h == 0) {
-    stats[2 * (wave * C::kRows + col)] = m;
-    stats[2 * (wave * C::kRows + col) + 1] = l;
-  }
+  if (h == 0) *reinterpret_cast<f32x2*>(stats + 2 * (wave * C::kRows + col)) = f32x2{m, l};
   __syncthreads();
-  float to = kTreeFloor, all = 0.f;
+  const auto joint = [&](int row, float* all) {
+    f32x2 st[4];
+    float to = kTreeFloor;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) to = fmaxf(to, stats[2 * (g * C::kRows + col)]);
+    for (int g = 0; g < 4; ++g) {
+      st[g] = *reinterpret_cast<const f32x2*>(stats + 2 * (g * C::kRows + row));
+      to = fmaxf(to, st[g][0]);
+    }
+    *all = 0.f;
 #pragma unroll
-  for (int g = 0; g < 4; ++g)
-    all += stats[2 * (g * C::kRows + col) + 1] * __builtin_amdgcn_exp2f(stats[2 * (g * C::kRows + col)] - to);
-  const float up = __builtin_amdgcn_exp2f(m - to) * (0x1p24f / st.factor), shift = 128.f * psum * 0x1p-24f;
+    for (int g = 0; g < 4; ++g) *all += st[g][1] * __builtin_amdgcn_exp2f(st[g][0] - to);
+    return to;
+  };
+  float all;
+  const float up = __builtin_amdgcn_exp2f(m - joint(col, &all)) * (0x1p24f / st.factor), shift = 128.f * psum * 0x1p-24f;
+  if (row.live)
+    tree_runs<D>(acc, h, [&](int c, f32x4 v) {
 #pragma unroll
-  for (int c = 0; c < KS; ++c)
+      for (int u = 0; u < 4; ++u) v[u] = (v[u] - shift) * up;
+      return *reinterpret_cast<f32x4*>(sum + (wave * C::kRows + col) * D + 4 * ((c / 4) ^ (col & (D / 4 - 1)))) = v;
+    });
+  __syncthreads();
+  const int first = it.tile * C::kRows, left = seq.count * p.r - first;
+  const int live = left < C::kRows ? left : C::kRows;
+  const bool split = tree_chunks(n, it.keys) > 1;
+  for (int i = threadIdx.x; i < live * (D / 4); i += kTreeThreads) {
+    const int rr = i / (D / 4), c = i % (D / 4);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int v = 0; v < 16; ++v) acc[c][v] = (acc[c][v] - shift) * up;
-  for (int g = 3; g >= 0; --g) {
-    if (wave == g)
-      tree_runs<D>(acc, h, [&](int c, f32x4 v) {
-        f32x4* at = reinterpret_cast<f32x4*>(sum + col * (D + 4) + c);
-        if (g < 3) v += *at;
-        return *at = v;
-      });
-    __syncthreads();
+    for (int g = 0; g < 4; ++g)
+      v += *reinterpret_cast<const f32x4*>(sum + (g * C::kRows + rr) * D + 4 * (c ^ (rr & (D / 4 - 1))));
+    const float to = joint(rr, &all);
+    const int64_t place = (int64_t)it.id * C::kRows + rr;
+    if (split) {
+      *reinterpret_cast<f32x4*>(p.part + place * D + 4 * c) = v;
+      if (c == 0) *reinterpret_cast<f32x2*>(p.stat + 2 * place) = f32x2{to, all};
+    } else {
+      const float inv = all == 0.f ? 0.f : 1.f / all;
+      const int j = (first + rr) / p.r, hh = first + rr - j * p.r;
+      *reinterpret_cast<u32x2*>(p.out + ((int64_t)(seq.start + j) * p.hq + it.kh * p.r + hh) * D + 4 * c) =
+          u32x2{pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv)};
+    }
   }
-  if (wave == 0 && row.live)
-    tree_result<D>(p, it, acc, tree_chunks(n, it.keys) > 1, to, all, row.j, row.hh, it.id * C::kRows + col, h);
 }
 
 // ---------------------------------------------------------------------------
