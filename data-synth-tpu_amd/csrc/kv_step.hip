@@ -9,9 +9,11 @@
 // the counts. The free pages are a stack, taken from and given back at its end in
 // the order of (sequence, page index), so all results are deterministic.
 //
-// Latency-bound: a few kilobytes for a decode step. The dependent round trips are
-// what counts, so every sum over earlier sequences is formed by each workgroup for
-// itself, from one load per 256 sequences, instead of by a launch of its own.
+// Latency-bound: a few kilobytes for a decode step. A step's calls are one launch of
+// one workgroup each (a plan and its release of 8 sequences with 16-token trees: 5
+// launches 20 us of kernels, 2 launches 11 us); larger ones take two or three, in
+// which every workgroup forms the sums over earlier sequences for itself, from one
+// load per 256 of them, instead of waiting for a launch more.
 #include "q6moe_api.h"
 #include "q6moe_device.h"
 
@@ -122,10 +124,10 @@ __global__ void __launch_bounds__(kStepThreads) plan_need_kernel(PlanParams p) {
 
 // Slot of the token at position t of sequence b, -1 without a page.
 __device__ __forceinline__ int64_t plan_slot(const PlanParams& p, int64_t b, int64_t t) {
-  const int64_t e = t / p.page;
-  if (e >= p.pps) return -1;
+  if (t >= p.pps * p.page) return -1;  // below 2^31, so that 32-bit divisions serve
+  const uint32_t page = (uint32_t)p.page, e = (uint32_t)t / page;
   const int64_t pg = p.table[b * p.pps + e];
-  return pg < 0 ? -1 : pg * p.page + (t - e * p.page);
+  return pg < 0 ? -1 : pg * p.page + ((uint32_t)t - e * page);
 }
 
 // Takes sequence b's pages from the stack; with a tree also its rows (at most
@@ -208,9 +210,9 @@ __global__ void __launch_bounds__(kStepThreads) plan_take_kernel(PlanParams p) {
 // trees they are written above), and the rows behind the last sequence.
 __global__ void __launch_bounds__(kStepThreads) plan_rows_kernel(PlanParams p) {
   const int64_t row = (int64_t)blockIdx.x * kStepThreads + threadIdx.x;
-  if (row >= p.rows) return;
   const int64_t used = p.starts[p.batch];
   if (row >= used) {
+    if (row >= p.rows) return;
     p.slots[row] = -1;
     p.positions[row] = 0;
     if (p.masks)
@@ -218,19 +220,161 @@ __global__ void __launch_bounds__(kStepThreads) plan_rows_kernel(PlanParams p) {
     return;
   }
   if (p.parents) return;
-  int64_t b = 0, hi = p.batch - 1;  // the last sequence with starts[b] <= row
-  while (b < hi) {
-    const int64_t mid = (b + hi + 1) / 2;
-    if (p.starts[mid] <= row)
-      b = mid;
-    else
-      hi = mid - 1;
+  // The last sequence with starts[b] <= row: for the wave's first row by 64 probes at
+  // a time, then on from there.
+  const int lane = threadIdx.x & 63;
+  const int64_t row0 = row - lane;
+  int b = 0, n = (int)p.batch;  // the sequence is one of b .. b + n - 1
+  while (n > 1) {
+    const int step = (n + 63) / 64, at = b + lane * step;
+    const int below = __popcll(__ballot(lane * step < n && p.starts[at] <= row0));
+    const int skip = (below - 1) * step;
+    b += skip;
+    n = n - skip < step ? n - skip : step;
   }
+  while (b + 1 < p.batch && p.starts[b + 1] <= row) ++b;
   const int64_t t = plan_len(p, b) + row - p.starts[b];
   const int64_t slot = plan_slot(p, b, t);
   p.slots[row] = slot;
   p.positions[row] = (int32_t)t;
   if (slot < 0) atomicAdd(p.missing, 1);
+}
+
+// ---- one workgroup for a step's plan ---------------------------------------
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallWaves = kSmallThreads / 64;
+constexpr int kSmallRows = 4096;     // rows, and words of masks, that one workgroup takes
+constexpr int kSmallTreeRows = 2048;
+constexpr int kSmallPages = 32;      // pages per sequence that its thread looks through
+
+// Sum of v over the threads before this one; *total: over all of them.
+__device__ __forceinline__ int small_before(int v, int* lds, int* total) {
+  int upto = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int x = __shfl_up(upto, off);
+    if ((int)(threadIdx.x & 63) >= off) upto += x;
+  }
+  __syncthreads();  // lds may still be read
+  if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = upto;
+  __syncthreads();
+  int before = upto - v, all = 0;
+#pragma unroll
+  for (int w = 0; w < kSmallWaves; ++w) {
+    if (w < (int)(threadIdx.x >> 6)) before += lds[w];
+    all += lds[w];
+  }
+  *total = all;
+  return before;
+}
+
+// At most 1024 sequences, one per thread, and few rows: the steps of the three
+// kernels above in turn. The trees of all sequences are resolved together.
+template <bool kTree>
+__global__ void __launch_bounds__(kSmallThreads) plan_small_kernel(PlanParams p) {
+  __shared__ int lds[kSmallWaves];
+  __shared__ int s_start[kSmallThreads + 1], s_len[kSmallThreads];
+  __shared__ uint64_t sees[kTree ? kSmallRows : 1];
+  __shared__ int up[kTree ? kSmallTreeRows : 1], depth[kTree ? kSmallTreeRows : 1];
+  const int t = threadIdx.x, batch = (int)p.batch, rows = (int)p.rows;
+  int64_t len = 0, asked = 0, first = 0, end = 0;
+  int count = 0, all, need = 0;
+  if (t < batch) {
+    len = plan_len(p, t);
+    asked = plan_asked(p, t);
+    count = (int)(asked < p.max_count ? (asked < rows ? asked : rows) : (p.max_count < rows ? p.max_count : rows));
+  }
+  const int64_t have0 = p.free_count[0];
+  const int have = (int)(have0 < 0 ? 0 : (have0 < p.free_capacity ? have0 : p.free_capacity));
+  const int before = small_before(count, lds, &all);
+  const int used = all < rows ? all : rows;
+  int32_t* table = p.table + t * p.pps;
+  if (t < batch) {
+    count = (int)plan_fit(p, count, before);
+    plan_pages(p, len, count, &first, &end);
+    for (int64_t e = first; e < end; ++e) need += table[e] < 0;
+    s_start[t] = before < rows ? before : rows;
+    s_len[t] = (int)len;
+    p.starts[t] = s_start[t];
+  }
+  if (t == 0) p.starts[batch] = used;
+  int taken;
+  int rank = small_before(need, lds, &taken);
+  if (need)
+    for (int64_t e = first; e < end; ++e)
+      if (table[e] < 0) {
+        if (rank < have) table[e] = p.free_pages[have - 1 - rank];
+        ++rank;
+      }
+  if (t == 0) p.free_count[0] = have - (taken < have ? taken : have);
+  const int64_t over = asked - count;
+  int missing = t < batch ? (int)(over < (1 << 20) ? over : 1 << 20) : 0;
+  __syncthreads();  // the entries and sums above
+  const auto sequence = [&](int row) {  // the last one with s_start[b] <= row
+    int b = 0, hi = batch - 1;
+    while (b < hi) {
+      const int mid = (b + hi + 1) >> 1;
+      if (s_start[mid] <= row)
+        b = mid;
+      else
+        hi = mid - 1;
+    }
+    return b;
+  };
+  if constexpr (kTree) {
+    const int words = p.words;
+    for (int row = t; row < used; row += kSmallThreads) {
+      const int b = sequence(row), j = row - s_start[b], parent = p.parents[row];
+      up[row] = parent >= 0 && parent < j ? s_start[b] + parent : -1;
+      depth[row] = up[row] >= 0;
+      for (int w = 0; w < words; ++w) sees[row * words + w] = w == j >> 6 ? 1ull << (j & 63) : 0;
+    }
+    for (int reach = 1; reach < p.max_count; reach *= 2) {
+      uint64_t more[kSmallTreeRows / kSmallThreads][kMaxTree / 64];
+      int to[kSmallTreeRows / kSmallThreads], deeper[kSmallTreeRows / kSmallThreads];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kSmallTreeRows / kSmallThreads; ++k) {
+        const int row = t + k * kSmallThreads, u = row < used ? up[row] : -1;
+        to[k] = -1;
+        deeper[k] = 0;
+        if (u >= 0) {
+          to[k] = up[u];
+          deeper[k] = depth[u];
+        }
+#pragma unroll
+        for (int w = 0; w < kMaxTree / 64; ++w) more[k][w] = u >= 0 && w < words ? sees[u * words + w] : 0;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kSmallTreeRows / kSmallThreads; ++k) {
+        const int row = t + k * kSmallThreads;
+        if (row >= used) continue;
+        up[row] = to[k];
+        depth[row] += deeper[k];
+#pragma unroll
+        for (int w = 0; w < kMaxTree / 64; ++w)
+          if (w < words) sees[row * words + w] |= more[k][w];
+      }
+    }
+    __syncthreads();
+  }
+  for (int row = t; row < rows; row += kSmallThreads) {
+    int64_t slot = -1;
+    int position = 0;
+    if (row < used) {
+      const int b = sequence(row), j = row - s_start[b];
+      slot = plan_slot(p, b, (int64_t)s_len[b] + j);
+      position = s_len[b] + (kTree ? depth[row] : j);
+      missing += slot < 0;
+    }
+    p.slots[row] = slot;
+    p.positions[row] = position;
+    if constexpr (kTree)
+      for (int w = 0; w < p.words; ++w) p.masks[(int64_t)row * p.words + w] = row < used ? sees[row * p.words + w] : 0;
+  }
+  small_before(missing, lds, &all);
+  if (t == 0) p.missing[0] = all;
 }
 
 struct ReleaseParams {
@@ -296,17 +440,58 @@ __global__ void __launch_bounds__(kStepThreads) release_put_kernel(ReleaseParams
   }
 }
 
+// At most 1024 sequences and 4096 entries, a run of them per thread. (16384 entries
+// took one workgroup 22 us, the two launches above 7.7.)
+constexpr int kSmallEntries = 4;
+__global__ void __launch_bounds__(kSmallThreads) release_small_kernel(ReleaseParams p) {
+  __shared__ int lds[kSmallWaves];
+  __shared__ int s_first[kSmallThreads];
+  const int t = threadIdx.x, pps = (int)p.pps, entries = (int)p.batch * pps;
+  const int per = (entries + kSmallThreads - 1) / kSmallThreads, i0 = t * per;
+  if (t < p.batch) s_first[t] = (int)release_first(p, t);
+  const int64_t have0 = p.free_count[0];
+  const int64_t have = have0 < 0 ? 0 : (have0 < p.free_capacity ? have0 : p.free_capacity);
+  int32_t pg[kSmallEntries];
+#pragma unroll
+  for (int k = 0; k < kSmallEntries; ++k) pg[k] = k < per && i0 + k < entries ? p.table[i0 + k] : -1;
+  __syncthreads();
+  int b = i0 / pps, e = i0 - b * pps, n = 0, total;
+#pragma unroll
+  for (int k = 0; k < kSmallEntries; ++k) {
+    if (pg[k] >= 0 && e < s_first[b]) pg[k] = -1;
+    n += pg[k] >= 0;
+    if (++e == pps) {
+      e = 0;
+      ++b;
+    }
+  }
+  int rank = small_before(n, lds, &total);
+#pragma unroll
+  for (int k = 0; k < kSmallEntries; ++k)
+    if (pg[k] >= 0) {
+      const int64_t at = have + total - 1 - rank++;
+      if (at < p.free_capacity) {
+        p.free_pages[at] = pg[k];
+        p.table[i0 + k] = -1;
+      }
+    }
+  if (t == 0) p.free_count[0] = (int32_t)(have + total < p.free_capacity ? have + total : p.free_capacity);
+}
+
 // ---------------------------------------------------------------------------
 // Accepted tokens of a tree moved to the front of its places, in the caches of
 // all layers: row of position len + path[i] -> row of position len + i. A
-// workgroup takes one sequence, one pool and kKeepUnits units of its rows; every
-// thread holds what it moves in registers and all of a workgroup's reads come
-// before its writes, so a path may cross itself.
+// workgroup takes one sequence, one pool and a column of its rows; every thread
+// holds what it moves in registers and all of a workgroup's reads come before its
+// writes, so a path may cross itself. Bound by its chain of round trips: accepted,
+// path, two page-table entries, the row.
 // ---------------------------------------------------------------------------
 constexpr int kKeepPools = 128;  // pools per launch: their pointers are kernel arguments
-constexpr int kKeepUnits = 8;    // units (16, 4 or 1 bytes) of a row per workgroup
 constexpr int kKeepRows = 256;   // most accepted tokens of a sequence
-constexpr int kKeepTurns = kKeepRows * kKeepUnits / kStepThreads;
+constexpr int kKeepTurns = 8;    // units (16, 4 or 1 bytes) that a thread holds
+// Units of a row per workgroup: 32, which covers 512 bytes of codes, for up to 64
+// accepted tokens, else 8.
+constexpr int kKeepWide = 32, kKeepNarrow = kKeepTurns * kStepThreads / kKeepRows;
 
 struct KeepParams {
   const int32_t* table;
@@ -314,66 +499,98 @@ struct KeepParams {
   const int32_t* path;
   const int32_t* accepted;
   int64_t pps, page, pool_pages, most;
-  int64_t units;  // per row
-  void* pool[kKeepPools];
+  int64_t units[2];  // per row of the codes, and of the scales
+  int blocks;        // workgroups over a row of codes; further ones take the scales
+  void* pool[kKeepPools][2];
 };
 
 __device__ __forceinline__ int64_t keep_row(const KeepParams& p, int64_t b, int64_t t) {
-  if (t < 0 || t >= p.pps * p.page) return -1;
-  const int64_t pg = p.table[b * p.pps + t / p.page];
-  return pg < 0 || pg >= p.pool_pages ? -1 : pg * p.page + t % p.page;
+  if (t < 0 || t >= p.pps * p.page) return -1;  // below 2^31, so that 32-bit divisions serve
+  const uint32_t page = (uint32_t)p.page, e = (uint32_t)t / page;
+  const int64_t pg = p.table[b * p.pps + e];
+  return pg < 0 || pg >= p.pool_pages ? -1 : pg * p.page + ((uint32_t)t - e * page);
 }
 
-template <typename Unit>
-__global__ void __launch_bounds__(kStepThreads) keep_kernel(KeepParams p) {
-  const int64_t b = blockIdx.y;
-  const int64_t asked = p.accepted[b];
-  const int n = (int)(asked < p.most ? asked : p.most);
-  if (n <= 0) return;
-  const int64_t u = (int64_t)blockIdx.x * kKeepUnits + threadIdx.x % kKeepUnits;
+template <int kUnits, typename Unit>
+__device__ __forceinline__ void keep_move(const KeepParams& p, int what, int64_t block, int n) {
+  const int64_t b = blockIdx.y, units = p.units[what];
+  const int64_t u = block * kUnits + threadIdx.x % kUnits;
   const int64_t len = p.lengths[b];
-  Unit* pool = reinterpret_cast<Unit*>(p.pool[blockIdx.z]);
+  Unit* pool = reinterpret_cast<Unit*>(p.pool[blockIdx.z][what]);
   Unit held[kKeepTurns];
   int64_t to[kKeepTurns];
 #pragma unroll
   for (int k = 0; k < kKeepTurns; ++k) {
-    const int i = k * (kStepThreads / kKeepUnits) + (int)threadIdx.x / kKeepUnits;
+    const int i = k * (kStepThreads / kUnits) + (int)threadIdx.x / kUnits;
     to[k] = -1;
-    if (i < n && u < p.units && len >= 0) {
+    if (i < n && u < units && len >= 0) {
       const int64_t step = p.path[b * p.most + i];
       const int64_t from = step < 0 ? -1 : keep_row(p, b, len + step);
       to[k] = from < 0 || step == i ? -1 : keep_row(p, b, len + i);
-      if (to[k] >= 0) held[k] = pool[from * p.units + u];
+      if (to[k] >= 0) held[k] = pool[from * units + u];
     }
   }
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kKeepTurns; ++k)
-    if (to[k] >= 0) pool[to[k] * p.units + u] = held[k];
+    if (to[k] >= 0) pool[to[k] * units + u] = held[k];
 }
 
-template <typename Unit>
-static void keep_launch(KeepParams& p, int64_t bytes, int64_t batch, int pools, hipStream_t s) {
-  p.units = bytes / (int64_t)sizeof(Unit);
-  hipLaunchKernelGGL(keep_kernel<Unit>, dim3((unsigned)cdiv(p.units, kKeepUnits), (unsigned)batch, (unsigned)pools),
-                     dim3(kStepThreads), 0, s, p);
+template <int kUnits, typename Codes, typename Scales>
+__global__ void __launch_bounds__(kStepThreads) keep_kernel(KeepParams p) {
+  const int64_t asked = p.accepted[blockIdx.y];
+  const int n = (int)(asked < p.most ? asked : p.most);
+  if (n <= 0) return;
+  if ((int)blockIdx.x < p.blocks)
+    keep_move<kUnits, Codes>(p, 0, blockIdx.x, n);
+  else
+    keep_move<kUnits, Scales>(p, 1, blockIdx.x - p.blocks, n);
 }
 
-// Rows of ``bytes`` bytes in the pools at base[i] (every second pointer of the caller's list).
-static int keep_pools(KeepParams p, void* const* base, int64_t pools, int64_t bytes, int64_t batch, hipStream_t s) {
-  for (int64_t i0 = 0; i0 < pools; i0 += kKeepPools) {
-    const int n = (int)(pools - i0 < kKeepPools ? pools - i0 : kKeepPools);
-    int64_t a = bytes;
-    for (int i = 0; i < n; ++i) {
-      p.pool[i] = base[2 * (i0 + i)];
-      a |= (int64_t)reinterpret_cast<uintptr_t>(p.pool[i]);
-    }
-    if (a % 16 == 0)
-      keep_launch<u32x4>(p, bytes, batch, n, s);
-    else if (a % 4 == 0)
-      keep_launch<uint32_t>(p, bytes, batch, n, s);
+// The largest unit of 16, 4 and 1 bytes that rows and pools are multiples of.
+static int keep_unit(int64_t bits) { return bits % 16 == 0 ? 16 : (bits % 4 == 0 ? 4 : 1); }
+
+template <int kUnits, typename Codes>
+static void keep_launch(const KeepParams& p, int scale_unit, dim3 grid, hipStream_t s) {
+  if (scale_unit == 16)
+    hipLaunchKernelGGL((keep_kernel<kUnits, Codes, u32x4>), grid, dim3(kStepThreads), 0, s, p);
+  else if (scale_unit == 4)
+    hipLaunchKernelGGL((keep_kernel<kUnits, Codes, uint32_t>), grid, dim3(kStepThreads), 0, s, p);
+  else
+    hipLaunchKernelGGL((keep_kernel<kUnits, Codes, uint8_t>), grid, dim3(kStepThreads), 0, s, p);
+}
+
+template <int kUnits>
+static void keep_width(const KeepParams& p, const int* unit, dim3 grid, hipStream_t s) {
+  if (unit[0] == 16)
+    keep_launch<kUnits, u32x4>(p, unit[1], grid, s);
+  else if (unit[0] == 4)
+    keep_launch<kUnits, uint32_t>(p, unit[1], grid, s);
+  else
+    keep_launch<kUnits, uint8_t>(p, unit[1], grid, s);
+}
+
+// The pools of the caller's list, as many per launch as its arguments hold.
+static int keep_pools(KeepParams p, const q6moe_kv_keep_args* a, hipStream_t s) {
+  for (int64_t i0 = 0; i0 < a->count; i0 += kKeepPools) {
+    const int n = (int)(a->count - i0 < kKeepPools ? a->count - i0 : kKeepPools);
+    int64_t bits[2] = {a->code_bytes, a->scale_bytes};
+    for (int i = 0; i < n; ++i)
+      for (int w = 0; w < 2; ++w) {
+        p.pool[i][w] = a->pools[2 * (i0 + i) + w];
+        bits[w] |= (int64_t)reinterpret_cast<uintptr_t>(p.pool[i][w]);
+      }
+    const int unit[2] = {keep_unit(bits[0]), keep_unit(bits[1])};
+    p.units[0] = a->code_bytes / unit[0];
+    p.units[1] = a->scale_bytes / unit[1];
+    const bool wide = p.most <= kKeepTurns * kStepThreads / kKeepWide;
+    const int per = wide ? kKeepWide : kKeepNarrow;
+    p.blocks = (int)cdiv(p.units[0], per);
+    const dim3 grid((unsigned)(p.blocks + cdiv(p.units[1], per)), (unsigned)a->batch, (unsigned)n);
+    if (wide)
+      keep_width<kKeepWide>(p, unit, grid, s);
     else
-      keep_launch<uint8_t>(p, bytes, batch, n, s);
+      keep_width<kKeepNarrow>(p, unit, grid, s);
     if (const int rc = check_launch("kv_keep")) return rc;
   }
   return Q6MOE_OK;
@@ -428,6 +645,16 @@ extern "C" int q6moe_kv_plan(const q6moe_kv_plan_args* a, void* stream) {
   p.missing = a->missing;
   p.need = reinterpret_cast<int32_t*>(a->workspace);
   hipStream_t s = (hipStream_t)stream;
+  // One launch where a thread can take a sequence's pages and one workgroup the rows.
+  const int64_t most = p.max_count < p.rows ? p.max_count : p.rows;
+  if (p.batch <= kSmallThreads && p.rows <= kSmallRows && most / p.page + 2 <= kSmallPages &&
+      (!p.parents || (p.rows <= kSmallTreeRows && p.rows * p.words <= kSmallRows))) {
+    if (p.parents)
+      hipLaunchKernelGGL(plan_small_kernel<true>, dim3(1), dim3(kSmallThreads), 0, s, p);
+    else
+      hipLaunchKernelGGL(plan_small_kernel<false>, dim3(1), dim3(kSmallThreads), 0, s, p);
+    return check_launch("kv_plan kernel");
+  }
   hipLaunchKernelGGL(plan_need_kernel, dim3((unsigned)p.batch), dim3(kStepThreads), 0, s, p);
   hipLaunchKernelGGL(plan_take_kernel, dim3((unsigned)p.batch), dim3(kStepThreads), 0, s, p);
   hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)cdiv(p.rows, kStepThreads)), dim3(kStepThreads), 0, s, p);
@@ -450,6 +677,10 @@ extern "C" int q6moe_kv_release(int32_t* page_table, const int32_t* lengths, int
   ReleaseParams p{page_table, lengths, free_pages, free_capacity, free_count, batch, pages_per_seq, page_size,
                   reinterpret_cast<int32_t*>(workspace)};
   hipStream_t s = (hipStream_t)stream;
+  if (batch <= kSmallThreads && batch * pages_per_seq <= kSmallThreads * kSmallEntries) {
+    hipLaunchKernelGGL(release_small_kernel, dim3(1), dim3(kSmallThreads), 0, s, p);
+    return check_launch("kv_release kernel");
+  }
   hipLaunchKernelGGL(release_count_kernel, dim3((unsigned)batch), dim3(kStepThreads), 0, s, p);
   hipLaunchKernelGGL(release_put_kernel, dim3((unsigned)batch), dim3(kStepThreads), 0, s, p);
   return check_launch("kv_release kernels");
@@ -463,8 +694,9 @@ extern "C" int q6moe_kv_keep(const q6moe_kv_keep_args* a, void* stream) {
   Q6MOE_REQUIRE(a->code_bytes >= 1 && a->scale_bytes >= 1 && a->code_bytes < (1 << 24) && a->scale_bytes < (1 << 24),
                 "kv_keep: row sizes must be positive and below 2^24 bytes");
   Q6MOE_REQUIRE(a->pool_pages >= 1 && a->pages_per_seq >= 1 && a->page_size >= 1 && a->pool_pages < (1ll << 31) &&
-                    a->pages_per_seq < (1ll << 31) && a->page_size < (1ll << 31),
-                "kv_keep: pool_pages, pages_per_seq and page_size must be positive and below 2^31");
+                    a->pages_per_seq < (1ll << 31) && a->page_size < (1ll << 31) &&
+                    a->pages_per_seq * a->page_size < (1ll << 31),
+                "kv_keep: pool_pages, pages_per_seq and page_size must be positive, a sequence's capacity below 2^31");
   Q6MOE_REQUIRE(a->path_len >= 1 && a->path_len <= kKeepRows, "kv_keep: a path holds 1 to 256 tokens");
   for (int64_t i = 0; i < 2 * a->count; ++i) Q6MOE_REQUIRE(a->pools[i], "kv_keep: null pool");
   KeepParams p;
@@ -477,6 +709,5 @@ extern "C" int q6moe_kv_keep(const q6moe_kv_keep_args* a, void* stream) {
   p.pool_pages = a->pool_pages;
   p.most = a->path_len;
   hipStream_t s = (hipStream_t)stream;
-  if (const int rc = keep_pools(p, a->pools, a->count, a->code_bytes, a->batch, s)) return rc;
-  return keep_pools(p, a->pools + 1, a->count, a->scale_bytes, a->batch, s);
+  return keep_pools(p, a, s);
 }
