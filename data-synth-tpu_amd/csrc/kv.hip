@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvQuant q, KvWrite w, int
 // kv_code's: the product with the rounded reciprocal r is within 2 ulp, one
 // correction by its exact FMA residual brings it within one, and from there a second
 // rounds correctly (Markstein, IBM J. Res. Dev. 34, 1990). Five instructions where the
-// general division takes some ten; 24 K rows of 1024 values: 38.8 us with it, @@ here.
+// general division takes some ten; 20.5 K rows of 1024 values: 38.8 us with it, 32.0 here.
 // Divisors whose reciprocal or residuals leave the normal range take the division.
 struct KvRows {
   const void* x[2];

@@ -207,23 +207,16 @@ __global__ void __launch_bounds__(kStepThreads) plan_take_kernel(PlanParams p) {
 }
 
 // Rows of the ragged batch: slots and positions of the sequences' tokens (of
-// trees they are written above), and the rows behind the last sequence.
+// trees they are written above), and the rows behind the last sequence. Four rows
+// per thread, whose table entries are on their way together: 638 K rows 8.8 us with
+// one, 8.3 with four.
+constexpr int kPlanRows = 4;
 __global__ void __launch_bounds__(kStepThreads) plan_rows_kernel(PlanParams p) {
-  const int64_t row = (int64_t)blockIdx.x * kStepThreads + threadIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int64_t row0 = ((int64_t)blockIdx.x * kStepThreads + (threadIdx.x & ~63)) * kPlanRows;  // of the wave
   const int64_t used = p.starts[p.batch];
-  if (row >= used) {
-    if (row >= p.rows) return;
-    p.slots[row] = -1;
-    p.positions[row] = 0;
-    if (p.masks)
-      for (int w = 0; w < p.words; ++w) p.masks[row * p.words + w] = 0;
-    return;
-  }
-  if (p.parents) return;
   // The last sequence with starts[b] <= row: for the wave's first row by 64 probes at
   // a time, then on from there.
-  const int lane = threadIdx.x & 63;
-  const int64_t row0 = row - lane;
   int b = 0, n = (int)p.batch;  // the sequence is one of b .. b + n - 1
   while (n > 1) {
     const int step = (n + 63) / 64, at = b + lane * step;
@@ -232,12 +225,28 @@ __global__ void __launch_bounds__(kStepThreads) plan_rows_kernel(PlanParams p) {
     b += skip;
     n = n - skip < step ? n - skip : step;
   }
-  while (b + 1 < p.batch && p.starts[b + 1] <= row) ++b;
-  const int64_t t = plan_len(p, b) + row - p.starts[b];
-  const int64_t slot = plan_slot(p, b, t);
-  p.slots[row] = slot;
-  p.positions[row] = (int32_t)t;
-  if (slot < 0) atomicAdd(p.missing, 1);
+  int lost = 0;
+#pragma unroll
+  for (int k = 0; k < kPlanRows; ++k) {
+    const int64_t row = row0 + 64 * k + lane;
+    if (row >= used) {
+      if (row < p.rows) {
+        p.slots[row] = -1;
+        p.positions[row] = 0;
+        if (p.masks)
+          for (int w = 0; w < p.words; ++w) p.masks[row * p.words + w] = 0;
+      }
+      continue;
+    }
+    if (p.parents) continue;
+    while (b + 1 < p.batch && p.starts[b + 1] <= row) ++b;
+    const int64_t t = plan_len(p, b) + row - p.starts[b];
+    const int64_t slot = plan_slot(p, b, t);
+    p.slots[row] = slot;
+    p.positions[row] = (int32_t)t;
+    lost += slot < 0;
+  }
+  if (lost) atomicAdd(p.missing, lost);
 }
 
 // ---- one workgroup for a step's plan ---------------------------------------
@@ -365,7 +374,7 @@ __global__ void __launch_bounds__(kSmallThreads) plan_small_kernel(PlanParams p)
     if (row < used) {
       const int b = sequence(row), j = row - s_start[b];
       slot = plan_slot(p, b, (int64_t)s_len[b] + j);
-      position = s_len[b] + (kTree ? depth[row] : j);
+      position = (int)((int64_t)s_len[b] + (kTree ? depth[row] : j));
       missing += slot < 0;
     }
     p.slots[row] = slot;
@@ -515,7 +524,7 @@ template <int kUnits, typename Unit>
 __device__ __forceinline__ void keep_move(const KeepParams& p, int what, int64_t block, int n) {
   const int64_t b = blockIdx.y, units = p.units[what];
   const int64_t u = block * kUnits + threadIdx.x % kUnits;
-  const int64_t len = p.lengths[b];
+  const int64_t len = p.lengths[b] < 0 ? 0 : p.lengths[b];
   Unit* pool = reinterpret_cast<Unit*>(p.pool[blockIdx.z][what]);
   Unit held[kKeepTurns];
   int64_t to[kKeepTurns];
@@ -523,7 +532,7 @@ __device__ __forceinline__ void keep_move(const KeepParams& p, int what, int64_t
   for (int k = 0; k < kKeepTurns; ++k) {
     const int i = k * (kStepThreads / kUnits) + (int)threadIdx.x / kUnits;
     to[k] = -1;
-    if (i < n && u < units && len >= 0) {
+    if (i < n && u < units) {
       const int64_t step = p.path[b * p.most + i];
       const int64_t from = step < 0 ? -1 : keep_row(p, b, len + step);
       to[k] = from < 0 || step == i ? -1 : keep_row(p, b, len + i);
@@ -657,7 +666,8 @@ extern "C" int q6moe_kv_plan(const q6moe_kv_plan_args* a, void* stream) {
   }
   hipLaunchKernelGGL(plan_need_kernel, dim3((unsigned)p.batch), dim3(kStepThreads), 0, s, p);
   hipLaunchKernelGGL(plan_take_kernel, dim3((unsigned)p.batch), dim3(kStepThreads), 0, s, p);
-  hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)cdiv(p.rows, kStepThreads)), dim3(kStepThreads), 0, s, p);
+  hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)cdiv(p.rows, kStepThreads * kPlanRows)),
+                     dim3(kStepThreads), 0, s, p);
   return check_launch("kv_plan kernels");
 }
 

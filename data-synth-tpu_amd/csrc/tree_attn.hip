@@ -46,6 +46,7 @@ struct TreeParams {
   int page_shift;
   int slots;       // workgroups that the work is split for
   int whole;       // no split over keys
+  int grid;        // workgroups of the launch
   float to_log2;   // log2(e) / sqrt(D)
   float* part;     // [workgroup][row of the tile][D] partial sums
   float* stat;     // [workgroup][row of the tile][2]: maximum (log2) and sum
@@ -178,8 +179,11 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
     const bool once = 2 * tiles <= p.slots;
     int lo = (int)(total / (float)(once ? p.slots : 2 * p.slots) * (1.f / STEP));
     lo = lo < 1 ? 1 : (lo < (1 << 30) / STEP / 2 - 1 ? lo : (1 << 30) / STEP / 2 - 1);
-    int hi = once ? 2 * lo + 2 : lo + 1;  // in steps; hi gives few enough chunks
-    if (once && p.batch <= 256)
+    // in steps; hi gives few enough chunks: each tile has at most one that is not full
+    const float sure = total / (float)(p.slots - tiles) * (1.00001f / STEP);
+    int hi = once ? (sure < (float)(1 << 30) / STEP - 1.f ? (int)sure : (1 << 30) / STEP - 1) + 1 : lo + 1;
+    // few tiles: hi is within an eighth of the least
+    if (once && 8 * tiles > p.slots && p.batch <= 256)
       for (int i = 0; i < 5 && lo < hi; ++i) {
         const int mid = (lo + hi) >> 1;
         // at least the number of chunks: a rounded quotient, raised by 2^-20
@@ -452,11 +456,11 @@ __device__ __forceinline__ void tree_runs(A& acc, int h, F&& f) {
 // A row's sums (of the values times the state's factor) to the workspace, or its output.
 template <int D, typename A>
 __device__ __forceinline__ void tree_result(const TreeParams& p, const TreeItem& it, A& acc, bool split, float m,
-                                            float l, int j, int hh, int place, int h) {
+                                            float l, int j, int hh, int64_t place, int h) {
   if (split) {
-    float* dst = p.part + (int64_t)place * D;
+    float* dst = p.part + place * D;
     tree_runs<D>(acc, h, [&](int c, f32x4 v) { return *reinterpret_cast<f32x4*>(dst + c) = v; });
-    if (h == 0) *reinterpret_cast<f32x2*>(p.stat + 2 * (int64_t)place) = f32x2{m, l};
+    if (h == 0) *reinterpret_cast<f32x2*>(p.stat + 2 * place) = f32x2{m, l};
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -955,7 +959,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
     for (int v = 0; v < 16; ++v) acc[c][v] *= up;
   if (row.live)
     tree_result<D>(p, it, acc, tree_chunks(n, it.keys) > 1, st.m, l, row.j, row.hh,
-                   it.id * C::kRows + wave * 32 + col, h);
+                   (int64_t)it.id * C::kRows + wave * 32 + col, h);
 }
 
 // The chunks' sums of a row and head joined in chunk order, D / 4 lanes of four
@@ -985,6 +989,8 @@ __global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p
   if (chunks == 1) return;
   const int64_t first = ((int64_t)from + (int64_t)kh * tiles + tile) * tile_rows + rr - tile * tile_rows;
   const int64_t step = (int64_t)p.kvh * tiles * tile_rows;
+  // starts that do not ascend can name more tiles than the workspace has places for
+  if (from < 0 || first + (chunks - 1) * step >= (int64_t)p.grid * tile_rows) return;
   const int in = lane & (W - 1);
   float m = kTreeFloor, l = 0.f;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
@@ -1157,6 +1163,7 @@ extern "C" int q6moe_kv_tree_attention(const q6moe_tree_attn_args* a, void* stre
   p.page_shift = 31 + lg;
   p.slots = L.slots;
   p.whole = L.whole;
+  p.grid = (int)L.grid;
   p.to_log2 = 1.4426950408889634f / sqrtf((float)a->head_dim);
   uint8_t* w = reinterpret_cast<uint8_t*>(a->workspace);
   p.info = reinterpret_cast<int32_t*>(w + L.info);

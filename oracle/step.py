@@ -83,10 +83,9 @@ def keep(pool, table, lengths, path, accepted, page):
     old, new = np.array(pool), np.array(pool)
     pages, cap = old.shape[0], table.shape[1] * page
     for b in range(table.shape[0]):
-        if lengths[b] < 0:
-            continue
+        n = max(0, int(lengths[b]))
         for i in range(min(int(accepted[b]), path.shape[1])):
-            to, at = lengths[b] + i, lengths[b] + path[b, i]
+            to, at = n + i, n + path[b, i]
             if path[b, i] < 0 or max(to, at) >= cap:
                 continue
             pt, pa = table[b, to // page], table[b, at // page]

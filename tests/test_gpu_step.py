@@ -6,6 +6,11 @@ Whole numbers, codes and scales must be equal. With A = sum p |v| / sum p an att
   2 d A           the scores: d bounds their error, (2^-15 + D 2^-24) max|q| sum|k| / sqrt(D). The first
                   term is half a step of q held in 16 bits, the second a chain of D roundings in FP32,
   2^-16 A         the hardware exponential (1 ulp) of FP32 arguments,
+  n 2^-21 max vs  probabilities near 0: p vs f is held in FP16, whose step below 2^-14 is 2^-24, with a factor
+                  f of at least 2^3 / max vs (the kernel brings the largest value scale to 2^3 or more), so
+                  that p vs is off by at most 2^-25 2^-3 max vs; times a code of at most 127, over n keys; the
+                  sum of p that divides it is at least 1. (Found with a row whose largest key has code 0 and
+                  all others p < 1e-9: 9.5e-11 over the bound without this term, at values of size 1.)
   n 2^-25 A       the sums over n keys: chains of n / 16 roundings, of codes up to 255 (the INT8 codes + 128)
                   where sum p |v| has their mean size, a seventh.
 """
@@ -55,7 +60,8 @@ def _plan_case(seed, batch, pps, page, most, tree, extra, short=0):
     (1, 1, 1, 1, 1, False, 0, 0), (2, 5, 7, 16, 40, False, 3, 0), (3, 300, 9, 64, 200, False, 100, 0),
     (4, 3, 600, 4, 2100, False, 0, 0), (5, 40, 8, 16, 30, False, 0, 11), (6, 1, 4, 8, 1, True, 2, 0),
     (7, 9, 12, 16, 64, True, 0, 0), (8, 33, 40, 7, 65, True, 17, 0), (9, 6, 64, 64, 256, True, 5, 4),
-    (10, 700, 3, 5, 4, True, 1, 50),
+    (10, 700, 3, 5, 4, True, 1, 50), (11, 9, 700, 8, 3000, False, 7, 0), (12, 70, 80, 16, 150, True, 300, 20),
+    (13, 1024, 5, 64, 3, False, 0, 0), (14, 1025, 4, 64, 3, False, 9, 0), (15, 3, 40, 4, 126, False, 0, 0),
 ])
 def test_plan_and_release(device, seed, batch, pps, page, most, tree, extra, short):
     table, lengths, counts, free, count, rows, parents = _plan_case(seed, batch, pps, page, most, tree, extra, short)
@@ -226,6 +232,7 @@ def _check(got, case, sees, rows=None, scales=None):
     d = (2.0**-15 + q.shape[2] * 2.0**-24) * top * slope
     n = min(max(lengths) + most, table.shape[1] * page)
     tol = 2.0**-8 * np.abs(want) + (2.0**-11 + 2 * d[..., None] + 2.0**-16 + n * 2.0**-25) * spread
+    tol += n * 2.0**-21 * np.nanmax(np.where(np.isfinite(vs), vs, 0))
     over = (np.abs(got - want) - tol)[live]
     assert np.isfinite(got[live]).all() and (over <= 0).all(), over.max()
     return live
@@ -256,25 +263,50 @@ def test_attention(device, page, kvh, r, dim, lengths, counts, extra, kind):
     np.testing.assert_array_equal(got, again)
 
 
+@pytest.mark.parametrize("batch,kvh,r,dim,count,most_len,spare_count", [
+    (300, 2, 2, 64, 1, 400, 0),    # few rows, more tiles than half the places: chunks run in turns
+    (520, 4, 1, 128, 1, 30, 0),    # so many that none is split
+    (70, 4, 9, 64, 12, 300, 5),    # many rows, in turns; max_count above any count
+    (390, 8, 25, 64, 4, 20, 0),    # many rows, none split
+])
+def test_attention_of_many_sequences(device, batch, kvh, r, dim, count, most_len, spare_count):
+    rng = np.random.default_rng(batch)
+    lengths = rng.integers(0, most_len + 1, batch)
+    counts = rng.integers(0, count + 1, batch)
+    k, ks, v, vs, table, _, starts, page, kvh, q, _ = _case(batch, lengths, counts, 16, kvh, r, dim, 2)
+    got = _attn(device, (k, ks, v, vs, table, lengths, starts, page, kvh, q, count + spare_count), None, fill=9.0)
+    assert (got[starts[-1]:] == 9.0).all()
+    for b in rng.permutation(batch)[:12]:  # each by itself
+        a, e = starts[b], starts[b + 1]
+        if e > a:
+            one = (k, ks, v, vs, table[b:b + 1], lengths[b:b + 1], np.array([0, e - a]), page, kvh, q[a:e], count)
+            _check(got[a:e], one, None)
+
+
 def test_attention_chain_of_a_prompt(device):
     case = _case(3, [0, 300], [333, 130], 64, 2, 3, 128)
     _check(_attn(device, case, None), case, None)
 
 
-def test_attention_rows_that_see_nothing(device):
+FEW_AND_MANY = pytest.mark.parametrize("r", [4, 20])  # query heads per KV head: few rows, and many
+
+
+@FEW_AND_MANY
+def test_attention_rows_that_see_nothing(device, r):
     # no cached tokens, empty masks: 0; a mask that names tokens past the sequence's own names nothing
-    case = _case(11, [0, 0, 9], [3, 2, 2], 16, 2, 4, 128)
-    sees = [set(), {2}, {0, 5, 63}, set(), {0}, set(), {1, 2, 40}]
+    case = _case(11, [0, 0, 9], [3, 2, 9], 16, 2, r, 128)
+    sees = [set(), {2}, {0, 5, 63}, set(), {0}, set(), {1, 2, 40}, {8}, {0}, {3, 4}, set(), {7}, {6, 5}, {8, 2}]
     got = _attn(device, case, sees)
     _check(got, case, sees)
     assert (got[0] == 0).all() and (got[3] == 0).all()
     assert got[1].any(-1).all()  # row 1 is one key's value, some of whose codes are 0
 
 
-def test_attention_garbage_where_nothing_looks(device):
+@FEW_AND_MANY
+def test_attention_garbage_where_nothing_looks(device, r):
     # scales of every place that no row sees are NaN or infinite, codes are -128
     lengths, counts = [70, 5], [6, 4]
-    case = _case(12, lengths, counts, 16, 2, 4, 128)
+    case = _case(12, lengths, counts, 16, 2, r, 128)
     k, ks, v, vs, table = case[:5]
     sees = [s - {3} for s in _sees(np.random.default_rng(1), counts, 0)]
     held = np.zeros(ks.shape[:2], bool)
@@ -293,9 +325,10 @@ def test_attention_garbage_where_nothing_looks(device):
         np.testing.assert_array_equal(_attn(device, case, sees), want)
 
 
-def test_attention_scales_far_apart(device):
+@FEW_AND_MANY
+def test_attention_scales_far_apart(device, r):
     # values whose scales span 2^40, some of them 0, in an order that grows; scores far from 0
-    case = _case(13, [900], [8], 64, 1, 8, 128, qscale=6.0)
+    case = _case(13, [900], [8], 64, 1, r, 128, qscale=6.0)
     k, ks, v, vs, table = case[:5]
     rng = np.random.default_rng(2)
     vs *= 2.0 ** rng.integers(-20, 21, vs.shape).astype(np.float32)
@@ -307,9 +340,10 @@ def test_attention_scales_far_apart(device):
         _check(_attn(device, (k, ks, v, vs2, *case[4:]), None), (k, ks, v, vs2, *case[4:]), None)
 
 
-def test_attention_queries_far_apart(device):
+@FEW_AND_MANY
+def test_attention_queries_far_apart(device, r):
     # rows of queries from 2^-100 to 2^100 (with keys to match), one of zeros
-    case = _case(14, [130], [6], 64, 1, 2, 128)
+    case = _case(14, [130], [6], 64, 1, r, 128)
     q = case[9]
     for i, e in enumerate((0, -100, -20, 3)):
         q[i] *= np.float32(2.0**e)
@@ -321,9 +355,10 @@ def test_attention_queries_far_apart(device):
     _check(_attn(device, case, None), case, None)
 
 
-def test_attention_unmapped_pages_and_short_tables(device):
+@FEW_AND_MANY
+def test_attention_unmapped_pages_and_short_tables(device, r):
     # unmapped pages read as zero; tokens past the table's width are not seen
-    case = _case(15, [60, 40], [8, 8], 16, 2, 4, 64, width=4)
+    case = _case(15, [60, 40], [8, 8], 16, 2, r, 64, width=4)
     k, ks, v, vs, table = case[:5]
     table[0, 1], table[1, 2] = -1, k.shape[0] + 4
     sees = _sees(np.random.default_rng(3), [8, 8], 0)
@@ -419,6 +454,7 @@ def test_keep_accepted(device, batch, page, pps, chans, groups, dtype, layers, m
     table = rng.permutation(pages)[:batch * pps].reshape(batch, pps).astype(np.int32)
     table[rng.random(table.shape) < 0.05] = -1
     lengths = rng.integers(0, max(1, cap - most // 2), batch).astype(np.int32)
+    lengths[-1] -= 2 * lengths[-1] * (batch > 3)  # below 0: as 0
     path = np.sort(rng.integers(-1, most + 10, (batch, most)), 1).astype(np.int32)
     path[0] = rng.permutation(most)  # any order: the places are read before they are written
     accepted = rng.integers(0, most + 3, batch).astype(np.int32)
