@@ -130,9 +130,19 @@ __device__ __forceinline__ int64_t plan_slot(const PlanParams& p, int64_t b, int
   return pg < 0 ? -1 : pg * p.page + ((uint32_t)t - e * page);
 }
 
-// Takes sequence b's pages from the stack; with a tree also its rows (at most
-// kMaxTree of them, one per thread): the ancestors by pointer doubling in LDS,
-// each round adds those 1, 2, 4, ... levels further up.
+constexpr int kTakeRows = 4096;  // rows of a sequence that its workgroup writes
+__device__ __forceinline__ void plan_behind(const PlanParams& p, int64_t row) {
+  p.slots[row] = -1;
+  p.positions[row] = 0;
+  if (p.masks)
+    for (int w = 0; w < p.words; ++w) p.masks[row * p.words + w] = 0;
+}
+
+// Takes sequence b's pages from the stack, then (kRows) writes its rows, and the
+// last workgroup those behind the last sequence. The rows of a tree, at most
+// kMaxTree, lie one per thread: the ancestors by pointer doubling in LDS, each round
+// adds those 1, 2, 4, ... levels further up.
+template <bool kRows>
 __global__ void __launch_bounds__(kStepThreads) plan_take_kernel(PlanParams p) {
   __shared__ int64_t lds[kStepWaves];
   const int64_t b = blockIdx.x;
@@ -165,11 +175,24 @@ __global__ void __launch_bounds__(kStepThreads) plan_take_kernel(PlanParams p) {
   }
   const int64_t lost = plan_asked(p, b) - count;
   if (threadIdx.x == 0 && lost) atomicAdd(p.missing, (int32_t)(lost < (1 << 30) ? lost : 1 << 30));
-  if (!p.parents) return;
+  if constexpr (!kRows) return;
+  __syncthreads();  // the table entries above
+  if (b == p.batch - 1)
+    for (int64_t row = start + count + threadIdx.x; row < p.rows; row += kStepThreads) plan_behind(p, row);
+  if (!p.parents) {
+    int none = 0;
+    for (int64_t j = threadIdx.x; j < count; j += kStepThreads) {
+      const int64_t slot = plan_slot(p, b, len + j);
+      p.slots[start + j] = slot;
+      p.positions[start + j] = (int32_t)(len + j);
+      none += slot < 0;
+    }
+    if (none) atomicAdd(p.missing, none);
+    return;
+  }
   __shared__ uint64_t sees[kMaxTree][kMaxTree / 64];
   __shared__ int up[kMaxTree], depth[kMaxTree];
   const int j = threadIdx.x;
-  __syncthreads();  // the table entries above
   if (j < count) {
     const int64_t parent = p.parents[start + j];
     up[j] = parent >= 0 && parent < j ? (int)parent : -1;
@@ -206,10 +229,9 @@ __global__ void __launch_bounds__(kStepThreads) plan_take_kernel(PlanParams p) {
   }
 }
 
-// Rows of the ragged batch: slots and positions of the sequences' tokens (of
-// trees they are written above), and the rows behind the last sequence. Four rows
-// per thread, whose table entries are on their way together: 638 K rows 8.8 us with
-// one, 8.3 with four.
+// Rows of the ragged batch where a sequence has more of them than one workgroup
+// should write: slots and positions, and the rows behind the last sequence. Four rows
+// per thread, whose table entries are on their way together.
 constexpr int kPlanRows = 4;
 __global__ void __launch_bounds__(kStepThreads) plan_rows_kernel(PlanParams p) {
   const int lane = threadIdx.x & 63;
@@ -230,15 +252,9 @@ __global__ void __launch_bounds__(kStepThreads) plan_rows_kernel(PlanParams p) {
   for (int k = 0; k < kPlanRows; ++k) {
     const int64_t row = row0 + 64 * k + lane;
     if (row >= used) {
-      if (row < p.rows) {
-        p.slots[row] = -1;
-        p.positions[row] = 0;
-        if (p.masks)
-          for (int w = 0; w < p.words; ++w) p.masks[row * p.words + w] = 0;
-      }
+      if (row < p.rows) plan_behind(p, row);
       continue;
     }
-    if (p.parents) continue;
     while (b + 1 < p.batch && p.starts[b + 1] <= row) ++b;
     const int64_t t = plan_len(p, b) + row - p.starts[b];
     const int64_t slot = plan_slot(p, b, t);
@@ -579,19 +595,27 @@ static void keep_width(const KeepParams& p, const int* unit, dim3 grid, hipStrea
     keep_launch<kUnits, uint8_t>(p, unit[1], grid, s);
 }
 
-// The pools of the caller's list, as many per launch as its arguments hold.
+// The caller's pools, as many per launch as its arguments hold.
 static int keep_pools(KeepParams p, const q6moe_kv_keep_args* a, hipStream_t s) {
-  for (int64_t i0 = 0; i0 < a->count; i0 += kKeepPools) {
-    const int n = (int)(a->count - i0 < kKeepPools ? a->count - i0 : kKeepPools);
-    int64_t bits[2] = {a->code_bytes, a->scale_bytes};
-    for (int i = 0; i < n; ++i)
+  const int64_t rows = a->pool_pages * a->page_size, bytes[2] = {a->code_bytes, a->scale_bytes};
+  int64_t cache = 0, place = 0;  // the next pool: number ``place`` of its cache's
+  while (cache < a->count) {
+    int64_t bits[2] = {bytes[0], bytes[1]};
+    int n = 0;
+    while (n < kKeepPools && cache < a->count) {
       for (int w = 0; w < 2; ++w) {
-        p.pool[i][w] = a->pools[2 * (i0 + i) + w];
-        bits[w] |= (int64_t)reinterpret_cast<uintptr_t>(p.pool[i][w]);
+        p.pool[n][w] = reinterpret_cast<uint8_t*>(a->pools[2 * cache + w]) + place * rows * bytes[w];
+        bits[w] |= (int64_t)reinterpret_cast<uintptr_t>(p.pool[n][w]);
       }
+      ++n;
+      if (++place == (a->stacked ? a->stacked[cache] : 1)) {
+        place = 0;
+        ++cache;
+      }
+    }
     const int unit[2] = {keep_unit(bits[0]), keep_unit(bits[1])};
-    p.units[0] = a->code_bytes / unit[0];
-    p.units[1] = a->scale_bytes / unit[1];
+    p.units[0] = bytes[0] / unit[0];
+    p.units[1] = bytes[1] / unit[1];
     const bool wide = p.most <= kKeepTurns * kStepThreads / kKeepWide;
     const int per = wide ? kKeepWide : kKeepNarrow;
     p.blocks = (int)cdiv(p.units[0], per);
@@ -665,9 +689,15 @@ extern "C" int q6moe_kv_plan(const q6moe_kv_plan_args* a, void* stream) {
     return check_launch("kv_plan kernel");
   }
   hipLaunchKernelGGL(plan_need_kernel, dim3((unsigned)p.batch), dim3(kStepThreads), 0, s, p);
-  hipLaunchKernelGGL(plan_take_kernel, dim3((unsigned)p.batch), dim3(kStepThreads), 0, s, p);
-  hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)cdiv(p.rows, kStepThreads * kPlanRows)),
-                     dim3(kStepThreads), 0, s, p);
+  // Sequences of up to 4096 new tokens by their own workgroups: 638 K rows of 256
+  // sequences in two launches 14.0 us, in three 17.0.
+  if (most <= kTakeRows) {
+    hipLaunchKernelGGL(plan_take_kernel<true>, dim3((unsigned)p.batch), dim3(kStepThreads), 0, s, p);
+  } else {
+    hipLaunchKernelGGL(plan_take_kernel<false>, dim3((unsigned)p.batch), dim3(kStepThreads), 0, s, p);
+    hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)cdiv(p.rows, kStepThreads * kPlanRows)),
+                       dim3(kStepThreads), 0, s, p);
+  }
   return check_launch("kv_plan kernels");
 }
 
@@ -709,6 +739,9 @@ extern "C" int q6moe_kv_keep(const q6moe_kv_keep_args* a, void* stream) {
                 "kv_keep: pool_pages, pages_per_seq and page_size must be positive, a sequence's capacity below 2^31");
   Q6MOE_REQUIRE(a->path_len >= 1 && a->path_len <= kKeepRows, "kv_keep: a path holds 1 to 256 tokens");
   for (int64_t i = 0; i < 2 * a->count; ++i) Q6MOE_REQUIRE(a->pools[i], "kv_keep: null pool");
+  if (a->stacked)
+    for (int64_t i = 0; i < a->count; ++i)
+      Q6MOE_REQUIRE(a->stacked[i] >= 1 && a->stacked[i] <= (1 << 20), "kv_keep: a cache stacks 1 to 2^20 pools");
   KeepParams p;
   p.table = a->page_table;
   p.lengths = a->lengths;

@@ -211,6 +211,7 @@ class TreeAttnArgs(ctypes.Structure):
 class KvKeepArgs(ctypes.Structure):
     _fields_ = [
         ("pools", ctypes.POINTER(_vp)),
+        ("stacked", ctypes.POINTER(_i64)),
         ("count", _i64),
         ("code_bytes", _i64),
         ("scale_bytes", _i64),

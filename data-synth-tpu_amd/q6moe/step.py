@@ -309,8 +309,8 @@ def keep_accepted(caches, page_table, lengths, path, accepted, *, page_size):
     any order: all are read before any is written. ``caches`` lists (codes, scales)
     pairs that share the page table: int8 [..., pages, page_size, channels] and
     [..., pages, page_size, groups], where leading dimensions stack the caches of
-    several layers; all are updated in one launch each for codes and scales. Then
-    ``lengths + accepted`` are the cached tokens.
+    several layers; up to 128 of them are updated in one launch. Then ``lengths +
+    accepted`` are the cached tokens.
     """
     caches = list(caches)
     if not caches:
@@ -324,7 +324,7 @@ def keep_accepted(caches, page_table, lengths, path, accepted, *, page_size):
         raise ValueError("page_table must be [batch, pages_per_seq], lengths and accepted [batch]")
     if path.ndim != 2 or path.shape[0] != table.shape[0] or not 1 <= path.shape[1] <= MAX_TREE:
         raise ValueError(f"path must be [batch, most] with at most {MAX_TREE} tokens")
-    pointers, row = [], None
+    pointers, stacked, spans, row = [], [], [], None
     for codes, scales in caches:
         if codes.dtype is not torch.int8 or codes.ndim < 3 or codes.device != device or not codes.is_contiguous() or \
                 codes.shape[-2] != page_size:
@@ -337,18 +337,19 @@ def keep_accepted(caches, page_table, lengths, path, accepted, *, page_size):
             row = sizes
         if sizes != row or not all(sizes):
             raise ValueError("all caches must have the same pages, channels and groups")
-        stacked = codes.numel() // (sizes[0] * page_size * sizes[1])
-        code_bytes, scale_bytes = sizes[0] * page_size * sizes[1], sizes[0] * page_size * sizes[2]
-        base, scale_base = codes.data_ptr(), scales.data_ptr()
-        for i in range(stacked):
-            pointers.append(base + i * code_bytes)
-            pointers.append(scale_base + i * scale_bytes)
-    if len(set(pointers)) != len(pointers):
+        held = codes.numel()
+        if held:
+            start, scale_start = codes.data_ptr(), scales.data_ptr()
+            pointers += (start, scale_start)
+            stacked.append(held // (sizes[0] * page_size * sizes[1]))
+            spans += ((start, start + held), (scale_start, scale_start + held // sizes[1] * sizes[2]))
+    spans.sort()
+    if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
         raise ValueError("a cache may be listed only once")
     if not pointers:
         return
     a = _lib.KvKeepArgs(
-        (ctypes.c_void_p * len(pointers))(*pointers), len(pointers) // 2, row[1], row[2], table.data_ptr(),
-        lens.data_ptr(), path.data_ptr(), taken.data_ptr(), path.shape[0], path.shape[1], row[0], table.shape[1],
-        page_size)
+        (ctypes.c_void_p * len(pointers))(*pointers), (ctypes.c_int64 * len(stacked))(*stacked), len(stacked), row[1],
+        row[2], table.data_ptr(), lens.data_ptr(), path.data_ptr(), taken.data_ptr(), path.shape[0], path.shape[1],
+        row[0], table.shape[1], page_size)
     _launch.run("kv_keep", _lib.load().q6moe_kv_keep, device, ctypes.byref(a))

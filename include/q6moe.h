@@ -483,7 +483,8 @@ int q6moe_kv_tree_attention(const q6moe_tree_attn_args* args, void* stream);
  * A row whose source or place is negative, past the table or unmapped is left out.
  */
 typedef struct q6moe_kv_keep_args {
-  void* const* pools;        /* HOST array of 2 * count device pointers: codes, scales of each pool */
+  void* const* pools;        /* HOST array of 2 * count device pointers: codes, scales of each cache */
+  const int64_t* stacked;    /* HOST array [count]: pools that a cache holds one after another, or NULL: 1 each */
   int64_t count;
   int64_t code_bytes;        /* bytes per pool row of the codes */
   int64_t scale_bytes;       /* and of the scales */

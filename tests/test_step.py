@@ -90,6 +90,7 @@ def test_attention_refusals(over, text):
     (dict(path=None), "null pointer"), (dict(count=0), "positive"), (dict(code_bytes=0), "row sizes"),
     (dict(path_len=257), "1 to 256"), (dict(path_len=0), "1 to 256"), (dict(pool_pages=0), "positive"),
     (dict(pools=(ctypes.c_void_p * 2)(FAKE, None)), "null pool"),
+    (dict(stacked=(ctypes.c_int64 * 1)(0)), "stacks 1 to"), (dict(pages_per_seq=1 << 16, page_size=1 << 16), "2^31"),
 ])
 def test_keep_refusals(over, text):
     a = _filled(_lib.KvKeepArgs, **{**dict(pools=(ctypes.c_void_p * 2)(FAKE, FAKE)), **over})
