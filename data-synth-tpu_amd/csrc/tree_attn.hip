@@ -20,6 +20,7 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTreeThreads = 256;
 constexpr int kTreeMaxHeads = 65535;
@@ -153,6 +154,22 @@ __device__ __forceinline__ T tree_wave_reduce(T v, F f) {
   return v;
 }
 
+// Sum of v over the lanes up to this one: shifts within rows of 16, then the rows'
+// last lanes spread over the rows after them.
+__device__ __forceinline__ int tree_wave_scan(int v) {
+  const auto add = [&](auto ctrl, auto rows) {
+    v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr:1
+  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});  // row_shr:2
+  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});  // row_shr:4
+  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});  // row_shr:8
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast:15 into rows 1 and 3
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // The workgroup's item, found by each wave for itself (lane t takes the sequences
 // t, t + 64, ..). The call's work, sum over sequences of tiles x heads x keys, is
 // cut into chunks of at most ``keys`` keys: the least number that gives no more
@@ -206,13 +223,7 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
   for (int b0 = 0; b0 < p.batch; b0 += 64) {  // 64 sequences at a time
     const TreeSeq s = b0 == 0 ? mine : (b0 + lane < p.batch ? tree_seq(p, b0 + lane) : none);
     const int n = units(s) * tree_chunks(s.n, keys);
-    int upto = n;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int v = __shfl_up(upto, off);
-      if (lane >= off) upto += v;
-    }
-    upto += base;
+    const int upto = base + tree_wave_scan(n);
     const uint64_t has = __ballot(id < upto);
     if (has) {
       const int at = __builtin_ctzll(has);
@@ -403,7 +414,7 @@ struct TreeRow {
     j = live ? row / p.r : 0;
     hh = live ? row - j * p.r : 0;
     const uint16_t* src = p.q + (int64_t)(it.seq.start + j) * p.q_stride + (int64_t)(it.kh * p.r + hh) * D;
-    uint32_t top = 0;
+    u16x2 tops = {0, 0};  // the largest magnitudes' bits
 #pragma unroll
     for (int s = 0; s < D / 32; ++s)
 #pragma unroll
@@ -416,13 +427,10 @@ struct TreeRow {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t a = raw[s][i][w] & 0x7fffu, b = (raw[s][i][w] >> 16) & 0x7fffu;
-          top = top > a ? top : a;
-          top = top > b ? top : b;
-        }
-    const uint32_t other = __shfl_xor(top, 32);
-    top = top > other ? top : other;
+        for (int w = 0; w < 4; ++w)
+          tops = __builtin_elementwise_max(tops, __builtin_bit_cast(u16x2, raw[s][i][w] & 0x7fff7fffu));
+    const uint32_t mine = tops[0] > tops[1] ? tops[0] : tops[1], other = __shfl_xor(mine, 32);
+    const uint32_t top = mine > other ? mine : other;
     bad = top >= 0x7f80u;
     // the largest stays below 127 * 256 + 128 in steps of 2^(e-14)
     e = (int)(top >> 7) - 127 + ((top & 0x7f) == 0x7f);
