@@ -971,39 +971,53 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
 }
 
 // The chunks' sums of a row and head joined in chunk order, D / 4 lanes of four
-// channels each. Eight chunks' sums are loaded at a time; lane i of the head holds
-// the weight of chunk i.
-template <int D>
-__global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p, int tile_rows) {
-  constexpr int W = D / 4;  // lanes per head
+// channels each. ``parts`` groups of lanes take a head's chunks between them, in
+// runs, and meet in LDS. Eight chunks' sums are loaded at a time; lane i of the
+// group holds the weight of chunk i.
+template <int D, bool kJoin>
+__global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p, int tile_rows, int log_parts) {
+  constexpr int W = D / 4, kGroups = kTreeThreads / W;
+  if (!kJoin) log_parts = 0;
+  __shared__ f32x4 sums[kTreeThreads];
+  __shared__ f32x2 stats[kGroups];
   const int row = blockIdx.x, lane = threadIdx.x & 63;
-  const int at = (blockIdx.y * kTreeThreads + threadIdx.x) * 4;  // within the row's heads
-  int b = 0;  // the sequences that end before the row
+  const int keys = p.info[p.batch];
+  TreeSeq s{0, 0, 0, 0};
+  int b = -1, from = 0;  // the row's sequence: the first that ends behind it
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
-    const uint64_t before = __ballot(b0 + lane < p.batch && p.starts[b0 + lane + 1] <= row);
-    b += __popcll(before);
-    if (!(before >> 63)) break;
+    const int mine = b0 + lane < p.batch ? b0 + lane : p.batch - 1;
+    const TreeSeq t = tree_seq(p, mine);
+    const int at = p.info[mine];
+    const uint64_t has = __ballot(b0 + lane < p.batch && p.starts[mine + 1] > row);
+    if (has) {
+      const int on = __builtin_ctzll(has);
+      b = b0 + on;
+      s.start = __builtin_amdgcn_readlane(t.start, on);
+      s.count = __builtin_amdgcn_readlane(t.count, on);
+      s.len = __builtin_amdgcn_readlane(t.len, on);
+      s.n = __builtin_amdgcn_readlane(t.n, on);
+      from = __builtin_amdgcn_readlane(at, on);
+      break;
+    }
   }
-  if (b >= p.batch) return;
-  const TreeSeq s = tree_seq(p, b);
-  const int keys = p.info[p.batch], from = p.info[b];
   const int j = row - s.start;
-  if (j < 0 || j >= s.count || at >= p.hq * D) return;  // whole heads
-  const int head = at / D, c = at - head * D, kh = head / p.r, rr = j * p.r + head - kh * p.r;
+  if (b < 0 || j < 0 || j >= s.count) return;  // the whole workgroup
+  const int parts = 1 << log_parts, group = threadIdx.x / W, part = group & (parts - 1), in = lane & (W - 1);
+  const int head = (int)(blockIdx.y * kGroups + group) >> log_parts, c = 4 * in;
+  const int kh = head / p.r, rr = j * p.r + head - kh * p.r;
   const int tile = rr / tile_rows, tiles = tree_tiles(p, s, tile_rows);
   int n, n_all;
   tree_reach(p, s, tile, tile_rows, &n, &n_all);
-  const int chunks = tree_chunks(n, keys);
-  if (chunks == 1) return;
+  int chunks = tree_chunks(n, keys);
   const int64_t first = ((int64_t)from + (int64_t)kh * tiles + tile) * tile_rows + rr - tile * tile_rows;
   const int64_t step = (int64_t)p.kvh * tiles * tile_rows;
   // starts that do not ascend can name more tiles than the workspace has places for
-  if (from < 0 || first + (chunks - 1) * step >= (int64_t)p.grid * tile_rows) return;
-  const int in = lane & (W - 1);
+  const bool live = head < p.hq && chunks > 1 && from >= 0 && first + (chunks - 1) * step < (int64_t)p.grid * tile_rows;
+  const int run = (chunks + parts - 1) >> log_parts, to_chunk = live ? (part + 1) * run < chunks ? (part + 1) * run : chunks : 0;
   float m = kTreeFloor, l = 0.f;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int i0 = 0; i0 < chunks; i0 += W) {
-    const bool on = i0 + in < chunks;
+  for (int i0 = part * run; i0 < to_chunk; i0 += W) {
+    const bool on = i0 + in < to_chunk;
     const f32x2 st = on ? *reinterpret_cast<const f32x2*>(p.stat + 2 * (first + (i0 + in) * step)) : f32x2{kTreeFloor, 0.f};
     float to = st[0];
 #pragma unroll
@@ -1017,7 +1031,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p
     l = l * fade + some;
 #pragma unroll
     for (int u = 0; u < 4; ++u) v[u] *= fade;
-    const int end = chunks - i0 < W ? chunks - i0 : W;
+    const int end = to_chunk - i0 < W ? to_chunk - i0 : W;
     for (int i = 0; i < end; i += 8) {
       f32x4 x[8];
 #pragma unroll
@@ -1034,8 +1048,29 @@ __global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p
       }
     }
   }
+  if constexpr (kJoin) {
+    sums[threadIdx.x] = v;
+    if (in == 0) stats[group] = f32x2{m, l};
+    __syncthreads();
+    if (part) return;
+    float to = m;
+    for (int g = 1; g < parts; ++g) to = fmaxf(to, stats[group + g][0]);
+    const float fade = __builtin_amdgcn_exp2f(m - to);
+    l *= fade;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] *= fade;
+    for (int g = 1; g < parts; ++g) {
+      const f32x2 st = stats[group + g];
+      const f32x4 x = sums[threadIdx.x + g * W];
+      const float weight = __builtin_amdgcn_exp2f(st[0] - to);
+      l = __builtin_fmaf(st[1], weight, l);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = __builtin_fmaf(x[u], weight, v[u]);
+    }
+  }
+  if (!live) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<u32x2*>(p.out + (int64_t)row * p.hq * D + at) =
+  *reinterpret_cast<u32x2*>(p.out + ((int64_t)row * p.hq + head) * D + c) =
       u32x2{pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv)};
 }
 
@@ -1044,7 +1079,8 @@ constexpr int kTreeCus = 256;
 struct TreeLayout {
   int wide;
   int slots, whole;
-  int64_t grid;  // at most so many workgroups have work
+  int64_t units;  // row tiles x KV heads, at most
+  int64_t grid;   // at most so many workgroups have work
   size_t info, stat, part, total;
 };
 
@@ -1053,18 +1089,36 @@ static size_t tree_align(size_t v) { return (v + 255) & ~(size_t)255; }
 template <int D>
 static int tree_per_cu(bool wide) { return wide ? TreeWide<D>::kPerCu : TreeThin<D>::kPerCu; }
 
-static TreeLayout tree_layout(int64_t batch, int64_t rows, int64_t max_count, int64_t hq, int64_t kvh, int64_t dim) {
+static TreeLayout tree_layout(int64_t batch, int64_t rows, int64_t max_count, int64_t hq, int64_t kvh, int64_t dim,
+                              int64_t cap) {
   TreeLayout L;
   const int64_t r = hq / kvh;
-  // Up to three thin tiles of rows per sequence and KV head read the keys through
-  // L2 and finish sooner than one wide tile: over 32 K tokens 64 rows 48 us against
-  // 60, 96 rows 61 against 70, 128 rows 79 against 80 (with the combine).
-  L.wide = max_count * r > 3 * TreeThin<128>::kRows;
-  const int64_t tile = L.wide ? TreeWide<128>::kRows : TreeThin<128>::kRows;
-  // row tiles of all sequences together: each ends with one that is not full
-  const int64_t by_batch = batch * cdiv(max_count * r, tile), by_rows = rows * r / tile + batch;
-  const int64_t units = kvh * (by_batch < by_rows ? by_batch : by_rows);
-  L.slots = kTreeCus * (dim == 64 ? tree_per_cu<64>(L.wide) : (dim == 128 ? tree_per_cu<128>(L.wide) : tree_per_cu<256>(L.wide)));
+  // row tiles of all sequences together, at most: each sequence ends with one that
+  // is not full
+  const auto tiles = [&](int64_t tile) {
+    const int64_t by_batch = batch * cdiv(max_count * r, tile), by_rows = rows * r / tile + batch;
+    return kvh * (by_batch < by_rows ? by_batch : by_rows);
+  };
+  const auto slots = [&](bool wide) {
+    return kTreeCus *
+           (dim == 64 ? tree_per_cu<64>(wide) : (dim == 128 ? tree_per_cu<128>(wide) : tree_per_cu<256>(wide)));
+  };
+  // The wide kernel has the higher rate, but its workgroups' partial sums are four
+  // times as many bytes: some 25 us more for writing and joining them. It is taken
+  // for more than three thin tiles per sequence and KV head where those would
+  // fill the chip (then they run in turns; 8 sequences of 64 tokens x 8 heads over
+  // 500 tokens 38 us against 44, over 32 K 239 against 335) or where the work, at
+  // the sequences' capacity (only the GPU knows the lengths), is beyond 2^36
+  // operations. With D = 128, thin against wide, in us with the join: 2 x 16
+  // tokens over 2000 18 and 34, 4 x 32 over 8000 35 and 47, 2 x 64 over 32 K (2^36)
+  // 87 and 90, 4 x 64 over 32 K (2^37) 184 and 145; 64 rows per head over 32 K 48
+  // and 60, 96 rows 61 and 70.
+  const int64_t thin = TreeThin<128>::kRows;
+  L.wide = max_count * r > 3 * thin &&
+           (2 * tiles(thin) > slots(false) || (double)rows * hq * cap * dim * 4. > 0x1p36);
+  const int64_t tile = L.wide ? TreeWide<128>::kRows : thin, units = tiles(tile);
+  L.slots = slots(L.wide);
+  L.units = units;
   L.whole = units >= 4 * L.slots;
   L.grid = L.whole ? units : (2 * units <= L.slots ? L.slots : units + 2 * L.slots);
   L.grid = cdiv(L.grid, 8) * 8;  // whole runs per XCD
@@ -1092,9 +1146,19 @@ static int tree_launch(const TreeParams& p, const TreeLayout& L, hipStream_t s) 
     tree_run<TreeWide<D>>(tree_wide_kernel<D>, wide, p, L, s);
   else
     tree_run<TreeThin<D>>(tree_thin_kernel<D>, thin, p, L, s);
-  if (!L.whole)
-    hipLaunchKernelGGL(tree_combine_kernel<D>, dim3((unsigned)p.rows, (unsigned)cdiv(p.hq * D, 4 * kTreeThreads)),
-                       dim3(kTreeThreads), 0, s, p, L.wide ? TreeWide<D>::kRows : TreeThin<D>::kRows);
+  if (!L.whole) {
+    constexpr int kGroups = 4 * kTreeThreads / D;
+    // A group of lanes for every 8 of the chunks that a row is expected to have: one
+    // sequence's token over 32 K tokens 14.3 us with one group, 5.8 with eight; its
+    // tree of 16 26.6 and 11.0. (For every 4: 8 chunks 4.0 us against 3.7.)
+    const int64_t share = L.slots / L.units, most = cdiv(p.cap, L.wide ? TreeWide<D>::kStep : TreeThin<D>::kStep);
+    const int64_t chunks = share < most ? share : most;
+    int log_parts = 0;
+    while ((1 << log_parts) < kGroups && (16 << log_parts) <= chunks) ++log_parts;
+    const auto kernel = log_parts ? tree_combine_kernel<D, true> : tree_combine_kernel<D, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)p.rows, (unsigned)cdiv((int64_t)p.hq << log_parts, kGroups)),
+                       dim3(kTreeThreads), 0, s, p, L.wide ? TreeWide<D>::kRows : TreeThin<D>::kRows, log_parts);
+  }
   return check_launch("tree_attention");
 }
 
@@ -1107,8 +1171,12 @@ extern "C" size_t q6moe_tree_attn_workspace_size(int64_t batch, int64_t rows, in
                                                  int64_t page_size) {
   if (batch < 1 || rows < 1 || max_count < 1 || query_heads < 1 || kv_heads < 1 || pages_per_seq < 1 || page_size < 1)
     return 0;
-  if (query_heads % kv_heads || batch > 65535 || rows >= (1 << 24) || max_count >= (1 << 24)) return 0;
-  return tree_layout(batch, rows, max_count, query_heads, kv_heads, head_dim).total;
+  if (query_heads % kv_heads || query_heads > kTreeMaxHeads || batch > 65535 || rows >= (1 << 24) ||
+      max_count >= (1 << 24) || pages_per_seq >= (1 << 30) || page_size >= (1 << 30) ||
+      pages_per_seq * page_size > (1 << 30))
+    return 0;
+  return tree_layout(batch, rows, max_count, query_heads, kv_heads, head_dim,
+                     pages_per_seq * page_size).total;
 }
 
 extern "C" int q6moe_kv_tree_attention(const q6moe_tree_attn_args* a, void* stream) {
@@ -1135,8 +1203,8 @@ extern "C" int q6moe_kv_tree_attention(const q6moe_tree_attn_args* a, void* stre
   Q6MOE_REQUIRE(aligned(a->q, 16) && aligned(a->k_codes, 16) && aligned(a->v_codes, 16) && aligned(a->out, 16) &&
                     aligned(a->workspace, 256),
                 "tree_attention: q, codes and out need 16-byte and workspace 256-byte alignment");
-  const TreeLayout L =
-      tree_layout(a->batch, a->rows, a->max_count, a->query_heads, a->kv_heads, a->head_dim);
+  const TreeLayout L = tree_layout(a->batch, a->rows, a->max_count, a->query_heads, a->kv_heads, a->head_dim,
+                                   a->pages_per_seq * a->page_size);
   Q6MOE_REQUIRE(L.grid < (1ll << 31), "tree_attention: too many rows");
   if (a->workspace_bytes < L.total) {
     set_error("tree_attention: workspace too small (need " + std::to_string(L.total) + " bytes)");

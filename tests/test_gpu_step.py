@@ -194,7 +194,8 @@ def _attn(device, case, sees, *, q=None, scales_dtype=torch.float32, masks=None,
     return got.float().cpu().numpy()
 
 
-def _case(seed, lengths, counts, page, kvh, r, dim, extra=0, spare_pages=3, width=None, qscale=2.0):
+def _case(seed, lengths, counts, page, kvh, r, dim, extra=0, spare_pages=3, width=None, qscale=2.0, room=False):
+    """``room``: tables wide enough that calls of many rows are taken for large ones."""
     rng = np.random.default_rng(seed)
     batch, most = len(lengths), max(1, *counts)
     pps = width or max(-(-(n + c) // page) for n, c in zip(lengths, counts)) + 1
@@ -204,6 +205,9 @@ def _case(seed, lengths, counts, page, kvh, r, dim, extra=0, spare_pages=3, widt
     table = rng.permutation(pages)[:batch * pps].reshape(batch, pps).astype(np.int32)
     starts = np.concatenate([[0], np.cumsum(counts)])
     q = bf16_round((rng.standard_normal((max(1, int(starts[-1]) + extra), kvh * r, dim)) * qscale).astype(np.float32))
+    if room:
+        wide = 2**36 // (4 * q.size * page) + 1
+        table = np.concatenate([table, np.full((batch, wide), -1, np.int32)], 1)
     return k, ks, v, vs, table, lengths, starts, page, kvh, q, most
 
 
@@ -251,8 +255,9 @@ def _check(got, case, sees, rows=None, scales=None):
     (64, 1, 4, 128, [2500, 5000, 17], [7, 2, 3], 0),               # split over keys
 ])
 @pytest.mark.parametrize("kind", ["tree", "any", "chain"])
-def test_attention(device, page, kvh, r, dim, lengths, counts, extra, kind):
-    case = _case(len(lengths) * page + dim, lengths, counts, page, kvh, r, dim, extra)
+@pytest.mark.parametrize("room", [False, True], ids=["small", "large"])
+def test_attention(device, page, kvh, r, dim, lengths, counts, extra, kind, room):
+    case = _case(len(lengths) * page + dim, lengths, counts, page, kvh, r, dim, extra, room=room)
     rng = np.random.default_rng(7)
     sees = None if kind == "chain" else _sees(rng, counts, extra, 0.3 if kind == "any" else None)
     scales = torch.bfloat16 if kind == "any" else torch.float32
@@ -283,18 +288,21 @@ def test_attention_of_many_sequences(device, batch, kvh, r, dim, count, most_len
             _check(got[a:e], one, None)
 
 
-def test_attention_chain_of_a_prompt(device):
-    case = _case(3, [0, 300], [333, 130], 64, 2, 3, 128)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("room", [False, True], ids=["small", "large"])
+def test_attention_chain_of_a_prompt(device, dim, room):
+    case = _case(3, [0, 300], [333, 130], 64, 2, 3, dim, room=room)
     _check(_attn(device, case, None), case, None)
 
 
-FEW_AND_MANY = pytest.mark.parametrize("r", [4, 20])  # query heads per KV head: few rows, and many
+# query heads per KV head: few rows, and many; of these as small calls and as large ones
+FEW_AND_MANY = pytest.mark.parametrize("r,room", [(4, False), (20, False), (20, True)])
 
 
 @FEW_AND_MANY
-def test_attention_rows_that_see_nothing(device, r):
+def test_attention_rows_that_see_nothing(device, r, room):
     # no cached tokens, empty masks: 0; a mask that names tokens past the sequence's own names nothing
-    case = _case(11, [0, 0, 9], [3, 2, 9], 16, 2, r, 128)
+    case = _case(11, [0, 0, 9], [3, 2, 9], 16, 2, r, 128, room=room)
     sees = [set(), {2}, {0, 5, 63}, set(), {0}, set(), {1, 2, 40}, {8}, {0}, {3, 4}, set(), {7}, {6, 5}, {8, 2}]
     got = _attn(device, case, sees)
     _check(got, case, sees)
@@ -303,10 +311,10 @@ def test_attention_rows_that_see_nothing(device, r):
 
 
 @FEW_AND_MANY
-def test_attention_garbage_where_nothing_looks(device, r):
+def test_attention_garbage_where_nothing_looks(device, r, room):
     # scales of every place that no row sees are NaN or infinite, codes are -128
     lengths, counts = [70, 5], [6, 4]
-    case = _case(12, lengths, counts, 16, 2, r, 128)
+    case = _case(12, lengths, counts, 16, 2, r, 128, room=room)
     k, ks, v, vs, table = case[:5]
     sees = [s - {3} for s in _sees(np.random.default_rng(1), counts, 0)]
     held = np.zeros(ks.shape[:2], bool)
@@ -326,9 +334,9 @@ def test_attention_garbage_where_nothing_looks(device, r):
 
 
 @FEW_AND_MANY
-def test_attention_scales_far_apart(device, r):
+def test_attention_scales_far_apart(device, r, room):
     # values whose scales span 2^40, some of them 0, in an order that grows; scores far from 0
-    case = _case(13, [900], [8], 64, 1, r, 128, qscale=6.0)
+    case = _case(13, [900], [8], 64, 1, r, 128, qscale=6.0, room=room)
     k, ks, v, vs, table = case[:5]
     rng = np.random.default_rng(2)
     vs *= 2.0 ** rng.integers(-20, 21, vs.shape).astype(np.float32)
@@ -341,9 +349,9 @@ def test_attention_scales_far_apart(device, r):
 
 
 @FEW_AND_MANY
-def test_attention_queries_far_apart(device, r):
+def test_attention_queries_far_apart(device, r, room):
     # rows of queries from 2^-100 to 2^100 (with keys to match), one of zeros
-    case = _case(14, [130], [6], 64, 1, r, 128)
+    case = _case(14, [130], [6], 64, 1, r, 128, room=room)
     q = case[9]
     for i, e in enumerate((0, -100, -20, 3)):
         q[i] *= np.float32(2.0**e)
@@ -356,14 +364,23 @@ def test_attention_queries_far_apart(device, r):
 
 
 @FEW_AND_MANY
-def test_attention_unmapped_pages_and_short_tables(device, r):
+def test_attention_unmapped_pages_and_short_tables(device, r, room):
     # unmapped pages read as zero; tokens past the table's width are not seen
-    case = _case(15, [60, 40], [8, 8], 16, 2, r, 64, width=4)
+    case = _case(15, [60, 40], [8, 8], 16, 2, r, 64, width=4, room=room)
     k, ks, v, vs, table = case[:5]
     table[0, 1], table[1, 2] = -1, k.shape[0] + 4
     sees = _sees(np.random.default_rng(3), [8, 8], 0)
     _check(_attn(device, case, sees), case, sees)
     _check(_attn(device, case, None), case, None)
+
+
+def test_attention_short_tables_of_many_sequences(device):
+    # enough of them that 6 tokens of 20 heads are many rows; tokens 32 and on are not seen
+    lengths = [20 + b % 13 for b in range(60)]
+    case = _case(19, lengths, [6] * 60, 16, 2, 20, 64, width=2)
+    _check(_attn(device, case, None), case, None)
+    sees = _sees(np.random.default_rng(4), [6] * 60, 0)
+    _check(_attn(device, case, sees), case, sees)
 
 
 def test_attention_counts_past_max_count_and_strided_queries(device):
