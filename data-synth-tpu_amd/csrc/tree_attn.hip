@@ -23,6 +23,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTreeThreads = 256;
+constexpr int kTreeCus = 256;
 constexpr int kTreeMaxHeads = 65535;
 constexpr float kTreeFloor = -0x1p126f;  // running maximum before the first seen key
 constexpr float kTreeSlack = 8.f;        // a score may pass the running maximum by 2^8 before that is raised
@@ -131,6 +132,24 @@ __device__ __forceinline__ void tree_reach(const TreeParams& p, const TreeSeq& s
   const int to = s.len + (last < s.count ? last + 1 : s.count), seen = s.len + first + 1;
   *n = to < p.cap ? to : p.cap;
   *all = seen < p.cap ? seen : p.cap;
+}
+
+// The priority of a wave in turn ``turn``: the N workgroups of a CU, which start
+// with different turns, take the first place in turn. With equal priorities the
+// oldest of three ran ahead (6500 cycles a turn, the youngest 9300) and the last
+// ended alone: 64-token trees over 32 K tokens 243 us, with turns 230; 16-token
+// trees in the thin kernel 74.7 and 73.3.
+template <int N>
+__device__ __forceinline__ void tree_priority(int turn) {
+  const int k = turn % N;
+  if (k == 0)
+    __builtin_amdgcn_s_setprio(0);
+  else if (k == 1)
+    __builtin_amdgcn_s_setprio(1);
+  else if (k == 2)
+    __builtin_amdgcn_s_setprio(2);
+  else
+    __builtin_amdgcn_s_setprio(3);
 }
 
 struct TreeItem {
@@ -667,7 +686,9 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
     issue(i, i);
   }
   int stage = 0;
+  const int place = (int)(blockIdx.x >> 3) / (kTreeCus / 8);  // 32 CUs per XCD
   const auto advance = [&](int i) {
+    if (C::kPerCu > 1) tree_priority<C::kPerCu>(place + i);
     tree_wait_vm<(C::kStages - 2) * 2 * KS>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // reads of the stage that is written next
     put.put(p, keys, scales + (C::kStages == 2 ? stage : (stage + 1) % C::kStages) * (C::kScale / 4));
@@ -940,7 +961,9 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
 
   // Turn i: the tile's DMA has landed; all waves convert it, issue the next tile
   // into its place, and compute.
+  const int place = (int)(blockIdx.x >> 3) / (kTreeCus / 8);  // 32 CUs per XCD
   const auto advance = [&](int i) {
+    tree_priority<C::kPerCu>(place + i);
     tree_wait_vm<0>();
     put.put(p, keys, scales);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -1074,7 +1097,6 @@ __global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p
       u32x2{pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv)};
 }
 
-constexpr int kTreeCus = 256;
 
 struct TreeLayout {
   int wide;
