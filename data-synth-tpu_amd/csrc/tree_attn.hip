@@ -232,17 +232,21 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
       }
     keys = hi * STEP;
   }
-  // Workgroup i runs on XCD i % 8: each XCD takes a contiguous run of items, so
-  // that the tiles that share a chunk's keys share its L2
-  const int id = (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3));
+  const auto chunks = [&](const TreeSeq& s) { return units(s) * tree_chunks(s.n, keys); };
+  int upto = tree_wave_scan(chunks(mine));
+  const int total = p.batch <= 64 ? __builtin_amdgcn_readlane(upto, 63) : sum(0, chunks);
+  // Workgroup i runs on XCD i % 8: each XCD takes a contiguous run of the items, so
+  // that the tiles that share a chunk's keys share its L2; the runs are alike.
+  // (Starts that do not ascend can name more items than there are workgroups.)
+  const int most = (int)(gridDim.x >> 3), run = (total + 7) >> 3 < most ? (total + 7) >> 3 : most;
+  const int place = (int)(blockIdx.x >> 3);
+  const int id = (int)(blockIdx.x & 7) * run + place;
   it.id = id;
-  int base = 0;
   it.b = -1;
   it.keys = keys;
-  for (int b0 = 0; b0 < p.batch; b0 += 64) {  // 64 sequences at a time
-    const TreeSeq s = b0 == 0 ? mine : (b0 + lane < p.batch ? tree_seq(p, b0 + lane) : none);
-    const int n = units(s) * tree_chunks(s.n, keys);
-    const int upto = base + tree_wave_scan(n);
+  if (place >= run || id >= total) return false;
+  TreeSeq s = mine;
+  for (int b0 = 0;;) {  // 64 sequences at a time
     const uint64_t has = __ballot(id < upto);
     if (has) {
       const int at = __builtin_ctzll(has);
@@ -251,7 +255,7 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
       it.seq.count = __builtin_amdgcn_readlane(s.count, at);
       it.seq.len = __builtin_amdgcn_readlane(s.len, at);
       it.seq.n = __builtin_amdgcn_readlane(s.n, at);
-      const int first = __builtin_amdgcn_readlane(upto - n, at), in = id - first;
+      const int first = __builtin_amdgcn_readlane(upto - chunks(s), at), in = id - first;
       const int tiles = tree_tiles(p, it.seq, ROWS), row = in / tiles;
       it.tile = in - row * tiles;
       it.chunk = row / p.kvh;
@@ -259,10 +263,14 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
       if (threadIdx.x == 0 && in == 0) p.info[it.b] = first;
       break;
     }
-    base = __builtin_amdgcn_readlane(upto, 63);
+    b0 += 64;
+    if (b0 >= p.batch) return false;
+    const int base = __builtin_amdgcn_readlane(upto, 63);
+    s = b0 + lane < p.batch ? tree_seq(p, b0 + lane) : none;
+    upto = base + tree_wave_scan(chunks(s));
   }
   if (threadIdx.x == 0 && id == 0) p.info[p.batch] = keys;
-  return it.b >= 0;
+  return true;
 }
 
 // A tile's rows in LDS: key t lies in row tree_row(t), bits 0 and 2 of t exchanged,
@@ -428,12 +436,11 @@ struct TreeRow {
   // Channels 32 s + 16 h + [0, 16) in raw[s] of half wave h, with ``kHalves`` 8 h' +
   // [0, 8) of 16 channels in raw: the operands' order.
   template <bool kBytes>
-  __device__ __forceinline__ void load(const TreeParams& p, const TreeItem& it, int row, int h) {
+  __device__ __forceinline__ void ask(const TreeParams& p, const TreeItem& it, int row, int h) {
     live = row < it.seq.count * p.r;
     j = live ? row / p.r : 0;
     hh = live ? row - j * p.r : 0;
     const uint16_t* src = p.q + (int64_t)(it.seq.start + j) * p.q_stride + (int64_t)(it.kh * p.r + hh) * D;
-    u16x2 tops = {0, 0};  // the largest magnitudes' bits
 #pragma unroll
     for (int s = 0; s < D / 32; ++s)
 #pragma unroll
@@ -441,6 +448,9 @@ struct TreeRow {
         const int c = kBytes ? 32 * s + 16 * h + 8 * i : 32 * s + 16 * i + 8 * h;
         raw[s][i] = live ? *reinterpret_cast<const u32x4*>(src + c) : u32x4{0u, 0u, 0u, 0u};
       }
+  }
+  __device__ __forceinline__ void scale() {
+    u16x2 tops = {0, 0};  // the largest magnitudes' bits
 #pragma unroll
     for (int s = 0; s < D / 32; ++s)
 #pragma unroll
@@ -531,6 +541,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   TreeScales<C::kTile> put;
   const auto tile_at = [&](int i) { return c0 + (wave + 4 * i) * C::kTile; };
   keys.ask(p, tile_at(0));
+  TreeRow<D> row;
+  row.template ask<true>(p, it, it.tile * C::kRows + col, h);
   if (keys.pick) {
     if (wave == 0) tree_wanted(p, seq, wanted);
     __syncthreads();
@@ -553,8 +565,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   };
   issue(0, 0);
 
-  TreeRow<D> row;
-  row.template load<true>(p, it, it.tile * C::kRows + col, h);
+  row.scale();
   i32x4 qhi[KS], qlo[KS];
   {
     // v = q 2^(14-e) rounded into the low bits of 1.5 * 2^23 + v; its low byte is lo,
@@ -803,6 +814,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   TreeScales<T> put;
   const auto tile_at = [&](int i) { return c0 + i * T; };
   keys.ask(p, tile_at(0));
+  TreeRow<D> row;
+  row.template ask<false>(p, it, it.tile * C::kRows + wave * 32 + col, h);
   if (keys.pick) {
     if (wave == 0) tree_wanted(p, seq, wanted);
     __syncthreads();
@@ -827,8 +840,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   };
   issue(0);
 
-  TreeRow<D> row;
-  row.template load<false>(p, it, it.tile * C::kRows + wave * 32 + col, h);
+  row.scale();
   f16x8 q[KS][2];
   {
     const float up = __builtin_ldexpf(1.f, 14 - row.e);
