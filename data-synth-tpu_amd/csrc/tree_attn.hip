@@ -6,6 +6,23 @@
 //   p_t = exp(s_t - max s)
 //
 // with the INT8 codes kc, vc and the FP32 scales ks, vs of (token, KV head).
+//
+// One pass over the keys with the running maximum and sum of the softmax. A
+// workgroup takes a tile of the (new token, head of the group) rows of one sequence
+// and KV head and a chunk of its keys; where there are several chunks their FP32 sums
+// meet in a second kernel. How long the chunks are is found on the GPU, from lengths
+// that the host does not know. Tiles of keys come from the pages to LDS by DMA while
+// the tile before is worked on. Two kernels: one for few rows, bound by memory, and
+// one for many, bound by the vector ALU that turns scores into probabilities beside
+// the matrix cores. 8 sequences of 8 K to 32 K tokens, 4 KV heads of 128 channels, 8
+// query heads each: one token each 45 us (the cache at 4.5 TB/s but for 10 us before
+// the first and after the last keys), trees of 16 68 us, of 64 204 us (617 TFLOP/s).
+//
+// Scores are exact sums of FP32-scaled products of the stored codes but for the FP32
+// rounding; the rounding to fewer bits that there is: a probability times its value
+// scale to the 11 bits of FP16, the second product's operand (an eighth of the BF16
+// output's half step), and queries that are more than 2^6 (few rows) or 2^28 (many)
+// below their row's largest. Maxima, sums and all accumulators are FP32.
 #include <atomic>
 #include <type_traits>
 
@@ -82,7 +99,12 @@ struct TreeWide {
   static constexpr int kPerCu = D == 64 ? 4 : (D == 128 ? 3 : 2);
   static constexpr int kHalf = kTile * D;
   static constexpr int kScale = 2 * kTile * 4 + 16;
-  static constexpr int kLds = 2 * kHalf + 4 * kHalf + 4 * kScale + 32;  // a tile's codes, the same in FP16
+  // Of a wave's 2 D / 32 operands of queries, those in LDS. (With all of them in
+  // registers some spilled, and their reload waited for the DMA just issued: 8 x
+  // 64-token trees over 32 K tokens 261 us against 236.)
+  static constexpr int kQueries = D == 256 ? 2 : 0;
+  // a tile's codes, the same in FP16, scales, masks, queries
+  static constexpr int kLds = 2 * kHalf + 4 * kHalf + 4 * kScale + 32 + 4096 * kQueries;
   static_assert(kPerCu * kLds <= 160 * 1024, "tile");
 };
 
@@ -120,6 +142,13 @@ __device__ __forceinline__ int tree_tiles(const TreeParams& p, const TreeSeq& s,
   return (s.count * p.r + rows - 1) / rows;
 }
 __device__ __forceinline__ int tree_chunks(int n, int keys) { return n <= keys ? 1 : (n + keys - 1) / keys; }
+// Keys per chunk, in whole steps: alike, and never more than ``keys`` of tree_chunks,
+// as that is whole steps too; then no chunk is empty either. (Full chunks and a rest:
+// a chunk of 1024 tokens over 1000 cached ones 89 us against 78, over 8 K 240 and 225.)
+__device__ __forceinline__ int tree_span(int n, int chunks, int step) {
+  const int steps = (n + step - 1) / step;
+  return (steps + chunks - 1) / chunks * step;
+}
 // Keys that the rows of one tile reach, and those that all of them see.
 __device__ __forceinline__ void tree_reach(const TreeParams& p, const TreeSeq& s, int tile, int rows, int* n,
                                            int* all) {
@@ -167,9 +196,13 @@ __device__ __forceinline__ T tree_wave_reduce(T v, F f) {
   step(std::integral_constant<int, 0x4e>{});   // quad_perm [2,3,0,1]
   step(std::integral_constant<int, 0x124>{});  // row_ror:4
   step(std::integral_constant<int, 0x128>{});  // row_ror:8
-  const auto swap = [&](auto r) { v = f(__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1])); };
-  swap(__builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false));
-  swap(__builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false));
+  const auto swap = [&](auto r) {
+    v = f(__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1]));
+  };
+  uint32_t w = __builtin_bit_cast(uint32_t, v);
+  swap(__builtin_amdgcn_permlane16_swap(w, w, false, false));
+  w = __builtin_bit_cast(uint32_t, v);
+  swap(__builtin_amdgcn_permlane32_swap(w, w, false, false));
   return v;
 }
 
@@ -194,7 +227,7 @@ __device__ __forceinline__ int tree_wave_scan(int v) {
 // cut into chunks of at most ``keys`` keys: the least number that gives no more
 // chunks than the chip holds workgroups, so that all run at once and, whatever the
 // lengths, end together. Only the GPU knows the lengths. (Cut at the mean instead,
-// 64-token trees made 640 chunks for 512 places: 321 us against 236.) Where the
+// 64-token trees made 640 chunks for then 512 places: 321 us against 236.) Where the
 // tiles themselves fill half of the places or more, the chunks are half as long as
 // the mean share and run in turns.
 template <int ROWS, int STEP>
@@ -433,8 +466,9 @@ struct TreeRow {
   int e;      // exponent of the row's largest magnitude
   bool bad;   // an infinite or NaN query: NaN scores
   u32x4 raw[D / 32][2];
-  // Channels 32 s + 16 h + [0, 16) in raw[s] of half wave h, with ``kHalves`` 8 h' +
-  // [0, 8) of 16 channels in raw: the operands' order.
+  // raw[s][i] of half wave h: channels 32 s + 16 h + 8 i + [0, 8), the order of INT8
+  // operands, or 32 s + 16 i + 8 h + [0, 8), that of FP16 ones. The loads, and then
+  // what needs them.
   template <bool kBytes>
   __device__ __forceinline__ void ask(const TreeParams& p, const TreeItem& it, int row, int h) {
     live = row < it.seq.count * p.r;
@@ -503,13 +537,16 @@ __device__ __forceinline__ void tree_result(const TreeParams& p, const TreeItem&
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* dst = p.out + ((int64_t)(it.seq.start + j) * p.hq + it.kh * p.r + hh) * D;
   tree_runs<D>(acc, h, [&](int c, f32x4 v) {
-    *reinterpret_cast<u32x2*>(dst + c) = u32x2{pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv)};
+    const u32x2 y = {pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv)};
+    *reinterpret_cast<u32x2*>(dst + c) = y;
     return v;
   });
 }
 
 // ---------------------------------------------------------------------------
-// Few rows. Queries are 16-bit integers in two INT8 operands, q = (256 hi + lo)
+// Few rows. The waves have keys of their own and do not wait for each other; a turn
+// of 32 keys costs some 300 vector instructions, 16 exponentials and 16 MFMAs (128
+// channels). Queries are 16-bit integers in two INT8 operands, q = (256 hi + lo)
 // 2^(e-14): exact for values down to 2^-6 of the row's largest. So the INT8 codes
 // of the keys are matrix operands as they lie, and the sums are exact. The values'
 // codes + 128 enter the second product as FP16 subnormals, (code + 128) 2^-24, one
@@ -528,9 +565,10 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   const TreeSeq seq = it.seq;
   int n, n_all;
   tree_reach(p, seq, it.tile, C::kRows, &n, &n_all);
-  const int c0 = it.chunk * it.keys;
-  if (c0 > 0 && c0 >= n) return;
-  const int c1 = n - c0 < it.keys ? n : c0 + it.keys;
+  const int chunks = tree_chunks(n, it.keys);
+  if (it.chunk >= chunks) return;
+  const int span = tree_span(n, chunks, C::kStep), c0 = it.chunk * span;
+  const int c1 = n - c0 < span ? n : c0 + span;
   const int turns = (c1 - c0 + C::kStep - 1) / C::kStep;
 
   uint8_t* ring = smem + wave * (C::kStages * 2 * C::kHalf);
@@ -748,7 +786,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
     return to;
   };
   float all;
-  const float up = __builtin_amdgcn_exp2f(m - joint(col, &all)) * (0x1p24f / st.factor), shift = 128.f * psum * 0x1p-24f;
+  const float up = __builtin_amdgcn_exp2f(m - joint(col, &all)) * (0x1p24f / st.factor);
+  const float shift = 128.f * psum * 0x1p-24f;
   if (row.live)
     tree_runs<D>(acc, h, [&](int c, f32x4 v) {
 #pragma unroll
@@ -758,7 +797,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   __syncthreads();
   const int first = it.tile * C::kRows, left = seq.count * p.r - first;
   const int live = left < C::kRows ? left : C::kRows;
-  const bool split = tree_chunks(n, it.keys) > 1;
+  const bool split = chunks > 1;
   for (int i = threadIdx.x; i < live * (D / 4); i += kTreeThreads) {
     const int rr = i / (D / 4), c = i % (D / 4);
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
@@ -783,8 +822,15 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
 // Many rows. The four waves bring a tile's codes to FP16 together, (code) 2^-24,
 // exact, in the order of the matrix operands; each then works on its 32 rows.
 // Queries are FP16 too, scaled by a power of two: exact for values down to 2^-28
-// of the row's largest. A conversion by each wave for itself took a third of the
-// vector instructions; with it two workgroups shared a CU, now three.
+// of the row's largest. (A chunk of 1024 tokens over 8 K, 256-wide heads: 300 us in
+// the kernel for few rows, 235 here; with three workgroups per CU in place of two at
+// 128 channels, 64-token trees over 32 K 238 and 220.) With 128 channels, 64 keys cost
+// a wave some 450 vector instructions and 32 MFMAs, 1024 cycles of the matrix cores;
+// a SIMD needs 2600 cycles for them, in 81 % of which a vector instruction issues.
+// Measured and left: 64 rows per wave, which share the operands from LDS (registers
+// spill at 128 channels: 347 us against 247; at 64, two waves per SIMD, 294 against
+// 293); addresses within the tile held in registers (1 % faster at 128 channels, 4 %
+// slower at 256).
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_kernel(TreeParams p) {
@@ -798,9 +844,10 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   const TreeSeq seq = it.seq;
   int n, n_all;
   tree_reach(p, seq, it.tile, C::kRows, &n, &n_all);
-  const int c0 = it.chunk * it.keys;
-  if (c0 > 0 && c0 >= n) return;
-  const int c1 = n - c0 < it.keys ? n : c0 + it.keys;
+  const int chunks = tree_chunks(n, it.keys);
+  if (it.chunk >= chunks) return;
+  const int span = tree_span(n, chunks, C::kStep), c0 = it.chunk * span;
+  const int c1 = n - c0 < span ? n : c0 + span;
   const int turns = (c1 - c0 + T - 1) / T;
 
   uint8_t* kr = smem;                  // the codes as they lie in the cache
@@ -809,6 +856,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   uint8_t* vf = kf + 2 * C::kHalf;     // [16 keys][half][channel block][row] x 8 keys
   float* scales = reinterpret_cast<float*>(vf + 2 * C::kHalf + wave * C::kScale);
   uint64_t* wanted = reinterpret_cast<uint64_t*>(vf + 2 * C::kHalf + 4 * C::kScale);
+  uint8_t* ql = vf + 2 * C::kHalf + 4 * C::kScale + 32 + 1024 * C::kQueries * wave + 16 * lane;
   TreeLookup<T> keys{p.table + (int64_t)it.b * p.pps, wanted, c1, seq.len, it.kh, lane, p.masks && c1 > seq.len,
                      0, 0, 0, false};
   TreeScales<T> put;
@@ -850,6 +898,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int k = 0; k < 8; ++k) q[s][i][k] = (_Float16)(row.value(s, i, k) * up);
+#pragma unroll
+    for (int k = 0; k < C::kQueries; ++k) *reinterpret_cast<f16x8*>(ql + 1024 * k) = q[k >> 1][k & 1];
   }
   const float qf = row.bad ? __builtin_nanf("") : __builtin_ldexpf(p.to_log2, row.e + 10);
   const bool rows = it.tile * C::kRows + wave * 32 < seq.count * p.r;  // the wave has any
@@ -887,28 +937,28 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
     const uint32_t quad = tid % kLanes;
 #pragma unroll
     for (int k = 0; k < T / 4 * kLanes / kTreeThreads; ++k) {
-    const uint32_t four = tid / kLanes + k * (kTreeThreads / kLanes);  // keys 4 four + [0, 4)
-    uint32_t x[4][W];
+      const uint32_t four = tid / kLanes + k * (kTreeThreads / kLanes);  // keys 4 four + [0, 4)
+      uint32_t x[4][W];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint8_t* src = vr + tree_row(4 * four + i) * D + 4 * W * quad;
-      if constexpr (W == 2) {
-        const u32x2 y = *reinterpret_cast<const u32x2*>(src);
-        x[i][0] = y[0] ^ 0x80808080u;
-        x[i][1] = y[1] ^ 0x80808080u;
-      } else {
-        x[i][0] = *reinterpret_cast<const uint32_t*>(src) ^ 0x80808080u;
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* src = vr + tree_row(4 * four + i) * D + 4 * W * quad;
+        if constexpr (W == 2) {
+          const u32x2 y = *reinterpret_cast<const u32x2*>(src);
+          x[i][0] = y[0] ^ 0x80808080u;
+          x[i][1] = y[1] ^ 0x80808080u;
+        } else {
+          x[i][0] = *reinterpret_cast<const uint32_t*>(src) ^ 0x80808080u;
+        }
       }
-    }
-    // keys 4 four + i: 16 keys' block four / 4, half wave four & 1, operand place 4 (four / 2 & 1) + i
-    uint8_t* dst = vf + 16 * ((four >> 2) * 2 + (four & 1)) * KS * 32 + 8 * (four >> 1 & 1);
+      // keys 4 four + i: 16 keys' block four / 4, half wave four & 1, operand place 4 (four / 2 & 1) + i
+      uint8_t* dst = vf + 16 * ((four >> 2) * 2 + (four & 1)) * KS * 32 + 8 * (four >> 1 & 1);
 #pragma unroll
-    for (int b = 0; b < 4 * W; ++b) {
-      const uint32_t sel = 0x0c040c00u + (uint32_t)(b & 3) * 0x00010001u;
-      const u32x2 y = {half2(x[1][b >> 2], x[0][b >> 2], sel), half2(x[3][b >> 2], x[2][b >> 2], sel)};
-      const uint32_t c = D == 64 ? b & 1 : b, r = D == 64 ? quad + 16 * (b >> 1) : quad;
-      *reinterpret_cast<u32x2*>(dst + 16 * (c * 32 + r)) = y;
-    }
+      for (int b = 0; b < 4 * W; ++b) {
+        const uint32_t sel = 0x0c040c00u + (uint32_t)(b & 3) * 0x00010001u;
+        const u32x2 y = {half2(x[1][b >> 2], x[0][b >> 2], sel), half2(x[3][b >> 2], x[2][b >> 2], sel)};
+        const uint32_t c = D == 64 ? b & 1 : b, r = D == 64 ? quad + 16 * (b >> 1) : quad;
+        *reinterpret_cast<u32x2*>(dst + 16 * (c * 32 + r)) = y;
+      }
     }
   };
   const auto compute = [&](auto slow, int t0) {
@@ -922,8 +972,9 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
       for (int v = 0; v < 16; ++v) s[v] = 0.f;
 #pragma unroll
       for (int k = 0; k < 2 * KS; ++k)
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(kt + 16 * (2 * k * T + 32 * nb)),
-                                                   q[k >> 1][k & 1], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+            *reinterpret_cast<const f16x8*>(kt + 16 * (2 * k * T + 32 * nb)),
+            k < C::kQueries ? *reinterpret_cast<const f16x8*>(ql + 1024 * k) : q[k >> 1][k & 1], s, 0, 0, 0);
       uint32_t vis = 0;
       if constexpr (slow) vis = row.live ? tree_visible(p, seq, row.j, t0 + 32 * nb, c1, h) : 0u;
       float top = -__builtin_inff();
@@ -1001,7 +1052,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[c][v] *= up;
   if (row.live)
-    tree_result<D>(p, it, acc, tree_chunks(n, it.keys) > 1, st.m, l, row.j, row.hh,
+    tree_result<D>(p, it, acc, chunks > 1, st.m, l, row.j, row.hh,
                    (int64_t)it.id * C::kRows + wave * 32 + col, h);
 }
 
@@ -1048,12 +1099,14 @@ __global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p
   const int64_t step = (int64_t)p.kvh * tiles * tile_rows;
   // starts that do not ascend can name more tiles than the workspace has places for
   const bool live = head < p.hq && chunks > 1 && from >= 0 && first + (chunks - 1) * step < (int64_t)p.grid * tile_rows;
-  const int run = (chunks + parts - 1) >> log_parts, to_chunk = live ? (part + 1) * run < chunks ? (part + 1) * run : chunks : 0;
+  const int run = (chunks + parts - 1) >> log_parts, end_run = (part + 1) * run;
+  const int to_chunk = live ? (end_run < chunks ? end_run : chunks) : 0;
   float m = kTreeFloor, l = 0.f;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   for (int i0 = part * run; i0 < to_chunk; i0 += W) {
     const bool on = i0 + in < to_chunk;
-    const f32x2 st = on ? *reinterpret_cast<const f32x2*>(p.stat + 2 * (first + (i0 + in) * step)) : f32x2{kTreeFloor, 0.f};
+    const f32x2* from = reinterpret_cast<const f32x2*>(p.stat + 2 * (first + (i0 + in) * step));
+    const f32x2 st = on ? *from : f32x2{kTreeFloor, 0.f};
     float to = st[0];
 #pragma unroll
     for (int off = 1; off < W; off <<= 1) to = fmaxf(to, __shfl_xor(to, off));
