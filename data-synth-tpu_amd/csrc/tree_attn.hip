@@ -1196,13 +1196,15 @@ static TreeLayout tree_layout(int64_t batch, int64_t rows, int64_t max_count, in
   // fill the chip (then they run in turns; 8 sequences of 64 tokens x 8 heads over
   // 500 tokens 38 us against 44, over 32 K 239 against 335) or where the work, at
   // the sequences' capacity (only the GPU knows the lengths), is beyond 2^36
-  // operations. With D = 128, thin against wide, in us with the join: 2 x 16
+  // operations, 2^35 with D = 64, whose exponentials weigh more. With D = 128, thin against wide, in us with the join: 2 x 16
   // tokens over 2000 18 and 34, 4 x 32 over 8000 35 and 47, 2 x 64 over 32 K (2^36)
   // 87 and 90, 4 x 64 over 32 K (2^37) 184 and 145; 64 rows per head over 32 K 48
-  // and 60, 96 rows 61 and 70.
+  // and 60, 96 rows 61 and 70. With D = 64, 8 KV heads, 1 x 64 over 8000 31 and 40,
+  // 4 x 16 over 32 K (2^35) 66 and 58; with D = 256, 2 KV heads, 4 x 16 over 32 K
+  // (2^35) 64 and 72, 4 x 32 (2^36) 110 and 96.
   const int64_t thin = TreeThin<128>::kRows;
   L.wide = max_count * r > 3 * thin &&
-           (2 * tiles(thin) > slots(false) || (double)rows * hq * cap * dim * 4. > 0x1p36);
+           (2 * tiles(thin) > slots(false) || (double)rows * hq * cap * dim * 4. > (dim == 64 ? 0x1p35 : 0x1p36));
   const int64_t tile = L.wide ? TreeWide<128>::kRows : thin, units = tiles(tile);
   L.slots = slots(L.wide);
   L.units = units;
