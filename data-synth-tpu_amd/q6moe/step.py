@@ -28,7 +28,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _launch, _lib
-from .attention_cache import _dtype_code, _int32, _row_values
+from .attention_cache import _dtype_code, _int32
 
 MAX_TREE = 256  # new tokens of a sequence that masks tell apart
 
@@ -176,10 +176,11 @@ def _rows_of(x, rows, kv_heads, head_dim, device, name):
 
 
 def _pool_rows(pool, scales, chans, groups, device, name):
-    if pool.dtype is not torch.int8 or pool.ndim < 3 or pool.device != device or not pool.is_contiguous() or \
-            _row_values(pool) != chans:
+    shape = pool.shape
+    n = shape[0] * shape[1] if len(shape) > 2 else 0
+    if pool.dtype is not torch.int8 or not n or pool.device != device or not pool.is_contiguous() or \
+            pool.numel() != n * chans:
         raise ValueError(f"{name} pool must be contiguous int8 [pages, page_size, kv_heads * head_dim] on {device}")
-    n = pool.shape[0] * pool.shape[1]
     if scales.dtype not in (torch.bfloat16, torch.float32) or scales.device != device or \
             not scales.is_contiguous() or scales.numel() != n * groups:
         raise ValueError(f"{name} scales must be contiguous BF16 or FP32 [pages, page_size, {groups}] on {device}")
@@ -211,13 +212,13 @@ def write_tokens(k_pool, k_scales, v_pool, v_scales, key, value, slots, *, kv_he
     n = _pool_rows(k_pool, k_scales, chans, chans // group, device, "k")
     if _pool_rows(v_pool, v_scales, chans, chans // group, device, "v") != n or k_scales.dtype != v_scales.dtype:
         raise ValueError("the k and v pools must have the same size and scale type")
-    if n and (k_pool.data_ptr() == v_pool.data_ptr() or k_scales.data_ptr() == v_scales.data_ptr()):
+    if k_pool.data_ptr() == v_pool.data_ptr() or k_scales.data_ptr() == v_scales.data_ptr():
         raise ValueError("the k and v pools must not be the same memory")
     key, key_stride = _rows_of(key, rows, kv_heads, head_dim, device, "key")
     value, value_stride = _rows_of(value, rows, kv_heads, head_dim, device, "value")
     if key.dtype != value.dtype:
         raise ValueError("key and value must have the same type")
-    if rows == 0 or n == 0:
+    if rows == 0:
         return
     a = _lib.KvWriteRowsArgs(
         key.data_ptr(), value.data_ptr(), key_stride, value_stride, _dtype_code(key.dtype), k_pool.data_ptr(),
@@ -264,10 +265,10 @@ def paged_tree_attention(q, k_pool, k_scales, v_pool, v_scales, page_table, leng
             k_scales.dtype != v_scales.dtype:
         raise ValueError("the pools must be [pages, page_size, kv_heads * head_dim], of the same size and scale type")
     table, lens, first = _int32(page_table, device), _int32(lengths, device), _int32(starts, device)
-    if table.ndim != 2 or not table.shape[0] or not table.shape[1] or lens.shape != (table.shape[0],) or \
-            first.shape != (table.shape[0] + 1,):
+    shape = table.shape
+    if len(shape) != 2 or 0 in shape or lens.shape != shape[:1] or first.shape != (shape[0] + 1,):
         raise ValueError("page_table must be [batch, pages_per_seq], lengths [batch] and starts [batch + 1]")
-    batch, pps = table.shape
+    batch, pps = shape
     words = 0
     if masks is not None:
         if not isinstance(masks, torch.Tensor) or masks.ndim != 2 or masks.shape[0] != rows or \
