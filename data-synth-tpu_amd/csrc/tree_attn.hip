@@ -80,12 +80,11 @@ struct TreeThin {
   static constexpr int kRows = 32;    // (new token, head of the group) rows per workgroup
   static constexpr int kTile = 32;    // keys per tile of a wave
   static constexpr int kStep = 128;   // keys per turn of the workgroup
-  static constexpr int kStages = D > 64 ? 2 : 3;
   static constexpr int kPerCu = D > 128 ? 1 : 2;  // workgroups per CU
   static constexpr int kHalf = kTile * D;         // bytes of a tile's keys, and of its values
-  static constexpr int kScale = 2 * 32 * 4 + 16;  // per wave and stage: key and value scales, value factor
-  static constexpr int kRing = 4 * kStages * 2 * kHalf;
-  static constexpr int kLds = kRing + 4 * kStages * kScale + 32;  // and four words of masks
+  static constexpr int kScale = 2 * 32 * 4 + 16;  // per wave: a tile's key and value scales, value factor
+  static constexpr int kRing = 4 * 2 * 2 * kHalf;  // per wave a tile in work and one on its way
+  static constexpr int kLds = kRing + 4 * kScale + 32;  // and four words of masks
   static_assert(kPerCu * kLds <= 160 * 1024, "tile");
 };
 
@@ -571,9 +570,9 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   const int c1 = n - c0 < span ? n : c0 + span;
   const int turns = (c1 - c0 + C::kStep - 1) / C::kStep;
 
-  uint8_t* ring = smem + wave * (C::kStages * 2 * C::kHalf);
-  float* scales = reinterpret_cast<float*>(smem + C::kRing + wave * (C::kStages * C::kScale));
-  uint64_t* wanted = reinterpret_cast<uint64_t*>(smem + C::kRing + 4 * C::kStages * C::kScale);
+  uint8_t* ring = smem + wave * (4 * C::kHalf);
+  float* scales = reinterpret_cast<float*>(smem + C::kRing + wave * C::kScale);
+  uint64_t* wanted = reinterpret_cast<uint64_t*>(smem + C::kRing + 4 * C::kScale);
   TreeLookup<C::kTile> keys{p.table + (int64_t)it.b * p.pps, wanted, c1, seq.len, it.kh, lane,
                             p.masks && c1 > seq.len, 0, 0, 0, false};
   TreeScales<C::kTile> put;
@@ -643,7 +642,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   const auto compute = [&](auto slow, int t0, int stage) {
     const uint8_t* kt = ring + stage * 2 * C::kHalf + koff;
     const uint8_t* vt = ring + stage * 2 * C::kHalf + C::kHalf + voff;
-    const float* sc = scales + stage * (C::kScale / 4) + 4 * h;
+    const float* sc = scales + 4 * h;
     i32x16 hi, lo;
 #pragma unroll
     for (int v = 0; v < 16; ++v) hi[v] = lo[v] = 0;
@@ -726,22 +725,17 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
     }
   };
 
-  // Turn i issues the tile of turn i + kStages - 1; its scales reach LDS a turn
-  // later. Waits count DMA instructions: those of the tiles after this one may
-  // still be in flight. The waves work apart.
-#pragma unroll
-  for (int i = 1; i < C::kStages - 1; ++i) {
-    put.put(p, keys, scales + (i - 1) * (C::kScale / 4));
-    issue(i, i);
-  }
+  // Turn i: its tile has landed; the next is issued into the other half of the ring,
+  // whose reads are done. The waves work apart. (A third stage: at 64 channels 13.1 us
+  // against 12.5 for 24 trees of 5 over 3000 tokens, one token over 32 K 12.5 and 11.7.)
   int stage = 0;
   const int place = (int)(blockIdx.x >> 3) / (kTreeCus / 8);  // 32 CUs per XCD
   const auto advance = [&](int i) {
     if (C::kPerCu > 1) tree_priority<C::kPerCu>(place + i);
-    tree_wait_vm<(C::kStages - 2) * 2 * KS>();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // reads of the stage that is written next
-    put.put(p, keys, scales + (C::kStages == 2 ? stage : (stage + 1) % C::kStages) * (C::kScale / 4));
-    issue(i + C::kStages - 1, (stage + C::kStages - 1) % C::kStages);
+    tree_wait_vm<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and reads of the scales
+    put.put(p, keys, scales);
+    issue(i + 1, stage ^ 1);
   };
   // first the turns whose tile every row sees whole
   const int open = (n_all < c1 ? n_all : c1) - tile_at(0);
@@ -751,12 +745,12 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   for (; i < fast; ++i) {
     advance(i);
     compute(std::false_type{}, 0, stage);
-    stage = (stage + 1) % C::kStages;
+    stage ^= 1;
   }
   for (; i < turns; ++i) {
     advance(i);
     compute(std::true_type{}, tile_at(i), stage);
-    stage = (stage + 1) % C::kStages;
+    stage ^= 1;
   }
   tree_wait_vm<0>();
 
