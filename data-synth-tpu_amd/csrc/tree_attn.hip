@@ -21,8 +21,9 @@
 // Scores are exact sums of FP32-scaled products of the stored codes but for the FP32
 // rounding; the rounding to fewer bits that there is: a probability times its value
 // scale to the 11 bits of FP16, the second product's operand (an eighth of the BF16
-// output's half step), and queries that are more than 2^6 (few rows) or 2^28 (many)
-// below their row's largest. Maxima, sums and all accumulators are FP32.
+// output's half step), and query values that are more than 2^6 below their row's
+// largest (few rows) or 2^28 below that of 32 rows (many). Maxima, sums and all
+// accumulators are FP32.
 #include <atomic>
 #include <type_traits>
 
@@ -413,7 +414,9 @@ struct TreeLookup {
 template <int T>
 struct TreeScales {
   float factor = 1.f, limit = -1.f;  // of the newest tile
-  __device__ __forceinline__ void put(const TreeParams& p, const TreeLookup<T>& at, float* sc) {
+  // The key scales times ``unit`` 2^e.
+  __device__ __forceinline__ void put(const TreeParams& p, const TreeLookup<T>& at, float* sc, float unit = 1.f,
+                                      int e = 0) {
     const auto value = [&](uint32_t bits) {
       return at.on ? __builtin_bit_cast(float, p.scale_bf16 ? bits << 16 : bits) : 0.f;
     };
@@ -421,15 +424,15 @@ struct TreeScales {
     const float a = (T == 64 || at.lane >= 32) && fabsf(v) < __builtin_inff() ? fabsf(v) : 0.f;
     if (__any(a > limit)) {
       const float x = tree_wave_reduce(a, [](float c, float d) { return fmaxf(c, d); });
-      int e = (int)(__builtin_bit_cast(uint32_t, x) >> 23) - 127;
-      e = e < -110 ? -110 : e;
-      factor = __builtin_bit_cast(float, (uint32_t)(127 + 3 - e) << 23);  // 2^(3-e): at most 2^4 now
-      limit = __builtin_bit_cast(float, (uint32_t)(127 + e + 3 > 254 ? 254 : 127 + e + 3) << 23);
+      int ve = (int)(__builtin_bit_cast(uint32_t, x) >> 23) - 127;
+      ve = ve < -110 ? -110 : ve;
+      factor = __builtin_bit_cast(float, (uint32_t)(127 + 3 - ve) << 23);  // 2^(3-ve): at most 2^4 now
+      limit = __builtin_bit_cast(float, (uint32_t)(127 + ve + 3 > 254 ? 254 : 127 + ve + 3) << 23);
     }
     if (T == 32) {
-      sc[at.lane] = at.lane < 32 ? k : v * factor;
+      sc[at.lane] = at.lane < 32 ? __builtin_ldexpf(k * unit, e) : v * factor;
     } else {
-      sc[at.lane] = k;
+      sc[at.lane] = __builtin_ldexpf(k * unit, e);
       sc[T + at.lane] = v * factor;
     }
     if (at.lane == 0) sc[2 * T] = factor;
@@ -454,6 +457,30 @@ __device__ __forceinline__ void tree_raise(TreeState& st, float top, float facto
     st.factor = factor;
     st.m = to;
     st.l *= f;
+  }
+}
+
+// The same where scores come less the row's maximum so far (``t``): the maximum is
+// raised where one is beyond 2^8, and set by the row's first seen keys.
+struct TreeLevel {
+  float m = 0.f, l = 0.f, factor = 1.f;
+  float limit = -3.4028235e38f;  // kTreeSlack once m is set
+};
+template <typename F>
+__device__ __forceinline__ void tree_level(TreeLevel& st, float* t, float top, float factor, F&& fade) {
+  factor = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, factor)));
+  if (__any(top > st.limit) || factor != st.factor) {  // uniform over the wave
+    const float both = fmaxf(top, __shfl_xor(top, 32));
+    const bool on = both > st.limit;
+    const float to = on ? st.m + both : st.m, by = on ? to - st.m : 0.f;
+    const float f = st.limit < 0.f ? 1.f : __builtin_amdgcn_exp2f(-by);
+    fade(f * (factor / st.factor));
+    st.factor = factor;
+    st.m = to;
+    st.l *= f;
+    st.limit = on ? kTreeSlack : st.limit;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) t[v] -= by;
   }
 }
 
@@ -815,8 +842,10 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
 // ---------------------------------------------------------------------------
 // Many rows. The four waves bring a tile's codes to FP16 together, (code) 2^-24,
 // exact, in the order of the matrix operands; each then works on its 32 rows.
-// Queries are FP16 too, scaled by a power of two: exact for values down to 2^-28
-// of the row's largest. (A chunk of 1024 tokens over 8 K, 256-wide heads: 300 us in
+// Queries are FP16 too, scaled by a power of two that the wave's rows share, so that
+// it and 1 / sqrt(D) go into the keys' scales and one FMA gives a score less its row's
+// maximum (221 us against 228 for 64-token trees over 32 K tokens): exact for values
+// down to 2^-28 of the largest of the 32 rows, below that off by 2^-39 of it. (A chunk of 1024 tokens over 8 K, 256-wide heads: 300 us in
 // the kernel for few rows, 235 here; with three workgroups per CU in place of two at
 // 128 channels, 64-token trees over 32 K 238 and 220.) With 128 channels, 64 keys cost
 // a wave some 450 vector instructions and 32 MFMAs, 1024 cycles of the matrix cores;
@@ -883,9 +912,12 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   issue(0);
 
   row.scale();
+  // the largest of the wave's rows
+  const int e = __builtin_amdgcn_readfirstlane(
+      tree_wave_reduce(row.bad ? -110 : row.e, [](int a, int b) { return a > b ? a : b; }));
   f16x8 q[KS][2];
   {
-    const float up = __builtin_ldexpf(1.f, 14 - row.e);
+    const float up = row.bad ? __builtin_nanf("") : __builtin_ldexpf(1.f, 14 - e);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -895,7 +927,6 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
 #pragma unroll
     for (int k = 0; k < C::kQueries; ++k) *reinterpret_cast<f16x8*>(ql + 1024 * k) = q[k >> 1][k & 1];
   }
-  const float qf = row.bad ? __builtin_nanf("") : __builtin_ldexpf(p.to_log2, row.e + 10);
   const bool rows = it.tile * C::kRows + wave * 32 < seq.count * p.r;  // the wave has any
 
   f32x16 acc[KS];
@@ -903,7 +934,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   for (int c = 0; c < KS; ++c)
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[c][v] = 0.f;
-  TreeState st;
+  TreeLevel st;
 
   // The tile's codes into FP16: a key's 16 channels per thread and turn, then four
   // keys' D / 32 channels (of D = 64: 4). Code + 128 as a subnormal, less 128.
@@ -971,18 +1002,19 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
             k < C::kQueries ? *reinterpret_cast<const f16x8*>(ql + 1024 * k) : q[k >> 1][k & 1], s, 0, 0, 0);
       uint32_t vis = 0;
       if constexpr (slow) vis = row.live ? tree_visible(p, seq, row.j, t0 + 32 * nb, c1, h) : 0u;
-      float top = -__builtin_inff();
+      float t[16], top = -__builtin_inff();
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 ksv = *reinterpret_cast<const f32x4*>(sc + 32 * nb + 8 * g);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          s[4 * g + u] *= ksv[u];
-          if constexpr (slow) s[4 * g + u] = vis >> (8 * g + u) & 1 ? s[4 * g + u] : -__builtin_inff();
-          top = fmaxf(top, s[4 * g + u]);
+          const int v = 4 * g + u;
+          t[v] = __builtin_fmaf(s[v], ksv[u], -st.m);
+          if constexpr (slow) t[v] = vis >> (8 * g + u) & 1 ? t[v] : -__builtin_inff();
+          top = fmaxf(top, t[v]);
         }
       }
-      tree_raise(st, top * qf, sc[2 * T - 4 * h], [&](float f) {
+      tree_level(st, t, top, sc[2 * T - 4 * h], [&](float f) {
 #pragma unroll
         for (int c = 0; c < KS; ++c)
 #pragma unroll
@@ -996,14 +1028,14 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
           const f32x4 vsv = *reinterpret_cast<const f32x4*>(sc + T + 32 * nb + 16 * mm + 8 * g);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * mm + 4 * g + u], qf, -st.m));
-            float w = e * vsv[u];
+            const float x = __builtin_amdgcn_exp2f(t[8 * mm + 4 * g + u]);
+            float w = x * vsv[u];
             if constexpr (slow) {
               const bool on = vis >> (16 * mm + 8 * g + u) & 1;
-              st.l += on ? e : 0.f;
+              st.l += on ? x : 0.f;
               w = on ? w : 0.f;
             } else {
-              st.l += e;
+              st.l += x;
             }
             pv[4 * g + u] = (_Float16)w;
           }
@@ -1022,7 +1054,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   const auto advance = [&](int i) {
     tree_priority<C::kPerCu>(place + i);
     tree_wait_vm<0>();
-    put.put(p, keys, scales);
+    put.put(p, keys, scales, p.to_log2, e + 10);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     convert();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -1046,7 +1078,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[c][v] *= up;
   if (row.live)
-    tree_result<D>(p, it, acc, chunks > 1, st.m, l, row.j, row.hh,
+    tree_result<D>(p, it, acc, chunks > 1, st.limit < 0.f ? kTreeFloor : st.m, l, row.j, row.hh,
                    (int64_t)it.id * C::kRows + wave * 32 + col, h);
 }
 
