@@ -995,11 +995,17 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
       f32x16 s;
 #pragma unroll
       for (int v = 0; v < 16; ++v) s[v] = 0.f;
+      const auto key = [&](int k) { return *reinterpret_cast<const f16x8*>(kt + 16 * (2 * k * T + 32 * nb)); };
+      f16x8 a[2 * KS];
+      a[0] = key(0);
+      a[1] = key(1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int k = 0; k < 2 * KS; ++k)
+      for (int k = 0; k < 2 * KS; ++k) {
         s = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-            *reinterpret_cast<const f16x8*>(kt + 16 * (2 * k * T + 32 * nb)),
-            k < C::kQueries ? *reinterpret_cast<const f16x8*>(ql + 1024 * k) : q[k >> 1][k & 1], s, 0, 0, 0);
+            a[k], k < C::kQueries ? *reinterpret_cast<const f16x8*>(ql + 1024 * k) : q[k >> 1][k & 1], s, 0, 0, 0);
+        if (k + 2 < 2 * KS) a[k + 2] = key(k + 2);
+      }
       uint32_t vis = 0;
       if constexpr (slow) vis = row.live ? tree_visible(p, seq, row.j, t0 + 32 * nb, c1, h) : 0u;
       float t[16], top = -__builtin_inff();
@@ -1020,30 +1026,40 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
 #pragma unroll
           for (int v = 0; v < 16; ++v) acc[c][v] *= f;
       });
+      // Two operands of each sixteen keys' values are on their way before their
+      // probabilities are formed, and nothing is moved across: left to itself the
+      // scheduler read them one by one, each product waiting for LDS (64-token trees
+      // over 32 K tokens 221 us against 210; with four of them registers spill, 232).
 #pragma unroll
       for (int mm = 0; mm < 2; ++mm) {
+        const auto value = [&](int c) {
+          return *reinterpret_cast<const f16x8*>(vt + 16 * (((2 * nb + mm) * 2 * KS + c) * 32));
+        };
+        const f16x8 x[2] = {value(0), value(1)};
         f16x8 pv;
+        f32x4 vsv[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) vsv[g] = *reinterpret_cast<const f32x4*>(sc + T + 32 * nb + 16 * mm + 8 * g);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const f32x4 vsv = *reinterpret_cast<const f32x4*>(sc + T + 32 * nb + 16 * mm + 8 * g);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const float x = __builtin_amdgcn_exp2f(t[8 * mm + 4 * g + u]);
-            float w = x * vsv[u];
+            const float y = __builtin_amdgcn_exp2f(t[8 * mm + 4 * g + u]);
+            float w = y * vsv[g][u];
             if constexpr (slow) {
               const bool on = vis >> (16 * mm + 8 * g + u) & 1;
-              st.l += on ? x : 0.f;
+              st.l += on ? y : 0.f;
               w = on ? w : 0.f;
             } else {
-              st.l += x;
+              st.l += y;
             }
             pv[4 * g + u] = (_Float16)w;
           }
         }
 #pragma unroll
         for (int c = 0; c < KS; ++c)
-          acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-              *reinterpret_cast<const f16x8*>(vt + 16 * (((2 * nb + mm) * 2 * KS + c) * 32)), pv, acc[c], 0, 0, 0);
+          acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(c < 2 ? x[c & 1] : value(c), pv, acc[c], 0, 0, 0);
       }
     }
   };
