@@ -673,11 +673,14 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
     i32x16 hi, lo;
 #pragma unroll
     for (int v = 0; v < 16; ++v) hi[v] = lo[v] = 0;
+    i32x4 a[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) a[s] = *reinterpret_cast<const i32x4*>(kt + 16 * ((2 * s + h) ^ ksw));
+    __builtin_amdgcn_sched_barrier(0);  // all on their way before the first product
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const i32x4 a = *reinterpret_cast<const i32x4*>(kt + 16 * ((2 * s + h) ^ ksw));
-      hi = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qhi[s], hi, 0, 0, 0);
-      lo = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qlo[s], lo, 0, 0, 0);
+      hi = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[s], qhi[s], hi, 0, 0, 0);
+      lo = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[s], qlo[s], lo, 0, 0, 0);
     }
     uint32_t vis = 0;
     if constexpr (slow) vis = row.live ? tree_visible(p, seq, row.j, t0, c1, h) : 0u;
@@ -702,14 +705,32 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
     });
 #pragma unroll
     for (int mm = 0; mm < 2; ++mm) {  // 16 keys: 8 of each half wave
+      // the lane's channels of its half wave's 8 keys; byte b of two keys makes one
+      // operand word
+      constexpr int W = D == 256 ? 2 : 1;
+      uint32_t x[8][W];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint8_t* src = vt + (16 * mm + tree_row(8 * (i >> 2) + (i & 3))) * D;
+        if constexpr (W == 2) {
+          const u32x2 y = *reinterpret_cast<const u32x2*>(src);
+          x[i][0] = y[0];
+          x[i][1] = y[1];
+        } else {
+          x[i][0] = *reinterpret_cast<const uint32_t*>(src);
+        }
+      }
+      f32x4 vsv[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) vsv[g] = *reinterpret_cast<const f32x4*>(sc + 32 + 16 * mm + 8 * g);
+      __builtin_amdgcn_sched_barrier(0);  // the same: 16-token trees over 32 K tokens 72.3 us, 70.6 so
       f16x8 pv;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const f32x4 vsv = *reinterpret_cast<const f32x4*>(sc + 32 + 16 * mm + 8 * g);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(t[8 * mm + 4 * g + u], qf, -st.m));
-          float w = e * vsv[u];
+          float w = e * vsv[g][u];
           if constexpr (slow) {
             const bool on = vis >> (16 * mm + 8 * g + u) & 1;
             st.l += on ? e : 0.f;
@@ -725,21 +746,10 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
         const f16x2 one = {(_Float16)1.f, (_Float16)1.f}, pair = {pv[2 * u], pv[2 * u + 1]};
         psum = __builtin_amdgcn_fdot2(pair, one, psum, false);
       }
-      // the lane's channels of its half wave's 8 keys; byte b of two keys makes one
-      // operand word
-      constexpr int W = D == 256 ? 2 : 1;
-      uint32_t x[8][W];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint8_t* src = vt + (16 * mm + tree_row(8 * (i >> 2) + (i & 3))) * D;
-        if constexpr (W == 2) {
-          const u32x2 y = *reinterpret_cast<const u32x2*>(src);
-          x[i][0] = y[0] ^ 0x80808080u;
-          x[i][1] = y[1] ^ 0x80808080u;
-        } else {
-          x[i][0] = *reinterpret_cast<const uint32_t*>(src) ^ 0x80808080u;
-        }
-      }
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int w = 0; w < W; ++w) x[i][w] ^= 0x80808080u;
 #pragma unroll
       for (int c = 0; c < KS; ++c) {
         u32x4 a;
@@ -841,19 +851,19 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
 
 // ---------------------------------------------------------------------------
 // Many rows. The four waves bring a tile's codes to FP16 together, (code) 2^-24,
-// exact, in the order of the matrix operands; each then works on its 32 rows.
-// Queries are FP16 too, scaled by a power of two that the wave's rows share, so that
-// it and 1 / sqrt(D) go into the keys' scales and one FMA gives a score less its row's
-// maximum (221 us against 228 for 64-token trees over 32 K tokens): exact for values
-// down to 2^-28 of the largest of the 32 rows, below that off by 2^-39 of it. (A chunk of 1024 tokens over 8 K, 256-wide heads: 300 us in
-// the kernel for few rows, 235 here; with three workgroups per CU in place of two at
-// 128 channels, 64-token trees over 32 K 238 and 220.) With 128 channels, 64 keys cost
-// a wave some 450 vector instructions and 32 MFMAs, 1024 cycles of the matrix cores;
-// a SIMD needs 2600 cycles for them, in 81 % of which a vector instruction issues.
-// Measured and left: 64 rows per wave, which share the operands from LDS (registers
-// spill at 128 channels: 347 us against 247; at 64, two waves per SIMD, 294 against
-// 293); addresses within the tile held in registers (1 % faster at 128 channels, 4 %
-// slower at 256).
+// exact, in the order of the matrix operands; each then works on its 32 rows. Queries
+// are FP16 too, scaled by a power of two that the wave's rows share, so that it and 1
+// / sqrt(D) go into the keys' scales and one FMA gives a score less its row's maximum
+// (221 us against 228 for 64-token trees over 32 K tokens): exact for values down to
+// 2^-28 of the largest of the 32 rows, below that off by 2^-39 of it. (A chunk of 1024
+// tokens over 8 K, 256-wide heads: 300 us in the kernel for few rows, 235 here; with
+// three workgroups per CU in place of two at 128 channels, 64-token trees over 32 K
+// 238 and 220.) With 128 channels, 64 keys cost a wave some 450 vector instructions
+// and 32 MFMAs, 1024 cycles of the matrix cores; a SIMD needs 2600 cycles for them, in
+// 81 % of which a vector instruction issues. Measured and left: 64 rows per wave,
+// which share the operands from LDS (registers spill at 128 channels: 347 us against
+// 247; at 64, two waves per SIMD, 294 against 293); addresses within the tile held in
+// registers (1 % faster at 128 channels, 4 % slower at 256).
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_kernel(TreeParams p) {
@@ -975,7 +985,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
           x[i][0] = *reinterpret_cast<const uint32_t*>(src) ^ 0x80808080u;
         }
       }
-      // keys 4 four + i: 16 keys' block four / 4, half wave four & 1, operand place 4 (four / 2 & 1) + i
+      // keys 4 four + i: 16 keys' block four / 4, half wave four & 1, operand place 4
+      // (four / 2 & 1) + i
       uint8_t* dst = vf + 16 * ((four >> 2) * 2 + (four & 1)) * KS * 32 + 8 * (four >> 1 & 1);
 #pragma unroll
       for (int b = 0; b < 4 * W; ++b) {
@@ -1233,17 +1244,17 @@ static TreeLayout tree_layout(int64_t batch, int64_t rows, int64_t max_count, in
            (dim == 64 ? tree_per_cu<64>(wide) : (dim == 128 ? tree_per_cu<128>(wide) : tree_per_cu<256>(wide)));
   };
   // The wide kernel has the higher rate, but its workgroups' partial sums are four
-  // times as many bytes: some 25 us more for writing and joining them. It is taken
-  // for more than three thin tiles per sequence and KV head where those would
-  // fill the chip (then they run in turns; 8 sequences of 64 tokens x 8 heads over
-  // 500 tokens 38 us against 44, over 32 K 239 against 335) or where the work, at
-  // the sequences' capacity (only the GPU knows the lengths), is beyond 2^36
-  // operations, 2^35 with D = 64, whose exponentials weigh more. With D = 128, thin against wide, in us with the join: 2 x 16
-  // tokens over 2000 18 and 34, 4 x 32 over 8000 35 and 47, 2 x 64 over 32 K (2^36)
-  // 87 and 90, 4 x 64 over 32 K (2^37) 184 and 145; 64 rows per head over 32 K 48
-  // and 60, 96 rows 61 and 70. With D = 64, 8 KV heads, 1 x 64 over 8000 31 and 40,
-  // 4 x 16 over 32 K (2^35) 66 and 58; with D = 256, 2 KV heads, 4 x 16 over 32 K
-  // (2^35) 64 and 72, 4 x 32 (2^36) 110 and 96.
+  // times as many bytes: some 25 us more for writing and joining them. It is taken for
+  // more than three thin tiles per sequence and KV head where those would fill the
+  // chip (then they run in turns; 8 sequences of 64 tokens x 8 heads over 500 tokens
+  // 38 us against 44, over 32 K 239 against 335) or where the work, at the sequences'
+  // capacity (only the GPU knows the lengths), is beyond 2^36 operations, 2^35 with D
+  // = 64, whose exponentials weigh more. With D = 128, thin against wide, in us with
+  // the join: 2 x 16 tokens over 2000 18 and 34, 4 x 32 over 8000 35 and 47, 2 x 64
+  // over 32 K (2^36) 87 and 90, 4 x 64 over 32 K (2^37) 184 and 145; 64 rows per head
+  // over 32 K 48 and 60, 96 rows 61 and 70. With D = 64, 8 KV heads, 1 x 64 over 8000
+  // 31 and 40, 4 x 16 over 32 K (2^35) 66 and 58; with D = 256, 2 KV heads, 4 x 16
+  // over 32 K (2^35) 64 and 72, 4 x 32 (2^36) 110 and 96.
   const int64_t thin = TreeThin<128>::kRows;
   L.wide = max_count * r > 3 * thin &&
            (2 * tiles(thin) > slots(false) || (double)rows * hq * cap * dim * 4. > (dim == 64 ? 0x1p35 : 0x1p36));
