@@ -15,8 +15,8 @@
 // the tile before is worked on. Two kernels: one for few rows, bound by memory, and
 // one for many, bound by the vector ALU that turns scores into probabilities beside
 // the matrix cores. 8 sequences of 8 K to 32 K tokens, 4 KV heads of 128 channels, 8
-// query heads each: one token each 45 us (the cache at 4.5 TB/s but for 10 us before
-// the first and after the last keys), trees of 16 68 us, of 64 204 us (617 TFLOP/s).
+// query heads each: one token each 47 us (the cache at 4.5 TB/s but for 10 us before
+// the first and after the last keys), trees of 16 70 us, of 64 199 us (634 TFLOP/s).
 //
 // Scores are exact sums of FP32-scaled products of the stored codes but for the FP32
 // rounding; the rounding to fewer bits that there is: a probability times its value
@@ -858,9 +858,9 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
 // 2^-28 of the largest of the 32 rows, below that off by 2^-39 of it. (A chunk of 1024
 // tokens over 8 K, 256-wide heads: 300 us in the kernel for few rows, 235 here; with
 // three workgroups per CU in place of two at 128 channels, 64-token trees over 32 K
-// 238 and 220.) With 128 channels, 64 keys cost a wave some 450 vector instructions
-// and 32 MFMAs, 1024 cycles of the matrix cores; a SIMD needs 2600 cycles for them, in
-// 81 % of which a vector instruction issues. Measured and left: 64 rows per wave,
+// 238 and 220.) With 128 channels, 64 keys cost a wave some 350 vector instructions
+// and 32 MFMAs, 1024 cycles of the matrix cores; a vector instruction issues in 61 %
+// of a SIMD's cycles and the matrix cores work in 33 %. Measured and left: 64 rows per wave,
 // which share the operands from LDS (registers spill at 128 channels: 347 us against
 // 247; at 64, two waves per SIMD, 294 against 293); addresses within the tile held in
 // registers (1 % faster at 128 channels, 4 % slower at 256).
