@@ -70,7 +70,8 @@ struct TreeParams {
   float to_log2;   // log2(e) / sqrt(D)
   float* part;     // [workgroup][row of the tile][D] partial sums
   float* stat;     // [workgroup][row of the tile][2]: maximum (log2) and sum
-  int32_t* info;   // [batch + 1]: first workgroup of each sequence; at [batch] the keys per workgroup
+  int32_t* info;   // [batch + 2]: first item of each sequence; at [batch] the keys per item, then the items
+  int32_t* whose;  // of many sequences: each item's
   uint16_t* out;
 };
 
@@ -222,87 +223,142 @@ __device__ __forceinline__ int tree_wave_scan(int v) {
   return v;
 }
 
-// The workgroup's item, found by each wave for itself (lane t takes the sequences
-// t, t + 64, ..). The call's work, sum over sequences of tiles x heads x keys, is
-// cut into chunks of at most ``keys`` keys: the least number that gives no more
-// chunks than the chip holds workgroups, so that all run at once and, whatever the
-// lengths, end together. Only the GPU knows the lengths. (Cut at the mean instead,
-// 64-token trees made 640 chunks for then 512 places: 321 us against 236.) Where the
-// tiles themselves fill half of the places or more, the chunks are half as long as
-// the mean share and run in turns.
+// The call's work, sum over sequences of tiles x heads x keys, is cut into chunks of
+// at most ``keys`` keys: the least number that gives no more chunks than the chip
+// holds workgroups, so that all run at once and, whatever the lengths, end together.
+// Only the GPU knows the lengths. (Cut at the mean instead, 64-token trees made 640
+// chunks for then 512 places: 321 us against 236.) Where the tiles themselves fill
+// half of the places or more, the chunks are half as long as the mean share and run
+// in turns. ``sum(zero, f)`` is the sum of f over the sequences.
+template <int ROWS, int STEP, typename S>
+__device__ __forceinline__ int tree_keys(const TreeParams& p, S&& sum) {
+  if (p.whole) return 1 << 30;
+  const auto units = [&](const TreeSeq& s) { return tree_tiles(p, s, ROWS) * p.kvh; };
+  const float total = sum(0.f, [&](const TreeSeq& s) { return (float)units(s) * (float)s.n; });
+  const int tiles = sum(0, units);
+  const bool once = 2 * tiles <= p.slots;
+  int lo = (int)(total / (float)(once ? p.slots : 2 * p.slots) * (1.f / STEP));
+  lo = lo < 1 ? 1 : (lo < (1 << 30) / STEP / 2 - 1 ? lo : (1 << 30) / STEP / 2 - 1);
+  // in steps; hi gives few enough chunks: each tile has at most one that is not full
+  const float sure = total / (float)(p.slots - tiles) * (1.00001f / STEP);
+  int hi = once ? (sure < (float)(1 << 30) / STEP - 1.f ? (int)sure : (1 << 30) / STEP - 1) + 1 : lo + 1;
+  // few tiles: hi is within an eighth of the least
+  if (once && 8 * tiles > p.slots)
+    for (int i = 0; i < 5 && lo < hi; ++i) {
+      const int mid = (lo + hi) >> 1;
+      // at least the number of chunks: a rounded quotient, raised by 2^-20
+      const float per = 1.000001f / (float)(mid * STEP);
+      const int n = sum(0, [&](const TreeSeq& s) { return units(s) * ((int)((float)s.n * per) + 1); });
+      if (n <= p.slots)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+  return hi * STEP;
+}
+
+// Items of a sequence: chunks x KV heads x tiles, tiles fastest.
+template <int ROWS>
+__device__ __forceinline__ int tree_items(const TreeParams& p, const TreeSeq& s, int keys) {
+  return tree_tiles(p, s, ROWS) * p.kvh * tree_chunks(s.n, keys);
+}
+
+// More sequences than a wave has lanes: one workgroup finds the items for all others
+// in one launch more, 4.3 us. One token each, every wave for itself and so: 65
+// sequences of up to 4 K tokens 45.0 and 47.1 us, 256 of 1000 58.0 and 52.8, 600 of
+// 300 71 and 52, 2000 of 200 358 and 132.
+constexpr int kTreeLanes = 64, kTreePlan = 1024;
+template <int ROWS, int STEP>
+__global__ void __launch_bounds__(kTreePlan) tree_plan_kernel(TreeParams p) {
+  __shared__ int lds[kTreePlan / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const auto sum = [&](auto zero, auto of) {
+    auto v = zero;
+    for (int b = threadIdx.x; b < p.batch; b += kTreePlan) v += of(tree_seq(p, b));
+    v = tree_wave_reduce(v, [](auto x, auto y) { return x + y; });
+    __syncthreads();  // lds may still be read
+    if (lane == 0) lds[wave] = __builtin_bit_cast(int, v);
+    __syncthreads();
+    v = zero;
+    for (int w = 0; w < kTreePlan / 64; ++w) v += __builtin_bit_cast(decltype(v), lds[w]);
+    return v;
+  };
+  const int keys = tree_keys<ROWS, STEP>(p, sum);
+  int base = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += kTreePlan) {
+    const int b = b0 + (int)threadIdx.x;
+    const int n = b < p.batch ? tree_items<ROWS>(p, tree_seq(p, b), keys) : 0;
+    const int upto = tree_wave_scan(n);
+    __syncthreads();
+    if (lane == 63) lds[wave] = upto;
+    __syncthreads();
+    int first = base + upto - n;
+    for (int w = 0; w < kTreePlan / 64; ++w) {
+      first += w < wave ? lds[w] : 0;
+      base += lds[w];
+    }
+    if (b < p.batch) {
+      p.info[b] = first;
+      for (int i = first < 0 ? 0 : first; i < first + n && i < p.grid; ++i) p.whose[i] = b;
+    }
+  }
+  if (threadIdx.x == 0) {
+    p.info[p.batch] = keys;
+    p.info[p.batch + 1] = base;
+  }
+}
+
+// The workgroup's item, from tree_plan_kernel or, of up to 64 sequences, found by each
+// wave for itself, a lane for each.
 template <int ROWS, int STEP>
 __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
   const int lane = threadIdx.x & 63;
-  const TreeSeq none{0, 0, 0, 0}, mine = lane < p.batch ? tree_seq(p, lane) : none;
-  const auto units = [&](const TreeSeq& s) { return tree_tiles(p, s, ROWS) * p.kvh; };
-  const auto sum = [&](auto zero, auto of) {
-    auto v = lane < p.batch ? of(mine) : zero;
-    for (int b = lane + 64; b < p.batch; b += 64) v += of(tree_seq(p, b));
-    v = tree_wave_reduce(v, [](auto x, auto y) { return x + y; });
-    return __builtin_bit_cast(decltype(v), __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
-  };
-  int keys = 1 << 30;
-  if (!p.whole) {
-    const float total = sum(0.f, [&](const TreeSeq& s) { return (float)units(s) * (float)s.n; });
-    const int tiles = sum(0, units);
-    const bool once = 2 * tiles <= p.slots;
-    int lo = (int)(total / (float)(once ? p.slots : 2 * p.slots) * (1.f / STEP));
-    lo = lo < 1 ? 1 : (lo < (1 << 30) / STEP / 2 - 1 ? lo : (1 << 30) / STEP / 2 - 1);
-    // in steps; hi gives few enough chunks: each tile has at most one that is not full
-    const float sure = total / (float)(p.slots - tiles) * (1.00001f / STEP);
-    int hi = once ? (sure < (float)(1 << 30) / STEP - 1.f ? (int)sure : (1 << 30) / STEP - 1) + 1 : lo + 1;
-    // few tiles: hi is within an eighth of the least
-    if (once && 8 * tiles > p.slots && p.batch <= 256)
-      for (int i = 0; i < 5 && lo < hi; ++i) {
-        const int mid = (lo + hi) >> 1;
-        // at least the number of chunks: a rounded quotient, raised by 2^-20
-        const float per = 1.000001f / (float)(mid * STEP);
-        const int n = sum(0, [&](const TreeSeq& s) { return units(s) * ((int)((float)s.n * per) + 1); });
-        if (n <= p.slots)
-          hi = mid;
-        else
-          lo = mid + 1;
-      }
-    keys = hi * STEP;
+  TreeSeq mine{0, 0, 0, 0};
+  int upto = 0, n = 0, total;
+  if (p.whose) {
+    it.keys = p.info[p.batch];
+    total = p.info[p.batch + 1];
+  } else {
+    if (lane < p.batch) mine = tree_seq(p, lane);
+    it.keys = tree_keys<ROWS, STEP>(p, [&](auto zero, auto of) {
+      auto v = of(mine);
+      v = tree_wave_reduce(v, [](auto x, auto y) { return x + y; });
+      return __builtin_bit_cast(decltype(v), __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+    });
+    n = tree_items<ROWS>(p, mine, it.keys);
+    upto = tree_wave_scan(n);
+    total = __builtin_amdgcn_readlane(upto, 63);
   }
-  const auto chunks = [&](const TreeSeq& s) { return units(s) * tree_chunks(s.n, keys); };
-  int upto = tree_wave_scan(chunks(mine));
-  const int total = p.batch <= 64 ? __builtin_amdgcn_readlane(upto, 63) : sum(0, chunks);
   // Workgroup i runs on XCD i % 8: each XCD takes a contiguous run of the items, so
   // that the tiles that share a chunk's keys share its L2; the runs are alike.
   // (Starts that do not ascend can name more items than there are workgroups.)
   const int most = (int)(gridDim.x >> 3), run = (total + 7) >> 3 < most ? (total + 7) >> 3 : most;
   const int place = (int)(blockIdx.x >> 3);
   const int id = (int)(blockIdx.x & 7) * run + place;
-  it.id = id;
-  it.b = -1;
-  it.keys = keys;
   if (place >= run || id >= total) return false;
-  TreeSeq s = mine;
-  for (int b0 = 0;;) {  // 64 sequences at a time
-    const uint64_t has = __ballot(id < upto);
-    if (has) {
-      const int at = __builtin_ctzll(has);
-      it.b = b0 + at;
-      it.seq.start = __builtin_amdgcn_readlane(s.start, at);
-      it.seq.count = __builtin_amdgcn_readlane(s.count, at);
-      it.seq.len = __builtin_amdgcn_readlane(s.len, at);
-      it.seq.n = __builtin_amdgcn_readlane(s.n, at);
-      const int first = __builtin_amdgcn_readlane(upto - chunks(s), at), in = id - first;
-      const int tiles = tree_tiles(p, it.seq, ROWS), row = in / tiles;
-      it.tile = in - row * tiles;
-      it.chunk = row / p.kvh;
-      it.kh = row - it.chunk * p.kvh;
-      if (threadIdx.x == 0 && in == 0) p.info[it.b] = first;
-      break;
-    }
-    b0 += 64;
-    if (b0 >= p.batch) return false;
-    const int base = __builtin_amdgcn_readlane(upto, 63);
-    s = b0 + lane < p.batch ? tree_seq(p, b0 + lane) : none;
-    upto = base + tree_wave_scan(chunks(s));
+  it.id = id;
+  int first;
+  if (p.whose) {
+    const int b = p.whose[id];
+    it.b = b < 0 || b >= p.batch ? 0 : b;  // as for the items that no workgroup has
+    it.seq = tree_seq(p, it.b);
+    first = p.info[it.b];
+  } else {
+    it.b = __builtin_ctzll(__ballot(id < upto));
+    it.seq.start = __builtin_amdgcn_readlane(mine.start, it.b);
+    it.seq.count = __builtin_amdgcn_readlane(mine.count, it.b);
+    it.seq.len = __builtin_amdgcn_readlane(mine.len, it.b);
+    it.seq.n = __builtin_amdgcn_readlane(mine.n, it.b);
+    first = __builtin_amdgcn_readlane(upto - n, it.b);
+    if (threadIdx.x == 0 && id == first) p.info[it.b] = first;
+    if (threadIdx.x == 0 && id == 0) p.info[p.batch] = it.keys;
   }
-  if (threadIdx.x == 0 && id == 0) p.info[p.batch] = keys;
+  const int in = id - first, tiles = tree_tiles(p, it.seq, ROWS);
+  if (in < 0 || tiles < 1) return false;
+  const int row = in / tiles;
+  it.tile = in - row * tiles;
+  it.chunk = row / p.kvh;
+  it.kh = row - it.chunk * p.kvh;
   return true;
 }
 
@@ -937,6 +993,11 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
 #pragma unroll
     for (int k = 0; k < C::kQueries; ++k) *reinterpret_cast<f16x8*>(ql + 1024 * k) = q[k >> 1][k & 1];
   }
+  // the lane's row, formed anew where registers are short: at 128 channels two more
+  // made a query operand spill, and its reload wait for the DMA (210 us became 230)
+  const auto which = [&] {
+    return it.tile * C::kRows + wave * 32 + (int)((D == 128 ? tree_opaque(lane) : (uint32_t)lane) & 31);
+  };
   const bool rows = it.tile * C::kRows + wave * 32 < seq.count * p.r;  // the wave has any
 
   f32x16 acc[KS];
@@ -1018,7 +1079,10 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
         if (k + 2 < 2 * KS) a[k + 2] = key(k + 2);
       }
       uint32_t vis = 0;
-      if constexpr (slow) vis = row.live ? tree_visible(p, seq, row.j, t0 + 32 * nb, c1, h) : 0u;
+      if constexpr (slow) {
+        const int i = which();
+        vis = i < seq.count * p.r ? tree_visible(p, seq, i / p.r, t0 + 32 * nb, c1, h) : 0u;
+      }
       float t[16], top = -__builtin_inff();
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -1104,8 +1168,9 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   for (int c = 0; c < KS; ++c)
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[c][v] *= up;
-  if (row.live)
-    tree_result<D>(p, it, acc, chunks > 1, st.limit < 0.f ? kTreeFloor : st.m, l, row.j, row.hh,
+  const int at = which();
+  if (at < seq.count * p.r)
+    tree_result<D>(p, it, acc, chunks > 1, st.limit < 0.f ? kTreeFloor : st.m, l, at / p.r, at % p.r,
                    (int64_t)it.id * C::kRows + wave * 32 + col, h);
 }
 
@@ -1221,7 +1286,7 @@ struct TreeLayout {
   int slots, whole;
   int64_t units;  // row tiles x KV heads, at most
   int64_t grid;   // at most so many workgroups have work
-  size_t info, stat, part, total;
+  size_t info, whose, stat, part, total;
 };
 
 static size_t tree_align(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -1266,7 +1331,8 @@ static TreeLayout tree_layout(int64_t batch, int64_t rows, int64_t max_count, in
   L.grid = cdiv(L.grid, 8) * 8;  // whole runs per XCD
   const int64_t parts = L.whole ? 0 : L.grid * tile;
   L.info = 0;
-  L.stat = tree_align(L.info + (size_t)(batch + 1) * 4);
+  L.whose = tree_align(L.info + (size_t)(batch + 2) * 4);
+  L.stat = tree_align(L.whose + (batch > kTreeLanes ? (size_t)L.grid * 4 : 0));
   L.part = tree_align(L.stat + (size_t)parts * 8);
   L.total = tree_align(L.part + (size_t)parts * dim * 4);
   return L;
@@ -1278,6 +1344,7 @@ static void tree_run(K kernel, std::atomic<uint64_t>& done, const TreeParams& p,
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                               C::kLds);
   });
+  if (p.whose) hipLaunchKernelGGL((tree_plan_kernel<C::kRows, C::kStep>), dim3(1), dim3(kTreePlan), 0, s, p);
   hipLaunchKernelGGL(kernel, dim3((unsigned)L.grid), dim3(kTreeThreads), C::kLds, s, p);
 }
 
@@ -1385,6 +1452,7 @@ extern "C" int q6moe_kv_tree_attention(const q6moe_tree_attn_args* a, void* stre
   p.to_log2 = 1.4426950408889634f / sqrtf((float)a->head_dim);
   uint8_t* w = reinterpret_cast<uint8_t*>(a->workspace);
   p.info = reinterpret_cast<int32_t*>(w + L.info);
+  p.whose = a->batch > kTreeLanes ? reinterpret_cast<int32_t*>(w + L.whose) : nullptr;
   p.stat = reinterpret_cast<float*>(w + L.stat);
   p.part = reinterpret_cast<float*>(w + L.part);
   p.out = a->out;
