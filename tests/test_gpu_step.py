@@ -273,6 +273,11 @@ def test_attention(device, page, kvh, r, dim, lengths, counts, extra, kind, room
     (520, 4, 1, 128, 1, 30, 0),    # so many that none is split
     (70, 4, 9, 64, 12, 300, 5),    # many rows, in turns; max_count above any count
     (390, 8, 25, 64, 4, 20, 0),    # many rows, none split
+    (64, 2, 3, 128, 3, 700, 0),    # the most that a wave looks through by itself
+    (65, 2, 3, 128, 3, 700, 1),    # and more
+    (1030, 1, 2, 64, 2, 60, 0),    # more than one workgroup has threads
+    (2100, 2, 4, 256, 1, 15, 0),
+    (80, 1, 4, 128, 2, 9000, 0),   # split into many chunks
 ])
 def test_attention_of_many_sequences(device, batch, kvh, r, dim, count, most_len, spare_count):
     rng = np.random.default_rng(batch)
