@@ -71,7 +71,7 @@ struct TreeParams {
   float* part;     // [workgroup][row of the tile][D] partial sums
   float* stat;     // [workgroup][row of the tile][2]: maximum (log2) and sum
   int32_t* info;   // [batch + 2]: first item of each sequence; at [batch] the keys per item, then the items
-  int32_t* whose;  // of many sequences: each item's
+  int32_t* whose;  // [workgroup] each item's sequence, where tree_plan_kernel finds the items; else null
   uint16_t* out;
 };
 
@@ -91,7 +91,6 @@ struct TreeThin {
 };
 
 // Calls of many rows: 128 rows per workgroup, 32 per wave, which share the keys.
-// Bound by the vector ALU.
 template <int D>
 struct TreeWide {
   static constexpr int kRows = 128;
@@ -109,10 +108,9 @@ struct TreeWide {
   static_assert(kPerCu * kLds <= 160 * 1024, "tile");
 };
 
-template <int N>
-__device__ __forceinline__ void tree_wait_vm() {
-  static_assert(N >= 0 && N < 64, "vmcnt range");
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+// The wave's loads and DMA have landed.
+__device__ __forceinline__ void tree_landed() {
+  __builtin_amdgcn_s_waitcnt(15 << 8 | 7 << 4);  // vmcnt(0)
   asm volatile("" ::: "memory");
 }
 
@@ -825,7 +823,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   const int place = (int)(blockIdx.x >> 3) / (kTreeCus / 8);  // 32 CUs per XCD
   const auto advance = [&](int i) {
     if (C::kPerCu > 1) tree_priority<C::kPerCu>(place + i);
-    tree_wait_vm<0>();
+    tree_landed();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and reads of the scales
     put.put(p, keys, scales);
     issue(i + 1, stage ^ 1);
@@ -845,7 +843,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
     compute(std::true_type{}, tile_at(i), stage);
     stage ^= 1;
   }
-  tree_wait_vm<0>();
+  tree_landed();
 
   // Both half waves hold half of a row's keys in l and psum.
   float l = st.l + __shfl_xor(st.l, 32), m = st.m;
@@ -1144,7 +1142,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   const int place = (int)(blockIdx.x >> 3) / (kTreeCus / 8);  // 32 CUs per XCD
   const auto advance = [&](int i) {
     tree_priority<C::kPerCu>(place + i);
-    tree_wait_vm<0>();
+    tree_landed();
     put.put(p, keys, scales, p.to_log2, e + 10);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     convert();
@@ -1162,7 +1160,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
     advance(i);
     if (rows) compute(std::true_type{}, tile_at(i));
   }
-  tree_wait_vm<0>();
+  tree_landed();
   const float l = st.l + __shfl_xor(st.l, 32), up = 0x1p24f / st.factor;
 #pragma unroll
   for (int c = 0; c < KS; ++c)

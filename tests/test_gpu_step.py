@@ -136,7 +136,8 @@ def test_write_tokens(device, rows, pages, page, kvh, dim, group, values, scales
                          xv[:, 1 + i].reshape(rows, -1), slots, group, scales) for i in range(2)]
     p = _dev(pools, device)
     for stride in ("apart", "together"):
-        key, value = (x[:, 1 + i] if stride == "apart" else x[:, 1 + i].reshape(rows, -1).contiguous() for i in range(2))
+        key, value = (x[:, 1 + i] if stride == "apart" else x[:, 1 + i].reshape(rows, -1).contiguous()
+                      for i in range(2))
         got, gs = p.clone(), sc.clone()
         write_tokens(got[0], gs[0], got[1], gs[1], key, value, _dev(slots, device), kv_heads=kvh, head_dim=dim,
                      group=group)
