@@ -67,10 +67,12 @@ struct TreeParams {
   int slots;       // workgroups that the work is split for
   int whole;       // no split over keys
   int grid;        // workgroups of the launch
+  int parts;       // places for partial sums
   float to_log2;   // log2(e) / sqrt(D)
-  float* part;     // [workgroup][row of the tile][D] partial sums
-  float* stat;     // [workgroup][row of the tile][2]: maximum (log2) and sum
-  int32_t* info;   // [batch + 2]: first item of each sequence; at [batch] the keys per item, then the items
+  float* part;     // [item of a split sequence][row of the tile][D] partial sums
+  float* stat;     // [item of a split sequence][row of the tile][2]: maximum (log2) and sum
+  int32_t* info;   // [2 batch + 2]: first place of each sequence's sums; the keys per item; the items; and
+                   // with ``whose`` the first item of each sequence
   int32_t* whose;  // [workgroup] each item's sequence, where tree_plan_kernel finds the items; else null
   uint16_t* out;
 };
@@ -181,7 +183,7 @@ __device__ __forceinline__ void tree_priority(int turn) {
 }
 
 struct TreeItem {
-  int id, b, tile, kh, chunk, keys;
+  int place, b, tile, kh, chunk, keys;  // place: of its partial sums
   TreeSeq seq;
 };
 
@@ -282,10 +284,7 @@ __global__ void __launch_bounds__(kTreePlan) tree_plan_kernel(TreeParams p) {
     return v;
   };
   const int keys = tree_keys<ROWS, STEP>(p, sum);
-  int base = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += kTreePlan) {
-    const int b = b0 + (int)threadIdx.x;
-    const int n = b < p.batch ? tree_items<ROWS>(p, tree_seq(p, b), keys) : 0;
+  const auto before = [&](int n, int& base) {  // of the threads before; base grows by all
     const int upto = tree_wave_scan(n);
     __syncthreads();
     if (lane == 63) lds[wave] = upto;
@@ -295,14 +294,23 @@ __global__ void __launch_bounds__(kTreePlan) tree_plan_kernel(TreeParams p) {
       first += w < wave ? lds[w] : 0;
       base += lds[w];
     }
+    return first;
+  };
+  int items = 0, places = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += kTreePlan) {
+    const int b = b0 + (int)threadIdx.x;
+    const TreeSeq s = b < p.batch ? tree_seq(p, b) : TreeSeq{0, 0, 0, 0};
+    const int n = tree_items<ROWS>(p, s, keys);
+    const int first = before(n, items), place = before(s.n > keys ? n : 0, places);
     if (b < p.batch) {
-      p.info[b] = first;
+      p.info[b] = place;
+      p.info[p.batch + 2 + b] = first;
       for (int i = first < 0 ? 0 : first; i < first + n && i < p.grid; ++i) p.whose[i] = b;
     }
   }
   if (threadIdx.x == 0) {
     p.info[p.batch] = keys;
-    p.info[p.batch + 1] = base;
+    p.info[p.batch + 1] = items;
   }
 }
 
@@ -312,7 +320,7 @@ template <int ROWS, int STEP>
 __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
   const int lane = threadIdx.x & 63;
   TreeSeq mine{0, 0, 0, 0};
-  int upto = 0, n = 0, total;
+  int upto = 0, n = 0, total;  // items of the lane's sequence and up to it
   if (p.whose) {
     it.keys = p.info[p.batch];
     total = p.info[p.batch + 1];
@@ -334,13 +342,13 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
   const int place = (int)(blockIdx.x >> 3);
   const int id = (int)(blockIdx.x & 7) * run + place;
   if (place >= run || id >= total) return false;
-  it.id = id;
-  int first;
+  int first, sums;  // first item of the sequence, and place of its sums
   if (p.whose) {
     const int b = p.whose[id];
     it.b = b < 0 || b >= p.batch ? 0 : b;  // as for the items that no workgroup has
     it.seq = tree_seq(p, it.b);
-    first = p.info[it.b];
+    sums = p.info[it.b];
+    first = p.info[p.batch + 2 + it.b];
   } else {
     it.b = __builtin_ctzll(__ballot(id < upto));
     it.seq.start = __builtin_amdgcn_readlane(mine.start, it.b);
@@ -348,11 +356,14 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, TreeItem& it) {
     it.seq.len = __builtin_amdgcn_readlane(mine.len, it.b);
     it.seq.n = __builtin_amdgcn_readlane(mine.n, it.b);
     first = __builtin_amdgcn_readlane(upto - n, it.b);
-    if (threadIdx.x == 0 && id == first) p.info[it.b] = first;
+    const int split = mine.n > it.keys ? n : 0;
+    sums = __builtin_amdgcn_readlane(tree_wave_scan(split) - split, it.b);
+    if (threadIdx.x == 0 && id == first) p.info[it.b] = sums;
     if (threadIdx.x == 0 && id == 0) p.info[p.batch] = it.keys;
   }
   const int in = id - first, tiles = tree_tiles(p, it.seq, ROWS);
-  if (in < 0 || tiles < 1) return false;
+  it.place = sums + in;
+  if (in < 0 || tiles < 1 || (it.seq.n > it.keys && (it.place < 0 || it.place >= p.parts))) return false;
   const int row = in / tiles;
   it.tile = in - row * tiles;
   it.chunk = row / p.kvh;
@@ -890,7 +901,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
     for (int g = 0; g < 4; ++g)
       v += *reinterpret_cast<const f32x4*>(sum + (g * C::kRows + rr) * D + 4 * (c ^ (rr & (D / 4 - 1))));
     const float to = joint(rr, &all);
-    const int64_t place = (int64_t)it.id * C::kRows + rr;
+    const int64_t place = (int64_t)it.place * C::kRows + rr;
     if (split) {
       *reinterpret_cast<f32x4*>(p.part + place * D + 4 * c) = v;
       if (c == 0) *reinterpret_cast<f32x2*>(p.stat + 2 * place) = f32x2{to, all};
@@ -1169,7 +1180,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   const int at = which();
   if (at < seq.count * p.r)
     tree_result<D>(p, it, acc, chunks > 1, st.limit < 0.f ? kTreeFloor : st.m, l, at / p.r, at % p.r,
-                   (int64_t)it.id * C::kRows + wave * 32 + col, h);
+                   (int64_t)it.place * C::kRows + wave * 32 + col, h);
 }
 
 // The chunks' sums of a row and head joined in chunk order, D / 4 lanes of four
@@ -1213,8 +1224,8 @@ __global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p
   int chunks = tree_chunks(n, keys);
   const int64_t first = ((int64_t)from + (int64_t)kh * tiles + tile) * tile_rows + rr - tile * tile_rows;
   const int64_t step = (int64_t)p.kvh * tiles * tile_rows;
-  // starts that do not ascend can name more tiles than the workspace has places for
-  const bool live = head < p.hq && chunks > 1 && from >= 0 && first + (chunks - 1) * step < (int64_t)p.grid * tile_rows;
+  // starts that do not ascend can name more items than the workspace has places for
+  const bool live = head < p.hq && chunks > 1 && from >= 0 && first + (chunks - 1) * step < (int64_t)p.parts * tile_rows;
   const int run = (chunks + parts - 1) >> log_parts, end_run = (part + 1) * run;
   const int to_chunk = live ? (end_run < chunks ? end_run : chunks) : 0;
   float m = kTreeFloor, l = 0.f;
@@ -1283,6 +1294,7 @@ struct TreeLayout {
   int wide;
   int slots, whole;
   int64_t units;  // row tiles x KV heads, at most
+  int64_t parts;  // places for partial sums
   int64_t grid;   // at most so many workgroups have work
   size_t info, whose, stat, part, total;
 };
@@ -1324,15 +1336,22 @@ static TreeLayout tree_layout(int64_t batch, int64_t rows, int64_t max_count, in
   const int64_t tile = L.wide ? TreeWide<128>::kRows : thin, units = tiles(tile);
   L.slots = slots(L.wide);
   L.units = units;
-  L.whole = units >= 4 * L.slots;
-  L.grid = L.whole ? units : (2 * units <= L.slots ? L.slots : units + 2 * L.slots);
+  // Many short sequences fill the chip without a split, and a launch less; one long
+  // one among them (its capacity tells) has to be split all the same: 600 of 300
+  // tokens and one of 30 K, one token each, 286 us without and 87 with.
+  const int64_t step = L.wide ? (dim == 256 ? TreeWide<256>::kStep : TreeWide<128>::kStep) : TreeThin<128>::kStep;
+  L.whole = units >= 4 * L.slots && cap <= 32 * step;
+  const bool once = 2 * units <= L.slots;
+  L.grid = L.whole ? units : (once ? L.slots : units + 2 * L.slots);
   L.grid = cdiv(L.grid, 8) * 8;  // whole runs per XCD
-  const int64_t parts = L.whole ? 0 : L.grid * tile;
+  // In turns a chunk has more keys than a half of a place's share, and a split
+  // sequence less than twice its keys' share of chunks (64: of the sum's rounding).
+  L.parts = L.whole ? 0 : (once ? L.grid : 4 * L.slots + 64);
   L.info = 0;
-  L.whose = tree_align(L.info + (size_t)(batch + 2) * 4);
+  L.whose = tree_align(L.info + (size_t)(2 * batch + 2) * 4);
   L.stat = tree_align(L.whose + (batch > kTreeLanes ? (size_t)L.grid * 4 : 0));
-  L.part = tree_align(L.stat + (size_t)parts * 8);
-  L.total = tree_align(L.part + (size_t)parts * dim * 4);
+  L.part = tree_align(L.stat + (size_t)(L.parts * tile) * 8);
+  L.total = tree_align(L.part + (size_t)(L.parts * tile) * dim * 4);
   return L;
 }
 
@@ -1447,6 +1466,7 @@ extern "C" int q6moe_kv_tree_attention(const q6moe_tree_attn_args* a, void* stre
   p.slots = L.slots;
   p.whole = L.whole;
   p.grid = (int)L.grid;
+  p.parts = (int)L.parts;
   p.to_log2 = 1.4426950408889634f / sqrtf((float)a->head_dim);
   uint8_t* w = reinterpret_cast<uint8_t*>(a->workspace);
   p.info = reinterpret_cast<int32_t*>(w + L.info);

@@ -294,6 +294,27 @@ def test_attention_of_many_sequences(device, batch, kvh, r, dim, count, most_len
             _check(got[a:e], one, None)
 
 
+@pytest.mark.parametrize("batch,kvh,r,dim,count", [(600, 4, 1, 64, 1), (300, 8, 2, 128, 2), (60, 2, 3, 128, 2)])
+def test_attention_of_long_sequences_among_many(device, batch, kvh, r, dim, count):
+    # two long ones among short ones are split, whatever fills the chip; pages are shared
+    rng = np.random.default_rng(batch)
+    k, ks = _cache(rng, 64, 64, kvh, dim)
+    v, vs = _cache(rng, 64, 64, kvh, dim)
+    lengths = rng.integers(0, 60, batch)
+    lengths[[7, batch - 2]] = 20000, 9001
+    counts = rng.integers(0, count + 1, batch)
+    counts[[7, batch - 2]] = count
+    starts = np.concatenate([[0], np.cumsum(counts)])
+    table = rng.integers(0, 64, (batch, 320)).astype(np.int32)
+    q = bf16_round((rng.standard_normal((int(starts[-1]), kvh * r, dim)) * 2).astype(np.float32))
+    got = _attn(device, (k, ks, v, vs, table, lengths, starts, 64, kvh, q, count), None)
+    for b in [7, batch - 2, *rng.permutation(batch)[:10]]:
+        a, e = starts[b], starts[b + 1]
+        if e > a:
+            one = (k, ks, v, vs, table[b:b + 1], lengths[b:b + 1], np.array([0, e - a]), 64, kvh, q[a:e], count)
+            _check(got[a:e], one, None)
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("room", [False, True], ids=["small", "large"])
 def test_attention_chain_of_a_prompt(device, dim, room):
