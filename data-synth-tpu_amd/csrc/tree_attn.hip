@@ -1225,7 +1225,8 @@ __global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p
   const int64_t first = ((int64_t)from + (int64_t)kh * tiles + tile) * tile_rows + rr - tile * tile_rows;
   const int64_t step = (int64_t)p.kvh * tiles * tile_rows;
   // starts that do not ascend can name more items than the workspace has places for
-  const bool live = head < p.hq && chunks > 1 && from >= 0 && first + (chunks - 1) * step < (int64_t)p.parts * tile_rows;
+  const bool live =
+      head < p.hq && chunks > 1 && from >= 0 && first + (chunks - 1) * step < (int64_t)p.parts * tile_rows;
   const int run = (chunks + parts - 1) >> log_parts, end_run = (part + 1) * run;
   const int to_chunk = live ? (end_run < chunks ? end_run : chunks) : 0;
   float m = kTreeFloor, l = 0.f;

@@ -509,7 +509,8 @@ def test_keep_accepted(device, batch, page, pps, chans, groups, dtype, layers, m
     after = scales.view(torch.uint8).view(layers, 2, pages, page, -1).cpu().numpy()
     for n in range(layers):
         for i in range(2):
-            np.testing.assert_array_equal(got[n, i].cpu().numpy(), oracle.keep(codes[n, i], table, lengths, path, accepted, page))
+            np.testing.assert_array_equal(got[n, i].cpu().numpy(),
+                                          oracle.keep(codes[n, i], table, lengths, path, accepted, page))
             np.testing.assert_array_equal(after[n, i], oracle.keep(bits[n, i], table, lengths, path, accepted, page))
 
 
@@ -567,7 +568,8 @@ def test_refusals(device):
             (dict(page_size=2), "page_size"), (dict(v_pool=other[:2], v_scales=scales[:2]), "same size"),
             (dict(starts=two), "starts"), (dict(lengths=one), "lengths"), (dict(masks=masks[:1]), "masks must be"),
             (dict(masks=masks.int()), "masks must be"), (dict(masks=masks, max_count=65), "bit for each"),
-            (dict(out=q[:1]), "out must be"), (dict(workspace=torch.zeros(8, dtype=torch.uint8, device=device)), "workspace"),
+            (dict(out=q[:1]), "out must be"),
+            (dict(workspace=torch.zeros(8, dtype=torch.uint8, device=device)), "workspace"),
             (dict(k_scales=scales.half()), "k scales must be"),
     ):
         with pytest.raises(ValueError, match=text):
@@ -646,7 +648,8 @@ def test_whole_steps_together(device):
                 s["lengths"] += taken
             release_pages(s["table"], s["lengths"], s["free"], s["count"], page_size=page)
             held = -(-s["lengths"].cpu().numpy() // page)
-            assert ((s["table"].cpu().numpy() >= 0).sum(1) == held).all() and s["count"].item() == batch * pps - held.sum()
+            assert ((s["table"].cpu().numpy() >= 0).sum(1) == held).all()
+            assert s["count"].item() == batch * pps - held.sum()
         s["lengths"].zero_()
         release_pages(s["table"], s["lengths"], s["free"], s["count"], page_size=page)
     stream.synchronize()
