@@ -16,7 +16,7 @@
 // one for many, bound by the vector ALU that turns scores into probabilities beside
 // the matrix cores. 8 sequences of 8 K to 32 K tokens, 4 KV heads of 128 channels, 8
 // query heads each: one token each 47 us (the cache at 4.5 TB/s but for 10 us before
-// the first and after the last keys), trees of 16 70 us, of 64 199 us (634 TFLOP/s).
+// the first and after the last keys), trees of 16 69 us, of 64 200 us (630 TFLOP/s).
 //
 // Scores are exact sums of FP32-scaled products of the stored codes but for the FP32
 // rounding; the rounding to fewer bits that there is: a probability times its value
