@@ -315,6 +315,36 @@ def test_attention_of_long_sequences_among_many(device, batch, kvh, r, dim, coun
             _check(got[a:e], one, None)
 
 
+@pytest.mark.parametrize("batch", [9, 70])
+def test_attention_replayed_with_other_lengths(device, batch):
+    # the same graph over other lengths and counts: how the work is cut is found anew each time
+    rng = np.random.default_rng(batch)
+    k, ks, v, vs, table, lengths, starts, page, kvh, q, most = _case(
+        batch, [2500] * batch, [3] * batch, 64, 2, 4, 128)
+    pools = [_dev(k.reshape(*k.shape[:2], -1), device), _dev(ks, device), _dev(v.reshape(*v.shape[:2], -1), device),
+             _dev(vs, device)]
+    state = [_dev(np.asarray(t, np.int32), device) for t in (table, lengths, starts)]
+    x, out = _dev(q, device, torch.bfloat16), torch.empty(q.shape, dtype=torch.bfloat16, device=device)
+    work = torch.empty(1 << 28, dtype=torch.uint8, device=device)
+
+    def attend(to, workspace):
+        return paged_tree_attention(x, *pools, *state, page_size=page, kv_heads=kvh, max_count=most, out=to,
+                                    workspace=workspace)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend(out, work)
+    for turn in range(4):
+        state[1].copy_(_dev(rng.integers(0, (2500, 40, 2500, 700)[turn], batch).astype(np.int32), device))
+        counts = rng.integers(0, 4, batch)
+        state[2].copy_(_dev(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32), device))
+        out.fill_(5.0)
+        graph.replay()
+        want = attend(torch.full_like(out, 5.0), None)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("room", [False, True], ids=["small", "large"])
 def test_attention_chain_of_a_prompt(device, dim, room):
