@@ -30,8 +30,6 @@ import torch
 
 own = False
 
-PACKAGE = str(Path(__file__).resolve().parents[1] / "data-synth-tpu_amd")
-
 MOST_TREE = 256  # new tokens of a sequence that masks tell apart
 
 
@@ -392,8 +390,9 @@ def run(s):
 
 
 def _run_own(s):
-    if PACKAGE not in sys.path:
-        sys.path.insert(0, PACKAGE)
+    package = str(Path(__file__).resolve().parents[1] / "data-synth-tpu_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
     import q6moe
 
     if s["kind"] == "plan":
