@@ -63,6 +63,7 @@ struct PlanParams {
   const int32_t* parents;
   int64_t batch, pps, page, rows, max_count;  // max_count: most new tokens per sequence that are placed
   int words;
+  int most_lost;  // that a sequence adds to ``missing``: with all rows no more than 2^31 - 1 for all of them
   int32_t* starts;
   int64_t* slots;
   int32_t* positions;
@@ -87,6 +88,10 @@ __device__ __forceinline__ int64_t plan_count(const PlanParams& p, int64_t b) {
 __device__ __forceinline__ int64_t plan_fit(const PlanParams& p, int64_t count, int64_t before) {
   const int64_t left = p.rows - before;
   return left <= 0 ? 0 : (count < left ? count : left);
+}
+// What a sequence adds to ``missing`` for tokens past max_count and rows.
+__device__ __forceinline__ int plan_lost(const PlanParams& p, int64_t lost) {
+  return lost < p.most_lost ? (int)lost : p.most_lost;
 }
 // Page indexes [first, end) that the new tokens of sequence b lie in.
 __device__ __forceinline__ void plan_pages(const PlanParams& p, int64_t len, int64_t count, int64_t* first,
@@ -174,7 +179,7 @@ __global__ void __launch_bounds__(kStepThreads) plan_take_kernel(PlanParams p) {
     }
   }
   const int64_t lost = plan_asked(p, b) - count;
-  if (threadIdx.x == 0 && lost) atomicAdd(p.missing, (int32_t)(lost < (1 << 30) ? lost : 1 << 30));
+  if (threadIdx.x == 0 && lost) atomicAdd(p.missing, plan_lost(p, lost));
   if constexpr (!kRows) return;
   __syncthreads();  // the table entries above
   if (b == p.batch - 1)
@@ -332,8 +337,7 @@ __global__ void __launch_bounds__(kSmallThreads) plan_small_kernel(PlanParams p)
         ++rank;
       }
   if (t == 0) p.free_count[0] = have - (taken < have ? taken : have);
-  const int64_t over = asked - count;
-  int missing = t < batch ? (int)(over < (1 << 20) ? over : 1 << 20) : 0;
+  int missing = t < batch ? plan_lost(p, asked - count) : 0;
   __syncthreads();  // the entries and sums above
   const auto sequence = [&](int row) {  // the last one with s_start[b] <= row
     int b = 0, hi = batch - 1;
@@ -671,6 +675,7 @@ extern "C" int q6moe_kv_plan(const q6moe_kv_plan_args* a, void* stream) {
   p.rows = a->rows;
   p.max_count = a->max_count;
   p.words = a->parents ? (int)cdiv(a->max_count, 64) : 0;
+  p.most_lost = (int)((0x7fffffff - a->rows) / a->batch);
   p.starts = a->starts;
   p.slots = a->slots;
   p.positions = a->positions;

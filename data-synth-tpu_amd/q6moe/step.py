@@ -101,8 +101,9 @@ def plan_pages(page_table, lengths, counts, free_pages, free_count, *, page_size
     depth: what rotary embeddings take; 0 for padding), ``masks`` (with parents:
     int64 [rows, ceil(max_count / 64)], bit jj of a row's words set where new
     token jj is an ancestor or the token itself) and ``missing`` (how many new
-    tokens got no slot: check it before the step's results are used). ``out``: a
-    plan whose buffers are written again.
+    tokens got no slot, of those past ``max_count`` and ``rows`` at most (2**31 -
+    1 - rows) // batch per sequence: check it before the step's results are used).
+    ``out``: a plan whose buffers are written again.
     """
     device, lens = _state(page_table, lengths, free_pages, free_count)
     _positive(page_size=page_size, rows=rows)

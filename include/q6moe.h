@@ -386,7 +386,8 @@ int q6moe_kv_decode_attention(const q6moe_attn_args* args, void* stream);
  * of word jj / 64 is set where new token jj is an ancestor of the row's token or itself.
  * parents[row] is the index (within the sequence) of the new token that the row's token
  * follows; -1, and anything that is no earlier token, means the last cached one.
- * *missing counts the asked-for tokens that got no slot.
+ * *missing counts the asked-for tokens that got no slot (of those past max_count and rows at
+ * most (2^31 - 1 - rows) / batch per sequence, so that it never wraps).
  */
 typedef struct q6moe_kv_plan_args {
   int32_t* page_table;       /* [batch, pages_per_seq], updated in place */

@@ -1,0 +1,31 @@
+"""GPU tests of the step operators at the ends of their ranges."""
+
+import numpy as np
+import pytest
+
+from q6moe import plan_pages
+
+from .test_gpu_step import _dev
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("batch,rows,paths", [(4, 100, "one workgroup"), (4, 6000, "two"), (2, 9000, "three"),
+                                              (1025, 50, "two, many")])
+@pytest.mark.parametrize("most", [2**30, 2**31 - 1])
+def test_missing_of_huge_counts(device, batch, rows, paths, most):
+    # every sequence asks for more than fits: what is missing is never read as none, whichever launches run
+    pps, page = 3, 64
+    counts = np.full(batch, most, np.int32)
+    table = _dev(np.arange(batch * pps, dtype=np.int32).reshape(batch, pps), device)
+    kw = {} if paths == "three" else dict(max_count=4000)
+    plan = plan_pages(table, _dev(np.zeros(batch, np.int32), device), _dev(counts, device),
+                      _dev(np.array([5], np.int32), device), _dev(np.array([0], np.int32), device), page_size=page,
+                      rows=rows, **kw)
+    fits, placed, lost = rows, 0, 0
+    for b in range(batch):
+        got = min(kw.get("max_count", rows), fits)
+        fits -= got
+        placed += min(got, pps * page)
+        lost += min(most - got, (2**31 - 1 - rows) // batch)
+    assert plan.missing.item() == lost + (rows - fits - placed) > 2**30
