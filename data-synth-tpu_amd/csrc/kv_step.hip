@@ -675,7 +675,8 @@ extern "C" int q6moe_kv_plan(const q6moe_kv_plan_args* a, void* stream) {
   p.rows = a->rows;
   p.max_count = a->max_count;
   p.words = a->parents ? (int)cdiv(a->max_count, 64) : 0;
-  p.most_lost = (int)((0x7fffffff - a->rows) / a->batch);
+  const int64_t lost = (0x7fffffff - a->rows) / a->batch;
+  p.most_lost = lost > 1 ? (int)lost : 1;
   p.starts = a->starts;
   p.slots = a->slots;
   p.positions = a->positions;
