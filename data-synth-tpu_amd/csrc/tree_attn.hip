@@ -1294,6 +1294,13 @@ __global__ void __launch_bounds__(kTreeThreads) tree_combine_kernel(TreeParams p
 }
 
 
+// The sizes that 32-bit indexes of tiles and tokens hold.
+static bool tree_holds(int64_t rows, int64_t hq, int64_t kvh, int64_t batch, int64_t max_count) {
+  return rows >= 1 && rows < (1 << 24) && max_count >= 1 && max_count < (1 << 24) && batch >= 1 && batch <= 65535 &&
+         kvh >= 1 && kvh <= kTreeMaxHeads && hq >= 1 && hq <= kTreeMaxHeads && hq % kvh == 0 &&
+         rows * (hq / kvh) < (1 << 30);
+}
+
 struct TreeLayout {
   int wide;
   int slots, whole;
@@ -1402,11 +1409,8 @@ using namespace q6moe;
 extern "C" size_t q6moe_tree_attn_workspace_size(int64_t batch, int64_t rows, int64_t max_count, int64_t query_heads,
                                                  int64_t kv_heads, int64_t head_dim, int64_t pages_per_seq,
                                                  int64_t page_size) {
-  if (batch < 1 || rows < 1 || max_count < 1 || query_heads < 1 || kv_heads < 1 || pages_per_seq < 1 || page_size < 1)
-    return 0;
-  if (query_heads % kv_heads || query_heads > kTreeMaxHeads || batch > 65535 || rows >= (1 << 24) ||
-      max_count >= (1 << 24) || pages_per_seq >= (1 << 30) || page_size >= (1 << 30) ||
-      pages_per_seq * page_size > (1 << 30))
+  if (!tree_holds(rows, query_heads, kv_heads, batch, max_count) || pages_per_seq < 1 || page_size < 1 ||
+      pages_per_seq >= (1 << 30) || page_size >= (1 << 30) || pages_per_seq * page_size > (1 << 30))
     return 0;
   return tree_layout(batch, rows, max_count, query_heads, kv_heads, head_dim,
                      pages_per_seq * page_size).total;
@@ -1415,7 +1419,7 @@ extern "C" size_t q6moe_tree_attn_workspace_size(int64_t batch, int64_t rows, in
 extern "C" int q6moe_kv_tree_attention(const q6moe_tree_attn_args* a, void* stream) {
   Q6MOE_REQUIRE(a, "tree_attention: null args");
   Q6MOE_REQUIRE(a->q && a->k_codes && a->v_codes && a->k_scales && a->v_scales && a->page_table && a->lengths &&
-                    a->starts && a->out && a->workspace,
+                    a->starts && a->out,
                 "tree_attention: null pointer");
   Q6MOE_REQUIRE(a->head_dim == 64 || a->head_dim == 128 || a->head_dim == 256,
                 "tree_attention: head_dim must be 64, 128 or 256");
@@ -1424,6 +1428,8 @@ extern "C" int q6moe_kv_tree_attention(const q6moe_tree_attn_args* a, void* stre
                 "tree_attention: query_heads must be a multiple of kv_heads, batch and heads at most 65535");
   Q6MOE_REQUIRE(a->rows >= 1 && a->rows < (1 << 24) && a->max_count >= 1 && a->max_count < (1 << 24),
                 "tree_attention: rows and max_count must be positive and below 2^24");
+  Q6MOE_REQUIRE(tree_holds(a->rows, a->query_heads, a->kv_heads, a->batch, a->max_count),
+                "tree_attention: rows x query heads per KV head must be below 2^30");
   Q6MOE_REQUIRE(a->page_size >= 1 && a->pages_per_seq >= 1 && a->pool_pages >= 1 && a->page_size < (1 << 30) &&
                     a->pages_per_seq < (1 << 30) && a->pool_pages < (1ll << 31) &&
                     a->pages_per_seq * a->page_size <= (1 << 30) && a->pool_pages * a->page_size < (1ll << 31),
@@ -1433,6 +1439,7 @@ extern "C" int q6moe_kv_tree_attention(const q6moe_tree_attn_args* a, void* stre
   Q6MOE_REQUIRE(!a->masks || (a->mask_words >= 1 && a->mask_words <= 4 && a->max_count <= 64 * a->mask_words),
                 "tree_attention: masks hold max_count bits in at most 4 words");
   Q6MOE_REQUIRE(a->q_stride >= 0 && a->q_stride % 8 == 0, "tree_attention: q_stride must be a multiple of 8");
+  Q6MOE_REQUIRE(a->workspace, "tree_attention: null pointer (workspace)");
   Q6MOE_REQUIRE(aligned(a->q, 16) && aligned(a->k_codes, 16) && aligned(a->v_codes, 16) && aligned(a->out, 16) &&
                     aligned(a->workspace, 256),
                 "tree_attention: q, codes and out need 16-byte and workspace 256-byte alignment");

@@ -452,8 +452,8 @@ int q6moe_kv_write_rows(const q6moe_kv_write_rows_args* args, void* stream);
  * sees nothing gives 0; unmapped pages read as zero codes with zero scales. Rows behind the
  * last sequence, and of a sequence those from max_count on, are left as they were in out.
  * head_dim 64, 128 or 256; one scale per token and KV head; pool_pages * page_size below 2^31,
- * pages_per_seq * page_size at most 2^30, rows and max_count below 2^24. Which kernel runs follows
- * from the sizes alone, never from lengths.
+ * pages_per_seq * page_size at most 2^30, rows and max_count below 2^24, rows * query_heads / kv_heads
+ * below 2^30. Which kernel runs follows from the sizes alone, never from lengths.
  */
 typedef struct q6moe_tree_attn_args {
   const uint16_t* q;         /* BF16 [rows, Hq, D], row r at q + r * q_stride */

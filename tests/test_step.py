@@ -87,6 +87,22 @@ def test_attention_refusals(over, text):
 
 
 @pytest.mark.parametrize("over,text", [
+    (dict(rows=1 << 24), "2^24"), (dict(pages_per_seq=1 << 20, page_size=1 << 20), "2^30"),
+    (dict(batch=65536), "65535"), (dict(query_heads=65536), "65535"), (dict(mask_words=5), "4 words"),
+    (dict(rows=(1 << 24) - 1, query_heads=65), "below 2^30"), (dict(), "null pointer (workspace)"),
+])
+def test_attention_names_the_limit_before_the_workspace(over, text):
+    # a caller beyond a limit has a workspace of 0 bytes, whose pointer may be null
+    sizes = {**dict.fromkeys(("batch", "rows", "max_count", "query_heads", "kv_heads", "pages_per_seq", "page_size"), 1),
+             **over, "head_dim": 128}
+    if text != "null pointer (workspace)" and "mask_words" not in over:
+        assert _lib.load().q6moe_tree_attn_workspace_size(*(sizes[n] for n in (
+            "batch", "rows", "max_count", "query_heads", "kv_heads", "head_dim", "pages_per_seq", "page_size"))) == 0
+    a = _filled(_lib.TreeAttnArgs, **{**dict(head_dim=128, q_stride=128, workspace=None, workspace_bytes=0), **over})
+    _refused(_lib.load().q6moe_kv_tree_attention, a, text)
+
+
+@pytest.mark.parametrize("over,text", [
     (dict(path=None), "null pointer"), (dict(count=0), "positive"), (dict(code_bytes=0), "row sizes"),
     (dict(path_len=257), "1 to 256"), (dict(path_len=0), "1 to 256"), (dict(pool_pages=0), "positive"),
     (dict(pools=(ctypes.c_void_p * 2)(FAKE, None)), "null pool"),
