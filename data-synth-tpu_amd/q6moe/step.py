@@ -197,7 +197,8 @@ def write_tokens(k_pool, k_scales, v_pool, v_scales, key, value, slots, *, kv_he
     ``slots`` int64 [rows] as ``plan_pages`` gives them; rows outside the pool (-1)
     are skipped, the others must be distinct. Pools int8 [pages, page_size, ...],
     scales [pages, page_size, kv_heads * head_dim / group] (group: head_dim by
-    default). Codes and scales are those of ``write_paged`` bit for bit.
+    default); K's and V's must not overlap. Codes and scales are those of
+    ``write_paged`` bit for bit.
     """
     _positive(kv_heads=kv_heads, head_dim=head_dim)
     group = head_dim if group is None else group
@@ -214,8 +215,9 @@ def write_tokens(k_pool, k_scales, v_pool, v_scales, key, value, slots, *, kv_he
     n = _pool_rows(k_pool, k_scales, chans, chans // group, device, "k")
     if _pool_rows(v_pool, v_scales, chans, chans // group, device, "v") != n or k_scales.dtype != v_scales.dtype:
         raise ValueError("the k and v pools must have the same size and scale type")
-    if k_pool.data_ptr() == v_pool.data_ptr() or k_scales.data_ptr() == v_scales.data_ptr():
-        raise ValueError("the k and v pools must not be the same memory")
+    if (abs(k_pool.data_ptr() - v_pool.data_ptr()) < n * chans
+            or abs(k_scales.data_ptr() - v_scales.data_ptr()) < n * (chans // group) * k_scales.element_size()):
+        raise ValueError("the k and v pools must not be the same memory, nor overlap")
     key, key_stride = _rows_of(key, rows, kv_heads, head_dim, device, "key")
     value, value_stride = _rows_of(value, rows, kv_heads, head_dim, device, "value")
     if key.dtype != value.dtype:

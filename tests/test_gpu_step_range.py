@@ -2,8 +2,9 @@
 
 import numpy as np
 import pytest
+import torch
 
-from q6moe import plan_pages
+from q6moe import plan_pages, write_tokens
 
 from .test_gpu_step import _dev
 
@@ -29,3 +30,16 @@ def test_missing_of_huge_counts(device, batch, rows, paths, most):
         placed += min(got, pps * page)
         lost += min(most - got, (2**31 - 1 - rows) // batch)
     assert plan.missing.item() == lost + (rows - fits - placed) > 2**30
+
+
+def test_write_refuses_pools_that_overlap(device):
+    both = torch.zeros(5, 4, 64, dtype=torch.int8, device=device)
+    scales, apart = torch.ones(5, 4, 1, device=device), torch.ones(3, 4, 1, device=device)
+    x, slots = torch.zeros(2, 64, device=device), torch.zeros(2, dtype=torch.int64, device=device)
+    other = torch.zeros(3, 4, 64, dtype=torch.int8, device=device)
+    kw = dict(kv_heads=1, head_dim=64)
+    for k, ks, v, vs in ((both[:3], scales[:3], both[2:], apart), (both[2:], scales[:3], both[:3], apart),
+                         (both[:3], scales[:3], other, scales[2:]), (both[:3], scales[2:], other, scales[:3])):
+        with pytest.raises(ValueError, match="same memory"):
+            write_tokens(k, ks, v, vs, x, x, slots, **kw)
+    write_tokens(both[:2], scales[:2], both[2:4], scales[2:4], x, x, slots, **kw)  # side by side
