@@ -253,8 +253,9 @@ def paged_tree_attention(q, k_pool, k_scales, v_pool, v_scales, page_table, leng
 
     Returns BF16 [rows, Hq, D]: softmax(q . k / sqrt(D)) . v with k and v the
     unrounded code * scale, rounded once. A row that sees nothing gives 0. Rows
-    behind the last sequence are left as they were in ``out``. Unmapped pages
-    read as zero keys and values.
+    behind the last sequence, and of a sequence those from ``max_count`` on, are
+    left as they were in ``out``; without ``out`` they are 0 (one launch more, for
+    the fill). Unmapped pages read as zero keys and values.
     """
     device = _gpu("q", q)
     if q.dtype is not torch.bfloat16 or q.ndim != 3 or q.shape[2] not in (64, 128, 256):
@@ -285,7 +286,7 @@ def paged_tree_attention(q, k_pool, k_scales, v_pool, v_scales, page_table, leng
     if q.stride(2) != 1 or q.stride(1) != dim or q.stride(0) % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
-        out = torch.empty((rows, hq, dim), dtype=torch.bfloat16, device=device)
+        out = torch.zeros((rows, hq, dim), dtype=torch.bfloat16, device=device)
     else:
         _on(device, "out", out, torch.bfloat16, (rows, hq, dim))
     if rows == 0:

@@ -6,7 +6,7 @@ import torch
 
 from q6moe import plan_pages, write_tokens
 
-from .test_gpu_step import _dev
+from .test_gpu_step import _attn, _case, _dev
 
 pytestmark = pytest.mark.gpu
 
@@ -30,6 +30,24 @@ def test_missing_of_huge_counts(device, batch, rows, paths, most):
         placed += min(got, pps * page)
         lost += min(most - got, (2**31 - 1 - rows) // batch)
     assert plan.missing.item() == lost + (rows - fits - placed) > 2**30
+
+
+@pytest.mark.parametrize("r,most", [(4, 6), (20, 6), (4, 3)])
+def test_attention_without_out_gives_zeros_where_nothing_is_computed(device, r, most):
+    # rows behind the last sequence, and those from max_count on, whatever the memory held
+    case = (*_case(38, [50, 3], [6, 5], 16, 2, r, 128, extra=9)[:10], most)
+    rows = case[9].shape
+    for _ in range(3):
+        dirty = torch.full(rows, float("nan"), dtype=torch.bfloat16, device=device)
+        torch.cuda.synchronize()
+        del dirty
+        got = _attn(device, case, None)
+        want = _attn(device, case, None, fill=7.0)
+        idle = np.ones(len(got), bool)
+        for first, end in ((0, 6), (6, 11)):
+            idle[first:min(end, first + most)] = False
+        assert (got[idle] == 0).all() and (want[idle] == 7.0).all()
+        np.testing.assert_array_equal(got[~idle], want[~idle])
 
 
 def test_write_refuses_pools_that_overlap(device):
