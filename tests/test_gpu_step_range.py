@@ -1,14 +1,26 @@
-"""GPU tests of the step operators at the ends of their ranges."""
+"""GPU tests of the step operators at the ends of their ranges: counts, scales and queries far
+apart, long contexts, every sequence of many.
+
+An output row (all heads of a token) is held to 2.5e-3 of its norm. With x its values and steps of 2^-7
+2^floor(log2 |x|), rounding to BF16 alone gives sqrt(sum step^2 / 12 / sum x^2), 1.6e-3 where the x are spread over
+their binades (at most 2^-7 / sqrt 12 = 2.3e-3, at 1, 2, 4, ...). Beside it a probability times its value scale is
+rounded to 11 bits: 2^-11 at most, 1.7e-4 where many keys count. Scores are off by some 2^-16 of their size.
+Rows have at least 128 values, so that the norm of the rounding errors stays within 30 % of its mean.
+"""
 
 import numpy as np
 import pytest
 import torch
 
+from oracle import step as oracle
+from oracle.packed_q6 import bf16_round
 from q6moe import plan_pages, write_tokens
 
-from .test_gpu_step import _attn, _case, _dev
+from .test_gpu_step import _attn, _cache, _case, _dev, _sees
 
 pytestmark = pytest.mark.gpu
+
+NORM = 2.5e-3
 
 
 @pytest.mark.parametrize("batch,rows,paths", [(4, 100, "one workgroup"), (4, 6000, "two"), (2, 9000, "three"),
@@ -61,3 +73,111 @@ def test_write_refuses_pools_that_overlap(device):
         with pytest.raises(ValueError, match="same memory"):
             write_tokens(k, ks, v, vs, x, x, slots, **kw)
     write_tokens(both[:2], scales[:2], both[2:4], scales[2:4], x, x, slots, **kw)  # side by side
+
+
+# ---------------------------------------------------------------------------
+# Attention
+# ---------------------------------------------------------------------------
+def _hold(got, want, rows=None):
+    """Every row that is not NaN in ``want`` (of ``rows``) is within NORM of its norm."""
+    live = ~np.isnan(want).any((1, 2))
+    if rows is not None:
+        live &= np.isin(np.arange(len(want)), rows)
+    assert live.any() and want[live][0].size >= 128
+    error = np.linalg.norm((got - want)[live].reshape(live.sum(), -1), axis=1)
+    size = np.linalg.norm(want[live].reshape(live.sum(), -1), axis=1)
+    ratio = error / np.maximum(size, 1e-300)
+    over = np.nonzero(live)[0][~(ratio <= NORM)].tolist()
+    assert not over, (over, ratio.max())
+
+
+def _exact(case, sees):
+    k, ks, v, vs, table, lengths, starts, page, kvh, q, most = case
+    return oracle.attention(q, k, ks, v, vs, table, lengths, starts, sees, page, most)[0]
+
+
+@pytest.mark.parametrize("lengths,counts,page,kvh,r,dim,kind,room", [
+    ([65533, 40000], [3, 2], 64, 1, 2, 64, "chain", False),           # a long context in few rows
+    ([65500], [30], 256, 1, 4, 64, "tree", False),                    # several tiles of it
+    ([65500], [30], 256, 1, 4, 64, "tree", True),                     # tiles of 128 rows
+    ([30000, 7, 12345, 0, 511], [16, 16, 3, 16, 1], 16, 2, 8, 128, "tree", False),
+    ([9000, 20000, 64], [40, 0, 60], 64, 1, 8, 128, "chain", True),
+    ([5000, 3001], [50, 20], 128, 1, 6, 256, "tree", True),
+    ([5000, 3001], [50, 20], 128, 1, 6, 256, "chain", False),
+    ([30000] + [50] * 70, [2] * 71, 64, 1, 4, 64, "chain", False),    # items found in a launch of their own
+    ([15000] * 8, [13] * 8, 256, 2, 8, 64, "tree", True),
+])
+def test_attention_counts_every_key_once(device, lengths, counts, page, kvh, r, dim, kind, room):
+    """All keys are equal, so every seen one has the same weight, and the value of token t is 1 in channel t / 16 % D
+    alone: an output is the number of a channel's seen tokens over that of all. Codes and scales (powers of two) are
+    exact, and so are sums over the values, whole numbers below 2^24. A weight is 2 to the power of a score of at most
+    2^4 less itself, off by half a step of it, 2^-21: with the exponential's step, and 11 bits that round it to 1
+    for the values, a quotient is off by less than 2^-16 before it is rounded to BF16. A run of 16 keys that is lost or
+    counted twice changes a channel by 16 D / n, at least 1.5 %."""
+    rng = np.random.default_rng(len(lengths) + page)
+    k, ks, v, vs, table, _, starts, page, kvh, q, most = _case(5, lengths, counts, page, kvh, r, dim, qscale=0.5, room=room)
+    k[:] = rng.integers(-127, 128, (1, 1, kvh, dim))
+    ks[:], vs[:], v[:] = 2.0**-7, 2.0**-6, 0
+    for b, (n, c) in enumerate(zip(lengths, counts)):
+        t = np.arange(n + c)
+        v[table[b, t // page], t % page, :, t // 16 % dim] = 64
+    sees = None if kind == "chain" else _sees(rng, counts, 0)
+    got = _attn(device, (k, ks, v, vs, table, lengths, starts, page, kvh, q, most), sees)
+    for b, (n, c) in enumerate(zip(lengths, counts)):
+        whole = np.bincount(np.arange(n) // 16 % dim, minlength=dim)
+        for j in range(c):
+            new = n + np.array(sorted(range(j + 1) if sees is None else sees[starts[b] + j]))
+            count = whole + np.bincount(new // 16 % dim, minlength=dim)
+            want = count / count.sum()
+            assert (np.abs(got[starts[b] + j] - want) <= want * (2.0**-8 + 2.0**-16)).all(), (b, j)
+
+
+def test_attention_long_contexts_by_the_norm(device):
+    # what an elementwise bound that grows with the number of keys cannot see
+    rng = np.random.default_rng(18)
+    k, ks = _cache(rng, 64, 64, 1, 64)
+    v, vs = _cache(rng, 64, 64, 1, 64)
+    table = rng.integers(0, 64, (2, 1024)).astype(np.int32)
+    q = bf16_round(rng.standard_normal((5, 4, 64)).astype(np.float32) * 2)
+    case = (k, ks, v, vs, table, [65533, 40000], np.array([0, 3, 5]), 64, 1, q, 3)
+    _hold(_attn(device, case, None), _exact(case, None))
+
+
+def _chain_exact(device, case):
+    """The oracle's chain in 64 bits on the GPU, all sequences at once."""
+    k, ks, v, vs, table, lengths, starts, page, kvh, q, most = case
+    batch, cap, (rows, hq, dim) = table.shape[0], table.shape[1] * page, q.shape
+    n, first = (_dev(np.asarray(t, np.int64), device) for t in (lengths, starts))
+    t = torch.arange(cap, device=device)
+    slot = _dev(table.astype(np.int64), device)[:, t // page] * page + t % page
+    x = _dev(q, device, torch.float64)
+    row = first[:-1, None] + torch.arange(most, device=device)
+    live = row < first[1:, None]
+    sees = t <= n[:, None, None] + torch.arange(most, device=device)[:, None]  # [batch, most, cap]
+    out = torch.full((rows, hq, dim), float("nan"), dtype=torch.float64, device=device)
+    for h in range(kvh):
+        kk, vv = (_dev(c[:, :, h].reshape(-1, dim), device)[slot].double()
+                  * _dev(s[:, :, h].reshape(-1), device)[slot].double()[..., None] for c, s in ((k, ks), (v, vs)))
+        kk = kk.transpose(1, 2).contiguous()
+        for g in range(h * hq // kvh, (h + 1) * hq // kvh):
+            s = torch.matmul(x[:, g][row.clamp(max=rows - 1)], kk) / dim**0.5
+            p = torch.softmax(s.masked_fill(~sees, -float("inf")), -1)
+            out[row[live], g] = torch.matmul(p, vv)[live]
+    return out.cpu().numpy()
+
+
+@pytest.mark.parametrize("batch,kvh,r,dim,count,most_len,spare_count", [
+    (300, 2, 2, 64, 1, 400, 0), (520, 4, 1, 128, 1, 30, 0), (70, 4, 9, 64, 12, 300, 5), (390, 8, 25, 64, 4, 20, 0),
+    (64, 2, 3, 128, 3, 700, 0), (65, 2, 3, 128, 3, 700, 1), (1023, 2, 2, 64, 2, 60, 0), (1024, 2, 2, 64, 1, 60, 0),
+    (1025, 2, 2, 64, 2, 60, 0), (2100, 2, 4, 256, 1, 15, 0), (80, 1, 4, 128, 2, 9000, 0), (3, 2, 4, 128, 700, 500, 0),
+])
+def test_attention_of_every_sequence_of_many(device, batch, kvh, r, dim, count, most_len, spare_count):
+    rng = np.random.default_rng(batch)
+    lengths = rng.integers(0, most_len + 1, batch)
+    counts = rng.integers(0, count + 1, batch)
+    counts[[0, -1]] = count
+    k, ks, v, vs, table, _, starts, page, kvh, q, _ = _case(batch, lengths, counts, 16, kvh, r, dim, 2)
+    case = (k, ks, v, vs, table, lengths, starts, page, kvh, q, count + spare_count)
+    got = _attn(device, case, None, fill=9.0)
+    assert (got[starts[-1]:] == 9.0).all()
+    _hold(got, _chain_exact(device, case))
