@@ -490,7 +490,7 @@ struct TreeScales {
     if (__any(a > limit)) {
       const float x = tree_wave_reduce(a, [](float c, float d) { return fmaxf(c, d); });
       int ve = (int)(__builtin_bit_cast(uint32_t, x) >> 23) - 127;
-      ve = ve < -110 ? -110 : ve;
+      ve = ve < -124 ? -124 : ve;
       factor = __builtin_bit_cast(float, (uint32_t)(127 + 3 - ve) << 23);  // 2^(3-ve): at most 2^4 now
       limit = __builtin_bit_cast(float, (uint32_t)(127 + ve + 3 > 254 ? 254 : 127 + ve + 3) << 23);
     }
@@ -882,12 +882,13 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
     return to;
   };
   float all;
-  const float up = __builtin_amdgcn_exp2f(m - joint(col, &all)) * (0x1p24f / st.factor);
+  // 2^24 / factor leaves the range of FP32 where the sums do not: two steps
+  const float up = __builtin_amdgcn_exp2f(m - joint(col, &all)) * (1.f / st.factor);
   const float shift = 128.f * psum * 0x1p-24f;
   if (row.live)
     tree_runs<D>(acc, h, [&](int c, f32x4 v) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = (v[u] - shift) * up;
+      for (int u = 0; u < 4; ++u) v[u] = (v[u] - shift) * 0x1p24f * up;
       return *reinterpret_cast<f32x4*>(sum + (wave * C::kRows + col) * D + 4 * ((c / 4) ^ (col & (D / 4 - 1)))) = v;
     });
   __syncthreads();
@@ -1172,11 +1173,11 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
     if (rows) compute(std::true_type{}, tile_at(i));
   }
   tree_landed();
-  const float l = st.l + __shfl_xor(st.l, 32), up = 0x1p24f / st.factor;
+  const float l = st.l + __shfl_xor(st.l, 32), up = 1.f / st.factor;
 #pragma unroll
   for (int c = 0; c < KS; ++c)
 #pragma unroll
-    for (int v = 0; v < 16; ++v) acc[c][v] *= up;
+    for (int v = 0; v < 16; ++v) acc[c][v] = acc[c][v] * 0x1p24f * up;  // two steps: 2^24 / factor may overflow
   const int at = which();
   if (at < seq.count * p.r)
     tree_result<D>(p, it, acc, chunks > 1, st.limit < 0.f ? kTreeFloor : st.m, l, at / p.r, at % p.r,

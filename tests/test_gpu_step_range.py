@@ -16,7 +16,7 @@ from oracle import step as oracle
 from oracle.packed_q6 import bf16_round
 from q6moe import plan_pages, write_tokens
 
-from .test_gpu_step import _attn, _cache, _case, _dev, _sees
+from .test_gpu_step import FEW_AND_MANY, _attn, _cache, _case, _dev, _sees
 
 pytestmark = pytest.mark.gpu
 
@@ -181,3 +181,16 @@ def test_attention_of_every_sequence_of_many(device, batch, kvh, r, dim, count, 
     got = _attn(device, case, None, fill=9.0)
     assert (got[starts[-1]:] == 9.0).all()
     _hold(got, _chain_exact(device, case))
+
+
+DIMS = pytest.mark.parametrize("dim", [64, 128, 256])
+
+
+@DIMS
+@FEW_AND_MANY
+@pytest.mark.parametrize("power", [104, 108, 112, -112])
+def test_attention_values_near_the_ends_of_fp32(device, dim, r, room, power):
+    # value scales of 2^power and 2^-7 of that; sums over 100 keys stay below 2^128
+    case = _case(36, [90, 3], [8, 5], 16, 1, r, dim, qscale=0.5, room=room)
+    case[3][:] = (case[3] * np.float32(2.0**power) if power < 0 else np.float32(2.0**power) * (case[3] / case[3].max()))
+    _hold(_attn(device, case, None), _exact(case, None))
