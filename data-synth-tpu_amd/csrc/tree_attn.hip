@@ -21,9 +21,9 @@
 // Scores are exact sums of FP32-scaled products of the stored codes but for the FP32
 // rounding; the rounding to fewer bits that there is: a probability times its value
 // scale to the 11 bits of FP16, the second product's operand (an eighth of the BF16
-// output's half step), and query values that are more than 2^6 below their row's
-// largest (few rows) or 2^28 below that of 32 rows (many). Maxima, sums and all
-// accumulators are FP32.
+// output's half step; for products far below the row's largest see TreeScales), and
+// query values that are more than 2^6 below their row's largest (few rows) or 2^28
+// below that of 32 rows (many). Maxima, sums and all accumulators are FP32.
 #include <atomic>
 #include <type_traits>
 
@@ -88,7 +88,7 @@ struct TreeThin {
   static constexpr int kHalf = kTile * D;         // bytes of a tile's keys, and of its values
   static constexpr int kScale = 2 * 32 * 4 + 16;  // per wave: a tile's key and value scales, value factor
   static constexpr int kRing = 4 * 2 * 2 * kHalf;  // per wave a tile in work and one on its way
-  static constexpr int kLds = kRing + 4 * kScale + 32;  // and four words of masks
+  static constexpr int kLds = kRing + 4 * kScale + 32 + 16;  // and four words of masks, four flags
   static_assert(kPerCu * kLds <= 160 * 1024, "tile");
 };
 
@@ -121,6 +121,26 @@ __device__ __forceinline__ void tree_landed() {
 __device__ __forceinline__ uint32_t tree_opaque(uint32_t v) {
   asm volatile("" : "+v"(v));
   return v;
+}
+
+// The kernel's arguments read again, and with them all that a chunk begun anew needs: what
+// it uses is not held in registers through the pass before.
+__device__ __forceinline__ TreeParams tree_again() {
+  auto args = (__attribute__((address_space(4))) const uint64_t*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  uint64_t word[sizeof(TreeParams) / 8];
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof word / 8); ++i) word[i] = args[i];
+  return __builtin_bit_cast(TreeParams, word);
+}
+
+// Whether a pass was left. The compiler is not to know it where it ends: it put the pass
+// after it in between, with the sums of the first in scratch memory (one token over
+// 16 K, 256-wide heads, 28.8 us became 33.5).
+__device__ __forceinline__ bool tree_left(bool whole) {
+  int v = __builtin_amdgcn_readfirstlane(whole);
+  asm volatile("" : "+s"(v));
+  return !v;
 }
 
 // What the rows of a sequence need: cached tokens, new tokens with rows, keys in reach.
@@ -439,7 +459,7 @@ struct TreeLookup {
   bool pick;
   int entry;        // page-table entry of the next tile's key
   uint32_t rk, rv;  // scales on their way, as they lie in the cache
-  bool on;          // and whether there are any
+  bool seen, on;    // whether some row sees the key, and whether it has any
 
   __device__ __forceinline__ int page_of(const TreeParams& p, int t) const {
     return (int)((uint64_t)(uint32_t)t * p.page_magic >> p.page_shift);
@@ -455,11 +475,12 @@ struct TreeLookup {
   // scales' loads, and the entry for the tile at t1.
   __device__ __forceinline__ int row(const TreeParams& p, int t0, int t1) {
     const int t = t0 + (lane & (T - 1)), tc = clamp(t);
-    on = t < c1 && entry >= 0 && entry < p.pool_pages;
+    seen = t < c1;
     if (pick && t0 + T > len) {  // uniform over the wave
       const int jj = t - len;
-      if (t < c1 && jj >= 0) on = on && (wanted[jj >> 6] >> (jj & 63) & 1);
+      if (t < c1 && jj >= 0) seen = wanted[jj >> 6] >> (jj & 63) & 1;
     }
+    on = seen && entry >= 0 && entry < p.pool_pages;
     const int r = on ? entry * p.page + (tc - page_of(p, tc) * p.page) : 0;
     ask(p, t1);
     const int64_t at = (int64_t)r * p.kvh + kh;
@@ -473,12 +494,24 @@ struct TreeLookup {
   }
 };
 
-// Scales of a tile into the wave's LDS. The value scales are brought to at most
-// 2^6 by a power of two that falls as larger ones are met, so that probability x
-// scale keeps its 11 bits in FP16.
-template <int T>
+// Scales of a tile into the wave's LDS. Probability x value scale is an FP16 operand,
+// which has 11 bits from 2^-14 on and a step of 2^-24 below. The value scales are
+// brought to at most 2^6 by a power of two that falls as larger ones are met. While
+// none is below 2^-5 then, a row, whose largest probability is at least 1, keeps 11
+// bits of products down to 2^-9 of its largest, and the others to 2^-20 of that.
+// Scales further apart (one that a row does not see, or that hardly counts in it, would
+// take the others' bits: below some 2^-5 or past 2^3 to 2^6 times the largest of the chunk's
+// first keys), of 0, beyond 2^100 and unmapped pages make the chunk ``odd``.
+// It is begun anew with the scales as they are, and each row finds a factor of its own
+// from the products that it sees (tree_any_scales), so that products keep 11 bits down
+// to 2^-17 of its largest and the others to 2^-28 of that. With a maximum and a factor
+// for each 32 keys, that is slower: with scales of 0 in every chunk one token each over
+// 32 K tokens 51 us against 41, trees of 16 97 against 75, of 64 364 against 203.
+template <int T, bool kAny>
 struct TreeScales {
   float factor = 1.f, limit = -1.f;  // of the newest tile
+  float low = -1.f;                  // the smallest scale that is not odd
+  bool odd = false;
   // The key scales times ``unit`` 2^e.
   __device__ __forceinline__ void put(const TreeParams& p, const TreeLookup<T>& at, float* sc, float unit = 1.f,
                                       int e = 0) {
@@ -486,13 +519,19 @@ struct TreeScales {
       return at.on ? __builtin_bit_cast(float, p.scale_bf16 ? bits << 16 : bits) : 0.f;
     };
     const float k = value(at.rk), v = T == 32 ? k : value(at.rv);
-    const float a = (T == 64 || at.lane >= 32) && fabsf(v) < __builtin_inff() ? fabsf(v) : 0.f;
-    if (__any(a > limit)) {
-      const float x = tree_wave_reduce(a, [](float c, float d) { return fmaxf(c, d); });
-      int ve = (int)(__builtin_bit_cast(uint32_t, x) >> 23) - 127;
-      ve = ve < -124 ? -124 : ve;
-      factor = __builtin_bit_cast(float, (uint32_t)(127 + 3 - ve) << 23);  // 2^(3-ve): at most 2^4 now
-      limit = __builtin_bit_cast(float, (uint32_t)(127 + ve + 3 > 254 ? 254 : 127 + ve + 3) << 23);
+    if constexpr (!kAny) {
+      const bool mine = (T == 64 || at.lane >= 32) & at.seen;  // a value scale that counts
+      const float a = fabsf(v);
+      if (__any(mine & ((a > limit) | (a < low)))) {
+        const bool finite = a < __builtin_inff();
+        const float x = tree_wave_reduce(mine && finite ? a : 0.f, [](float c, float d) { return fmaxf(c, d); });
+        int ve = __builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, x) >> 23)) - 127;
+        ve = ve < -124 ? -124 : ve;
+        if (low < 0.f) low = ve < -121 ? 0x1p-126f : __builtin_bit_cast(float, (uint32_t)(127 + ve - 5) << 23);
+        factor = __builtin_bit_cast(float, (uint32_t)(127 + 3 - ve) << 23);  // 2^(3-ve): at most 2^4 now
+        limit = __builtin_bit_cast(float, (uint32_t)(127 + ve + 3 > 254 ? 254 : 127 + ve + 3) << 23);
+        odd = __any(mine & ((a < low) | !finite)) || limit > low * 0x1p11f || limit > 0x1p100f;
+      }
     }
     if (T == 32) {
       sc[at.lane] = at.lane < 32 ? __builtin_ldexpf(k * unit, e) : v * factor;
@@ -548,6 +587,54 @@ __device__ __forceinline__ void tree_level(TreeLevel& st, float* t, float top, f
     for (int v = 0; v < 16; ++v) t[v] -= by;
   }
 }
+
+// The same for scales of any size: the scores ``t`` (log2, -inf where not seen) become
+// probability x value scale x the row's factor, which brings the largest product so
+// far, ``most``, to between 2^3 and 2^4. vs(g): the scales of keys 4 g + [0, 4).
+template <typename V, typename F>
+__device__ __forceinline__ void tree_any_scales(TreeState& st, float& most, float* t, V&& vs, F&& fade) {
+  float top = t[0];
+#pragma unroll
+  for (int v = 1; v < 16; ++v) top = fmaxf(top, t[v]);
+  const float to = fmaxf(st.m, fmaxf(top, __shfl_xor(top, 32)));
+  const float f = __builtin_amdgcn_exp2f(st.m - to);
+  st.m = to;
+  st.l *= f;
+  float x = 0.f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 by = vs(g);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int v = 4 * g + u;
+      const bool on = t[v] != -__builtin_inff();
+      const float e = __builtin_amdgcn_exp2f(t[v] - to);
+      st.l += on ? e : 0.f;
+      t[v] = on ? e * by[u] : 0.f;
+      x = fmaxf(x, fabsf(t[v]));
+    }
+  }
+  most = fmaxf(most * f, fmaxf(x, __shfl_xor(x, 32)));
+  float factor = st.factor;
+  int up = 0;
+  if (most > 0.f) {
+    const int e = (int)(__builtin_bit_cast(uint32_t, most) >> 23);
+    factor = __builtin_bit_cast(float, (uint32_t)(257 - (e < 3 ? 3 : e)) << 23);
+    up = (int)(__builtin_bit_cast(uint32_t, factor) >> 23) - (int)(__builtin_bit_cast(uint32_t, st.factor) >> 23);
+  }
+  fade(__builtin_ldexpf(f, up < 126 ? up : 126));  // more only where nothing was summed up
+  st.factor = factor;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) t[v] *= factor;
+}
+
+// A score is sum x key scale x ``by``, of which the last two may leave the range of FP32
+// where the score does not: the part of ``by`` below 1 goes first.
+struct TreeBy {
+  float pre, post;
+  __device__ __forceinline__ explicit TreeBy(float by) : pre(by < 1.f ? by : 1.f), post(by < 1.f ? 1.f : by) {}
+  __device__ __forceinline__ float operator()(float sum, float scale) const { return sum * pre * scale * post; }
+};
 
 // The rows of a workgroup: which query, and the bits of its channels.
 template <int D>
@@ -644,20 +731,20 @@ __device__ __forceinline__ void tree_result(const TreeParams& p, const TreeItem&
 // byte permutation per two of them; the 128 is taken back at the end with the sum
 // of the rounded probabilities.
 // ---------------------------------------------------------------------------
-template <int D>
-__global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_kernel(TreeParams p) {
+template <int D, bool kAny>
+__device__ __forceinline__ bool tree_thin_pass(const TreeParams& p) {
   using C = TreeThin<D>;
   constexpr int KS = D / 32;  // channel blocks of 32
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   TreeItem it;
-  if (!tree_item<C::kRows, C::kStep>(p, it)) return;  // uniform over the workgroup
+  if (!tree_item<C::kRows, C::kStep>(p, it)) return true;  // uniform over the workgroup
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
   const TreeSeq seq = it.seq;
   int n, n_all;
   tree_reach(p, seq, it.tile, C::kRows, &n, &n_all);
   const int chunks = tree_chunks(n, it.keys);
-  if (it.chunk >= chunks) return;
+  if (it.chunk >= chunks) return true;
   const int span = tree_span(n, chunks, C::kStep), c0 = it.chunk * span;
   const int c1 = n - c0 < span ? n : c0 + span;
   const int turns = (c1 - c0 + C::kStep - 1) / C::kStep;
@@ -666,8 +753,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   float* scales = reinterpret_cast<float*>(smem + C::kRing + wave * C::kScale);
   uint64_t* wanted = reinterpret_cast<uint64_t*>(smem + C::kRing + 4 * C::kScale);
   TreeLookup<C::kTile> keys{p.table + (int64_t)it.b * p.pps, wanted, c1, seq.len, it.kh, lane,
-                            p.masks && c1 > seq.len, 0, 0, 0, false};
-  TreeScales<C::kTile> put;
+                            p.masks && c1 > seq.len, 0, 0, 0, false, false};
+  TreeScales<C::kTile, kAny> put;
   const auto tile_at = [&](int i) { return c0 + (wave + 4 * i) * C::kTile; };
   keys.ask(p, tile_at(0));
   TreeRow<D> row;
@@ -718,6 +805,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   }
   const float qf = row.bad ? __builtin_nanf("") : __builtin_ldexpf(p.to_log2, row.e - 14);
 
+  const TreeBy score(qf);
+
   f32x16 acc[KS];
 #pragma unroll
   for (int c = 0; c < KS; ++c)
@@ -725,6 +814,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
     for (int v = 0; v < 16; ++v) acc[c][v] = 0.f;
   TreeState st;
   float psum = 0.f;  // of the rounded probabilities times the value scales
+  float most = 0.f;  // see tree_any_scales
 
   const int krow = tree_row(col);
   const uint32_t koff = krow * D, ksw = tree_swizzle<D>(krow);
@@ -756,18 +846,23 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int v = 4 * g + u;
-        t[v] = (float)((hi[v] << 8) + lo[v]) * ksv[u];
+        const float sum = (float)((hi[v] << 8) + lo[v]);
+        t[v] = kAny ? score(sum, ksv[u]) : sum * ksv[u];
         if constexpr (slow) t[v] = vis >> (8 * g + u) & 1 ? t[v] : -__builtin_inff();
         top = fmaxf(top, t[v]);
       }
     }
-    tree_raise(st, top * qf, sc[64 - 4 * h], [&](float f) {
+    const auto fade = [&](float f) {
       psum *= f;
 #pragma unroll
       for (int c = 0; c < KS; ++c)
 #pragma unroll
         for (int v = 0; v < 16; ++v) acc[c][v] *= f;
-    });
+    };
+    if constexpr (kAny)
+      tree_any_scales(st, most, t, [&](int g) { return *reinterpret_cast<const f32x4*>(sc + 32 + 8 * g); }, fade);
+    else
+      tree_raise(st, top * qf, sc[64 - 4 * h], fade);
 #pragma unroll
     for (int mm = 0; mm < 2; ++mm) {  // 16 keys: 8 of each half wave
       // the lane's channels of its half wave's 8 keys; byte b of two keys makes one
@@ -794,6 +889,10 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
       for (int g = 0; g < 2; ++g) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
+          if constexpr (kAny) {
+            pv[4 * g + u] = (_Float16)t[8 * mm + 4 * g + u];
+            continue;
+          }
           const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(t[8 * mm + 4 * g + u], qf, -st.m));
           float w = e * vsv[g][u];
           if constexpr (slow) {
@@ -844,17 +943,22 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   int fast = open >= C::kTile ? (open / C::kTile - 1) / 4 + 1 : 0;
   fast = fast < turns ? fast : turns;
   int i = 0;
-  for (; i < fast; ++i) {
+  if constexpr (!kAny)
+    for (; i < fast; ++i) {
+      advance(i);
+      if (put.odd) break;
+      compute(std::false_type{}, 0, stage);
+      stage ^= 1;
+    }
+  for (; i < turns && !put.odd; ++i) {
     advance(i);
-    compute(std::false_type{}, 0, stage);
-    stage ^= 1;
-  }
-  for (; i < turns; ++i) {
-    advance(i);
+    if (put.odd) break;
     compute(std::true_type{}, tile_at(i), stage);
     stage ^= 1;
   }
   tree_landed();
+  int* odd = reinterpret_cast<int*>(smem + C::kLds - 16);  // of each wave
+  if (!kAny && lane == 0) odd[wave] = put.odd;
 
   // Both half waves hold half of a row's keys in l and psum.
   float l = st.l + __shfl_xor(st.l, 32), m = st.m;
@@ -866,6 +970,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
   float* stats = reinterpret_cast<float*>(smem + 4 * C::kRows * D * 4);  // [wave][row]: maximum, sum
   static_assert(4 * C::kRows * (D * 4 + 8) <= C::kLds, "merge");
   __syncthreads();
+  if constexpr (!kAny)
+    if (odd[0] | odd[1] | odd[2] | odd[3]) return false;
   if (h == 0) *reinterpret_cast<f32x2*>(stats + 2 * (wave * C::kRows + col)) = f32x2{m, l};
   __syncthreads();
   const auto joint = [&](int row, float* all) {
@@ -882,13 +988,13 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
     return to;
   };
   float all;
-  // 2^24 / factor leaves the range of FP32 where the sums do not: two steps
-  const float up = __builtin_amdgcn_exp2f(m - joint(col, &all)) * (1.f / st.factor);
+  // 2^24 / factor may leave the range of FP32 where the sums do not: two steps there
+  const float up = __builtin_amdgcn_exp2f(m - joint(col, &all)) * ((kAny ? 1.f : 0x1p24f) / st.factor);
   const float shift = 128.f * psum * 0x1p-24f;
   if (row.live)
     tree_runs<D>(acc, h, [&](int c, f32x4 v) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = (v[u] - shift) * 0x1p24f * up;
+      for (int u = 0; u < 4; ++u) v[u] = kAny ? (v[u] - shift) * 0x1p24f * up : (v[u] - shift) * up;
       return *reinterpret_cast<f32x4*>(sum + (wave * C::kRows + col) * D + 4 * ((c / 4) ^ (col & (D / 4 - 1)))) = v;
     });
   __syncthreads();
@@ -913,6 +1019,15 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
           u32x2{pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv)};
     }
   }
+  return true;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_kernel(TreeParams p) {
+  if (tree_left(tree_thin_pass<D, false>(p))) {
+    __syncthreads();  // all have read the flags
+    tree_thin_pass<D, true>(tree_again());
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -931,20 +1046,20 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
 // 247; at 64, two waves per SIMD, 294 against 293); addresses within the tile held in
 // registers (1 % faster at 128 channels, 4 % slower at 256).
 // ---------------------------------------------------------------------------
-template <int D>
-__global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_kernel(TreeParams p) {
+template <int D, bool kAny>
+__device__ __forceinline__ bool tree_wide_pass(const TreeParams& p) {
   using C = TreeWide<D>;
   constexpr int KS = D / 32, T = C::kTile;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   TreeItem it;
-  if (!tree_item<C::kRows, C::kStep>(p, it)) return;  // uniform over the workgroup
+  if (!tree_item<C::kRows, C::kStep>(p, it)) return true;  // uniform over the workgroup
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
   const TreeSeq seq = it.seq;
   int n, n_all;
   tree_reach(p, seq, it.tile, C::kRows, &n, &n_all);
   const int chunks = tree_chunks(n, it.keys);
-  if (it.chunk >= chunks) return;
+  if (it.chunk >= chunks) return true;
   const int span = tree_span(n, chunks, C::kStep), c0 = it.chunk * span;
   const int c1 = n - c0 < span ? n : c0 + span;
   const int turns = (c1 - c0 + T - 1) / T;
@@ -957,8 +1072,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   uint64_t* wanted = reinterpret_cast<uint64_t*>(vf + 2 * C::kHalf + 4 * C::kScale);
   uint8_t* ql = vf + 2 * C::kHalf + 4 * C::kScale + 32 + 1024 * C::kQueries * wave + 16 * lane;
   TreeLookup<T> keys{p.table + (int64_t)it.b * p.pps, wanted, c1, seq.len, it.kh, lane, p.masks && c1 > seq.len,
-                     0, 0, 0, false};
-  TreeScales<T> put;
+                     0, 0, 0, false, false};
+  TreeScales<T, kAny> put;  // the waves look at the same scales, and find the same ones odd
   const auto tile_at = [&](int i) { return c0 + i * T; };
   keys.ask(p, tile_at(0));
   TreeRow<D> row;
@@ -988,9 +1103,11 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   issue(0);
 
   row.scale();
-  // the largest of the wave's rows
-  const int e = __builtin_amdgcn_readfirstlane(
-      tree_wave_reduce(row.bad ? -110 : row.e, [](int a, int b) { return a > b ? a : b; }));
+  // the largest of the wave's rows; each row's own where scales are odd
+  const int e = kAny ? row.e
+                     : __builtin_amdgcn_readfirstlane(
+                           tree_wave_reduce(row.bad ? -110 : row.e, [](int a, int b) { return a > b ? a : b; }));
+  const TreeBy score(__builtin_ldexpf(1.f, e + 10));
   f16x8 q[KS][2];
   {
     const float up = row.bad ? __builtin_nanf("") : __builtin_ldexpf(1.f, 14 - e);
@@ -1015,7 +1132,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   for (int c = 0; c < KS; ++c)
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[c][v] = 0.f;
-  TreeLevel st;
+  std::conditional_t<kAny, TreeState, TreeLevel> st;
+  float most = 0.f;  // see tree_any_scales
 
   // The tile's codes into FP16: a key's 16 channels per thread and turn, then four
   // keys' D / 32 channels (of D = 64: 4). Code + 128 as a subnormal, less 128.
@@ -1100,17 +1218,22 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int v = 4 * g + u;
-          t[v] = __builtin_fmaf(s[v], ksv[u], -st.m);
+          t[v] = kAny ? score(s[v], ksv[u]) : __builtin_fmaf(s[v], ksv[u], -st.m);
           if constexpr (slow) t[v] = vis >> (8 * g + u) & 1 ? t[v] : -__builtin_inff();
           top = fmaxf(top, t[v]);
         }
       }
-      tree_level(st, t, top, sc[2 * T - 4 * h], [&](float f) {
+      const auto fade = [&](float f) {
 #pragma unroll
         for (int c = 0; c < KS; ++c)
 #pragma unroll
           for (int v = 0; v < 16; ++v) acc[c][v] *= f;
-      });
+      };
+      if constexpr (kAny)
+        tree_any_scales(st, most, t, [&](int g) { return *reinterpret_cast<const f32x4*>(sc + T + 32 * nb + 8 * g); },
+                        fade);
+      else
+        tree_level(st, t, top, sc[2 * T - 4 * h], fade);
       // Two operands of each sixteen keys' values are on their way before their
       // probabilities are formed, and nothing is moved across: left to itself the
       // scheduler read them one by one, each product waiting for LDS (64-token trees
@@ -1130,6 +1253,10 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
         for (int g = 0; g < 2; ++g) {
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
+            if constexpr (kAny) {
+              pv[4 * g + u] = (_Float16)t[8 * mm + 4 * g + u];
+              continue;
+            }
             const float y = __builtin_amdgcn_exp2f(t[8 * mm + 4 * g + u]);
             float w = y * vsv[g][u];
             if constexpr (slow) {
@@ -1155,7 +1282,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   const auto advance = [&](int i) {
     tree_priority<C::kPerCu>(place + i);
     tree_landed();
-    put.put(p, keys, scales, p.to_log2, e + 10);
+    put.put(p, keys, scales, p.to_log2, kAny ? 0 : e + 10);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     convert();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -1164,24 +1291,38 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_k
   const int open = (n_all < c1 ? n_all : c1) - c0;
   const int fast = open >= T ? (open / T < turns ? open / T : turns) : 0;
   int i = 0;
-  for (; i < fast; ++i) {
+  if constexpr (!kAny)
+    for (; i < fast; ++i) {
+      advance(i);
+      if (put.odd) break;
+      if (rows) compute(std::false_type{}, 0);
+    }
+  for (; i < turns && !put.odd; ++i) {
     advance(i);
-    if (rows) compute(std::false_type{}, 0);
-  }
-  for (; i < turns; ++i) {
-    advance(i);
+    if (put.odd) break;
     if (rows) compute(std::true_type{}, tile_at(i));
   }
   tree_landed();
-  const float l = st.l + __shfl_xor(st.l, 32), up = 1.f / st.factor;
+  if (put.odd) return false;
+  const float l = st.l + __shfl_xor(st.l, 32), up = (kAny ? 1.f : 0x1p24f) / st.factor;
 #pragma unroll
   for (int c = 0; c < KS; ++c)
 #pragma unroll
-    for (int v = 0; v < 16; ++v) acc[c][v] = acc[c][v] * 0x1p24f * up;  // two steps: 2^24 / factor may overflow
+    for (int v = 0; v < 16; ++v) acc[c][v] = kAny ? acc[c][v] * 0x1p24f * up : acc[c][v] * up;  // as in the thin kernel
   const int at = which();
+  float m = st.m;
+  if constexpr (!kAny) m = st.limit < 0.f ? kTreeFloor : m;
   if (at < seq.count * p.r)
-    tree_result<D>(p, it, acc, chunks > 1, st.limit < 0.f ? kTreeFloor : st.m, l, at / p.r, at % p.r,
-                   (int64_t)it.place * C::kRows + wave * 32 + col, h);
+    tree_result<D>(p, it, acc, chunks > 1, m, l, at / p.r, at % p.r, (int64_t)it.place * C::kRows + wave * 32 + col, h);
+  return true;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kTreeThreads, TreeWide<D>::kPerCu) tree_wide_kernel(TreeParams p) {
+  if (tree_left(tree_wide_pass<D, false>(p))) {
+    __syncthreads();  // all are done with the masks
+    tree_wide_pass<D, true>(tree_again());
+  }
 }
 
 // The chunks' sums of a row and head joined in chunk order, D / 4 lanes of four

@@ -194,3 +194,74 @@ def test_attention_values_near_the_ends_of_fp32(device, dim, r, room, power):
     case = _case(36, [90, 3], [8, 5], 16, 1, r, dim, qscale=0.5, room=room)
     case[3][:] = (case[3] * np.float32(2.0**power) if power < 0 else np.float32(2.0**power) * (case[3] / case[3].max()))
     _hold(_attn(device, case, None), _exact(case, None))
+
+
+def _near(rng, case, spread=0.05):
+    """Queries of all rows and heads near one direction, which is returned."""
+    q = case[9]
+    base = rng.standard_normal(q.shape[2]).astype(np.float32) * 2
+    q[:] = bf16_round((base + spread * rng.standard_normal(q.shape)).astype(np.float32))
+    return base
+
+
+@DIMS
+@FEW_AND_MANY
+@pytest.mark.parametrize("power", [16, 20, 28, 60, 100])
+@pytest.mark.parametrize("kind", ["tree", "chain"])
+def test_attention_large_values_of_a_token_that_others_do_not_see(device, dim, r, room, power, kind):
+    # new token 3's values are 2^power times the others'; rows that may not see it are as exact as without it
+    counts = [8, 8]
+    case = _case(31, [500, 40], counts, 16, 1, r, dim, room=room)
+    vs, table, lengths = case[3], case[4], case[5]
+    for b, n in enumerate(lengths):
+        vs[table[b, (n + 3) // 16], (n + 3) % 16] *= np.float32(2.0**power)
+    sees = None if kind == "chain" else [s - {3} if i % 8 != 3 else s for i, s in
+                                         enumerate(_sees(np.random.default_rng(5), counts, 0))]
+    _hold(_attn(device, case, sees), _exact(case, sees))
+
+
+@DIMS
+@FEW_AND_MANY
+def test_attention_values_that_hardly_count(device, dim, r, room):
+    # cached tokens of large values whose probability is some 2^-150, met first, last and in the middle
+    case = _case(32, [700], [8], 64, 1, r, dim, room=room)
+    base = _near(np.random.default_rng(6), case)
+    k, ks, v, vs, table = case[:5]
+    for t, power in ((0, 24), (350, 30), (690, 34)):
+        at = table[0, t // 64], t % 64
+        k[at] = np.where(base > 0, -127, 127)
+        ks[at] *= 3
+        vs[at] *= np.float32(2.0**power)
+    _hold(_attn(device, case, None), _exact(case, None))
+
+
+@DIMS
+@FEW_AND_MANY
+@pytest.mark.parametrize("what", ["zero", "small", "unmapped"])
+def test_attention_first_token_without_values(device, dim, r, room, what):
+    # a first token (or page) that takes nearly all of the probability and has no value, or a small one: what
+    # is left of the others, 2^-20 and less, is the output
+    case = _case(33, [400], [8], 16, 1, r, dim, room=room)
+    base = _near(np.random.default_rng(7), case)
+    k, ks, v, vs, table = case[:5]
+    if what == "unmapped":  # its keys are zero; all others' scores are near -16 log2(e)
+        k[:] = np.clip(np.rint(k * 0.1 - base * (16 * dim**0.5 / (base @ base) / ks.mean())), -127, 127)
+        table[0, 0] = -1
+    else:
+        at = table[0, 0], 0
+        k[at] = np.clip(np.rint(base * (22 * dim**0.5 / (base @ base)) / ks[at][0]), -127, 127)
+        vs[at] = 0 if what == "zero" else vs[at] * np.float32(2.0**-30)
+    _hold(_attn(device, case, None), _exact(case, None))
+
+
+@DIMS
+@FEW_AND_MANY
+@pytest.mark.parametrize("power", [-0.2, -0.03, 0.03, 0.2])
+def test_attention_values_that_grow_or_fade(device, dim, r, room, power):
+    # value scales that go up or down by 2^180 in all
+    case = _case(34, [880, 300], [8, 5], 16, 1, r, dim, qscale=0.5, room=room)
+    vs, table, lengths = case[3], case[4], case[5]
+    for b, n in enumerate(lengths):
+        t = np.arange(n + 8)
+        vs[table[b, t // 16], t % 16] *= np.exp2(power * (t - t.mean()))[:, None].astype(np.float32)
+    _hold(_attn(device, case, None), _exact(case, None))
