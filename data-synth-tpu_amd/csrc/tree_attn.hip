@@ -105,8 +105,8 @@ struct TreeWide {
   // registers some spilled, and their reload waited for the DMA just issued: 8 x
   // 64-token trees over 32 K tokens 261 us against 236.)
   static constexpr int kQueries = D == 256 ? 2 : 0;
-  // a tile's codes, the same in FP16, scales, masks, queries
-  static constexpr int kLds = 2 * kHalf + 4 * kHalf + 4 * kScale + 32 + 4096 * kQueries;
+  // a tile's codes, the same in FP16, scales, masks, queries, four flags
+  static constexpr int kLds = 2 * kHalf + 4 * kHalf + 4 * kScale + 32 + 4096 * kQueries + 16;
   static_assert(kPerCu * kLds <= 160 * 1024, "tile");
 };
 
@@ -544,8 +544,13 @@ struct TreeScales {
 };
 
 // A row's softmax so far: maximum (log2), sum over the lane's keys, value factor.
+// A score less its maximum is formed by one FMA, of a maximum that is rounded. Beyond 2^13
+// (kTreeHuge) half a step of that is more than the 2^-11 by which a probability is
+// rounded, and from 2^27 on one could overflow: such maxima, too, make the chunk odd.
+constexpr float kTreeHuge = 0x1p13f;
 struct TreeState {
   float m = kTreeFloor, l = 0.f, factor = 1.f;
+  bool huge = false;  // of some row of the wave
 };
 
 // The maximum of 32 keys' scores, ``top``, and their value factor, taken into the
@@ -558,6 +563,7 @@ __device__ __forceinline__ void tree_raise(TreeState& st, float top, float facto
     const float to = fmaxf(st.m, fmaxf(top, __shfl_xor(top, 32)));
     const float f = __builtin_amdgcn_exp2f(st.m - to);
     fade(f * (factor / st.factor));
+    st.huge |= __any((fabsf(to) > kTreeHuge) & (to != kTreeFloor));
     st.factor = factor;
     st.m = to;
     st.l *= f;
@@ -569,6 +575,7 @@ __device__ __forceinline__ void tree_raise(TreeState& st, float top, float facto
 struct TreeLevel {
   float m = 0.f, l = 0.f, factor = 1.f;
   float limit = -3.4028235e38f;  // kTreeSlack once m is set
+  bool huge = false;
 };
 template <typename F>
 __device__ __forceinline__ void tree_level(TreeLevel& st, float* t, float top, float factor, F&& fade) {
@@ -579,6 +586,7 @@ __device__ __forceinline__ void tree_level(TreeLevel& st, float* t, float top, f
     const float to = on ? st.m + both : st.m, by = on ? to - st.m : 0.f;
     const float f = st.limit < 0.f ? 1.f : __builtin_amdgcn_exp2f(-by);
     fade(f * (factor / st.factor));
+    st.huge |= __any(fabsf(to) > kTreeHuge);
     st.factor = factor;
     st.m = to;
     st.l *= f;
@@ -958,7 +966,7 @@ __device__ __forceinline__ bool tree_thin_pass(const TreeParams& p) {
   }
   tree_landed();
   int* odd = reinterpret_cast<int*>(smem + C::kLds - 16);  // of each wave
-  if (!kAny && lane == 0) odd[wave] = put.odd;
+  if (!kAny && lane == 0) odd[wave] = put.odd || st.huge;
 
   // Both half waves hold half of a row's keys in l and psum.
   float l = st.l + __shfl_xor(st.l, 32), m = st.m;
@@ -1304,6 +1312,12 @@ __device__ __forceinline__ bool tree_wide_pass(const TreeParams& p) {
   }
   tree_landed();
   if (put.odd) return false;
+  if constexpr (!kAny) {
+    int* again = reinterpret_cast<int*>(smem + C::kLds - 16);  // of each wave
+    if (lane == 0) again[wave] = st.huge;
+    __syncthreads();
+    if (again[0] | again[1] | again[2] | again[3]) return false;
+  }
   const float l = st.l + __shfl_xor(st.l, 32), up = (kAny ? 1.f : 0x1p24f) / st.factor;
 #pragma unroll
   for (int c = 0; c < KS; ++c)

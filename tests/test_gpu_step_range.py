@@ -265,3 +265,25 @@ def test_attention_values_that_grow_or_fade(device, dim, r, room, power):
         t = np.arange(n + 8)
         vs[table[b, t // 16], t % 16] *= np.exp2(power * (t - t.mean()))[:, None].astype(np.float32)
     _hold(_attn(device, case, None), _exact(case, None))
+
+
+@DIMS
+@FEW_AND_MANY
+@pytest.mark.parametrize("power", [9, 13, 16, 20, 28, 60, 100])
+def test_attention_equal_keys_of_large_scores(device, dim, r, room, power):
+    # scores of some 2^(power + 4) and more; four equal keys of different tiles lie 2^(power + 3) above all others, so
+    # that a row is the mean of their values
+    case = _case(39, [300, 295], [8, 6], 16, 1, r, dim, room=room)
+    base = _near(np.random.default_rng(8), case)
+    k, ks, v, vs, table, _, starts = case[:7]
+    places = 5, 100, 200, 290
+    for t in places:
+        for b in range(2):
+            at = table[b, t // 16], t % 16
+            k[at], ks[at] = np.clip(np.rint(base * 30), -127, 127), 0.02
+    case[9][:] *= np.float32(2.0**power)
+    got = _attn(device, case, None)
+    for b in range(2):
+        at = table[b, np.array(places) // 16], np.array(places) % 16
+        want = (v[at].astype(np.float64) * vs[at].astype(np.float64)[..., None]).mean((0, 1))
+        _hold(got[starts[b]:starts[b + 1]], np.broadcast_to(want, got[starts[b]:starts[b + 1]].shape))
