@@ -22,8 +22,9 @@
 // rounding; the rounding to fewer bits that there is: a probability times its value
 // scale to the 11 bits of FP16, the second product's operand (an eighth of the BF16
 // output's half step; for products far below the row's largest see TreeScales), and
-// query values that are more than 2^6 below their row's largest (few rows) or 2^28
-// below that of 32 rows (many). Maxima, sums and all accumulators are FP32.
+// query values that are more than 2^6 below their row's largest (few rows) or 2^12 (many).
+// Maxima, sums and all accumulators are FP32, and so are scores, which have to be in its
+// range: a row with one past it is NaN, and it alone.
 #include <atomic>
 #include <type_traits>
 
@@ -1044,10 +1045,13 @@ __global__ void __launch_bounds__(kTreeThreads, TreeThin<D>::kPerCu) tree_thin_k
 // are FP16 too, scaled by a power of two that the wave's rows share, so that it and 1
 // / sqrt(D) go into the keys' scales and one FMA gives a score less its row's maximum
 // (221 us against 228 for 64-token trees over 32 K tokens): exact for values down to
-// 2^-28 of the largest of the 32 rows, below that off by 2^-39 of it. (A chunk of 1024
-// tokens over 8 K, 256-wide heads: 300 us in the kernel for few rows, 235 here; with
-// three workgroups per CU in place of two at 128 channels, 64-token trees over 32 K
-// 238 and 220.) With 128 channels, 64 keys cost a wave some 350 vector instructions
+// 2^-28 of the largest of the 32 rows, below that off by 2^-39 of it. Rows that lie
+// further apart than 2^16 take the pass for odd scales, where each has its own power, so
+// that a row's values are exact down to 2^-12 of its largest at least, and the others
+// off by 2^-23 of that. (A chunk of 1024 tokens over 8 K, 256-wide heads: 300 us in the
+// kernel for few rows, 235 here; with three workgroups per CU in place of two at 128
+// channels, 64-token trees over 32 K 238 and 220.)
+// With 128 channels, 64 keys cost a wave some 350 vector instructions
 // and 32 MFMAs, 1024 cycles of the matrix cores; a vector instruction issues in 61 %
 // of a SIMD's cycles and the matrix cores work in 33 %. Measured and left: 64 rows per wave,
 // which share the operands from LDS (registers spill at 128 channels: 347 us against
@@ -1116,6 +1120,10 @@ __device__ __forceinline__ bool tree_wide_pass(const TreeParams& p) {
                      : __builtin_amdgcn_readfirstlane(
                            tree_wave_reduce(row.bad ? -110 : row.e, [](int a, int b) { return a > b ? a : b; }));
   const TreeBy score(__builtin_ldexpf(1.f, e + 10));
+  // Rows whose largest is below 2^-16 of that lose bits, and scores of queries past 2^60 may
+  // leave the range of FP32 on the way: then each row by itself (rows of zeros, and of
+  // 2^-110 and less, whose scores are as good as 0, do not count).
+  const bool far = !kAny && (__any(!row.bad & (row.e > -110) & (e - row.e > 16)) || e > 60);
   f16x8 q[KS][2];
   {
     const float up = row.bad ? __builtin_nanf("") : __builtin_ldexpf(1.f, 14 - e);
@@ -1314,7 +1322,7 @@ __device__ __forceinline__ bool tree_wide_pass(const TreeParams& p) {
   if (put.odd) return false;
   if constexpr (!kAny) {
     int* again = reinterpret_cast<int*>(smem + C::kLds - 16);  // of each wave
-    if (lane == 0) again[wave] = st.huge;
+    if (lane == 0) again[wave] = far || st.huge;
     __syncthreads();
     if (again[0] | again[1] | again[2] | again[3]) return false;
   }

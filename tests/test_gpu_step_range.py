@@ -287,3 +287,24 @@ def test_attention_equal_keys_of_large_scores(device, dim, r, room, power):
         at = table[b, np.array(places) // 16], np.array(places) % 16
         want = (v[at].astype(np.float64) * vs[at].astype(np.float64)[..., None]).mean((0, 1))
         _hold(got[starts[b]:starts[b + 1]], np.broadcast_to(want, got[starts[b]:starts[b + 1]].shape))
+
+
+@DIMS
+@FEW_AND_MANY
+@pytest.mark.parametrize("power", [17, 28, 32, 40, 90, 126])
+@pytest.mark.parametrize("what", ["row", "head"])
+def test_attention_query_beside_a_larger_one(device, dim, r, room, power, what):
+    # one token's queries, or one head's, are 2^power times the others': these keep their scores
+    case = _case(35, [300, 77], [8, 6], 16, 1, r, dim, room=room)
+    q = case[9]
+    large = q[5] if what == "row" else q[2, 1]
+    large *= np.float32(2.0**power if power < 126 else 2.0**126 / np.abs(large).max())
+    bad = 5 if what == "row" else 2
+    got, want = _attn(device, case, None), _exact(case, None)
+    _hold(got, want, [i for i in range(len(q)) if i != bad])
+    if power < 126:  # at 2^126 its scores leave the range of FP32
+        _hold(got, want)
+    else:
+        others = [g for g in range(q.shape[1]) if g != 1]
+        if what == "head":
+            _hold(got[:, others], want[:, others])
