@@ -502,7 +502,8 @@ struct TreeLookup {
 // bits of products down to 2^-9 of its largest, and the others to 2^-20 of that.
 // Scales further apart (one that a row does not see, or that hardly counts in it, would
 // take the others' bits: below some 2^-5 or past 2^3 to 2^6 times the largest of the chunk's
-// first keys), of 0, beyond 2^100 and unmapped pages make the chunk ``odd``.
+// first keys), of 0, beyond 2^100 and unmapped pages make the chunk ``odd``, and so do key
+// scales beyond 2^20, of which a score could leave the range of FP32 on the way.
 // It is begun anew with the scales as they are, and each row finds a factor of its own
 // from the products that it sees (tree_any_scales), so that products keep 11 bits down
 // to 2^-17 of its largest and the others to 2^-28 of that. With a maximum and a factor
@@ -521,9 +522,13 @@ struct TreeScales {
     };
     const float k = value(at.rk), v = T == 32 ? k : value(at.rv);
     if constexpr (!kAny) {
-      const bool mine = (T == 64 || at.lane >= 32) & at.seen;  // a value scale that counts
-      const float a = fabsf(v);
-      if (__any(mine & ((a > limit) | (a < low)))) {
+      // of 32 keys a lane holds a key scale or a value scale
+      const bool keys = T == 32 && at.lane < 32;
+      const float a = fabsf(v), most = keys ? 0x1p20f : limit, least = keys ? -1.f : low;
+      bool out = (a > most) | (a < least);
+      if (T == 64) out |= fabsf(k) > 0x1p20f;
+      if (__any(out & at.seen)) {
+        const bool mine = !keys & at.seen, far = (T == 64 || keys) & at.seen & (fabsf(k) > 0x1p20f);
         const bool finite = a < __builtin_inff();
         const float x = tree_wave_reduce(mine && finite ? a : 0.f, [](float c, float d) { return fmaxf(c, d); });
         int ve = __builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, x) >> 23)) - 127;
@@ -531,7 +536,7 @@ struct TreeScales {
         if (low < 0.f) low = ve < -121 ? 0x1p-126f : __builtin_bit_cast(float, (uint32_t)(127 + ve - 5) << 23);
         factor = __builtin_bit_cast(float, (uint32_t)(127 + 3 - ve) << 23);  // 2^(3-ve): at most 2^4 now
         limit = __builtin_bit_cast(float, (uint32_t)(127 + ve + 3 > 254 ? 254 : 127 + ve + 3) << 23);
-        odd = __any(mine & ((a < low) | !finite)) || limit > low * 0x1p11f || limit > 0x1p100f;
+        odd = __any((mine & ((a < low) | !finite)) | far) || limit > low * 0x1p11f || limit > 0x1p100f;
       }
     }
     if (T == 32) {
@@ -637,11 +642,12 @@ __device__ __forceinline__ void tree_any_scales(TreeState& st, float& most, floa
   for (int v = 0; v < 16; ++v) t[v] *= factor;
 }
 
-// A score is sum x key scale x ``by``, of which the last two may leave the range of FP32
-// where the score does not: the part of ``by`` below 1 goes first.
+// A score is sum x key scale x unit 2^e, of which the last two may leave the range of
+// FP32 where the score does not: a 2^e below 1 goes first.
 struct TreeBy {
   float pre, post;
-  __device__ __forceinline__ explicit TreeBy(float by) : pre(by < 1.f ? by : 1.f), post(by < 1.f ? 1.f : by) {}
+  __device__ __forceinline__ TreeBy(float unit, int e)
+      : pre(__builtin_ldexpf(1.f, e < 0 ? e : 0)), post(__builtin_ldexpf(unit, e < 0 ? 0 : e)) {}
   __device__ __forceinline__ float operator()(float sum, float scale) const { return sum * pre * scale * post; }
 };
 
@@ -684,7 +690,7 @@ struct TreeRow {
     bad = top >= 0x7f80u;
     // the largest stays below 127 * 256 + 128 in steps of 2^(e-14)
     e = (int)(top >> 7) - 127 + ((top & 0x7f) == 0x7f);
-    e = e < -110 ? -110 : e;  // smaller queries lose bits: scores below 2^-90
+    e = e < -112 ? -112 : e;  // smaller queries lose bits: what is left is off by 2^-127 at most
   }
   __device__ __forceinline__ float value(int s, int i, int k) const {  // k of 8
     const uint32_t x = raw[s][i][k >> 1];
@@ -814,7 +820,7 @@ __device__ __forceinline__ bool tree_thin_pass(const TreeParams& p) {
   }
   const float qf = row.bad ? __builtin_nanf("") : __builtin_ldexpf(p.to_log2, row.e - 14);
 
-  const TreeBy score(qf);
+  const TreeBy score(row.bad ? __builtin_nanf("") : p.to_log2, row.e - 14);
 
   f32x16 acc[KS];
 #pragma unroll
@@ -1118,12 +1124,13 @@ __device__ __forceinline__ bool tree_wide_pass(const TreeParams& p) {
   // the largest of the wave's rows; each row's own where scales are odd
   const int e = kAny ? row.e
                      : __builtin_amdgcn_readfirstlane(
-                           tree_wave_reduce(row.bad ? -110 : row.e, [](int a, int b) { return a > b ? a : b; }));
-  const TreeBy score(__builtin_ldexpf(1.f, e + 10));
+                           tree_wave_reduce(row.bad ? -112 : row.e, [](int a, int b) { return a > b ? a : b; }));
+  const TreeBy score(1.f, e + 10);
   // Rows whose largest is below 2^-16 of that lose bits, and scores of queries past 2^60 may
   // leave the range of FP32 on the way: then each row by itself (rows of zeros, and of
-  // 2^-110 and less, whose scores are as good as 0, do not count).
-  const bool far = !kAny && (__any(!row.bad & (row.e > -110) & (e - row.e > 16)) || e > 60);
+  // 2^-112 and less, whose scores are as good as 0 with key scales that are not odd, do
+  // not count).
+  const bool far = !kAny && (__any(!row.bad & (row.e > -112) & (e - row.e > 16)) || e > 60);
   f16x8 q[KS][2];
   {
     const float up = row.bad ? __builtin_nanf("") : __builtin_ldexpf(1.f, 14 - e);

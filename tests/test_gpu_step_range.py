@@ -308,3 +308,16 @@ def test_attention_query_beside_a_larger_one(device, dim, r, room, power, what):
         others = [g for g in range(q.shape[1]) if g != 1]
         if what == "head":
             _hold(got[:, others], want[:, others])
+
+
+@DIMS
+@FEW_AND_MANY
+@pytest.mark.parametrize("power", [60, 92, 100, 110])
+def test_attention_small_queries_of_large_keys(device, dim, r, room, power):
+    # key scales of 2^power, queries of 2^-power: ordinary scores
+    case = _case(37, [200, 31], [8, 5], 16, 1, r, dim, room=room)
+    k, ks, v, vs, table, lengths, starts, page, kvh, q, most = case
+    small = bf16_round(q * np.float32(2.0**-power))
+    ks = (ks * np.float32(2.0**power)).astype(np.float32)
+    case = (k, ks, v, vs, table, lengths, starts, page, kvh, small, most)
+    _hold(_attn(device, case, None), _exact(case, None))
