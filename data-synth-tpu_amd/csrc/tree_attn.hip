@@ -258,11 +258,13 @@ __device__ __forceinline__ int tree_keys(const TreeParams& p, S&& sum) {
   const float total = sum(0.f, [&](const TreeSeq& s) { return (float)units(s) * (float)s.n; });
   const int tiles = sum(0, units);
   const bool once = 2 * tiles <= p.slots;
-  int lo = (int)(total / (float)(once ? p.slots : 2 * p.slots) * (1.f / STEP));
-  lo = lo < 1 ? 1 : (lo < (1 << 30) / STEP / 2 - 1 ? lo : (1 << 30) / STEP / 2 - 1);
+  constexpr int kMost = (1 << 30) / STEP - 1;  // with one more a chunk holds any sequence
+  const float share = total / (float)(once ? p.slots : 2 * p.slots) * (1.f / STEP);
+  int lo = share < (float)kMost ? (int)share : kMost;
+  lo = lo < 1 ? 1 : lo;
   // in steps; hi gives few enough chunks: each tile has at most one that is not full
   const float sure = total / (float)(p.slots - tiles) * (1.00001f / STEP);
-  int hi = once ? (sure < (float)(1 << 30) / STEP - 1.f ? (int)sure : (1 << 30) / STEP - 1) + 1 : lo + 1;
+  int hi = once ? (sure < (float)kMost ? (int)sure : kMost) + 1 : lo + 1;
   // few tiles: hi is within an eighth of the least
   if (once && 8 * tiles > p.slots)
     for (int i = 0; i < 5 && lo < hi; ++i) {
