@@ -16,7 +16,7 @@
 // one for many, bound by the vector ALU that turns scores into probabilities beside
 // the matrix cores. 8 sequences of 8 K to 32 K tokens, 4 KV heads of 128 channels, 8
 // query heads each: one token each 47 us (the cache at 4.5 TB/s but for 10 us before
-// the first and after the last keys), trees of 16 69 us, of 64 200 us (630 TFLOP/s).
+// the first and after the last keys), trees of 16 70 us, of 64 201 us (628 TFLOP/s).
 //
 // Scores are exact sums of FP32-scaled products of the stored codes but for the FP32
 // rounding; the rounding to fewer bits that there is: a probability times its value
@@ -1513,7 +1513,9 @@ static TreeLayout tree_layout(int64_t batch, int64_t rows, int64_t max_count, in
   // over 32 K (2^36) 87 and 90, 4 x 64 over 32 K (2^37) 184 and 145; 64 rows per head
   // over 32 K 48 and 60, 96 rows 61 and 70. With D = 64, 8 KV heads, 1 x 64 over 8000
   // 31 and 40, 4 x 16 over 32 K (2^35) 66 and 58; with D = 256, 2 KV heads, 4 x 16
-  // over 32 K (2^35) 64 and 72, 4 x 32 (2^36) 110 and 96.
+  // over 32 K (2^35) 64 and 72, 4 x 32 (2^36) 110 and 96. Short contexts under a wide
+  // table pay for it: in one of 128 K tokens 4 x 16 over 1000 21.3 us against 16.9 in a
+  // table of their own width, 4 x 32 over 8000 45.4 and 34.2.
   const int64_t thin = TreeThin<128>::kRows;
   L.wide = max_count * r > 3 * thin &&
            (2 * tiles(thin) > slots(false) || (double)rows * hq * cap * dim * 4. > (dim == 64 ? 0x1p35 : 0x1p36));

@@ -197,8 +197,8 @@ def write_tokens(k_pool, k_scales, v_pool, v_scales, key, value, slots, *, kv_he
     ``slots`` int64 [rows] as ``plan_pages`` gives them; rows outside the pool (-1)
     are skipped, the others must be distinct. Pools int8 [pages, page_size, ...],
     scales [pages, page_size, kv_heads * head_dim / group] (group: head_dim by
-    default); K's and V's must not overlap. Codes and scales are those of
-    ``write_paged`` bit for bit.
+    default; ``paged_tree_attention`` reads caches of one scale per head); K's and
+    V's must not overlap. Codes and scales are those of ``write_paged`` bit for bit.
     """
     _positive(kv_heads=kv_heads, head_dim=head_dim)
     group = head_dim if group is None else group
@@ -252,7 +252,12 @@ def paged_tree_attention(q, k_pool, k_scales, v_pool, v_scales, page_table, leng
     masks at most 64 * words).
 
     Returns BF16 [rows, Hq, D]: softmax(q . k / sqrt(D)) . v with k and v the
-    unrounded code * scale, rounded once. A row that sees nothing gives 0. Rows
+    unrounded code * scale, rounded once. Scores and sums are FP32 (a row with a
+    score past its range is NaN); a probability times its value scale has 11 bits
+    where it is 2^-9 of the row's largest or more, else it is off by up to 2^-20
+    of that. A page table far wider than the contexts can cost a fifth to a half
+    more time (128 K tokens over 500 to 8000): kernels are chosen by its width.
+    A row that sees nothing gives 0. Rows
     behind the last sequence, and of a sequence those from ``max_count`` on, are
     left as they were in ``out``; without ``out`` they are 0 (one launch more, for
     the fill). Unmapped pages read as zero keys and values.

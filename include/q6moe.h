@@ -453,7 +453,11 @@ int q6moe_kv_write_rows(const q6moe_kv_write_rows_args* args, void* stream);
  * last sequence, and of a sequence those from max_count on, are left as they were in out.
  * head_dim 64, 128 or 256; one scale per token and KV head; pool_pages * page_size below 2^31,
  * pages_per_seq * page_size at most 2^30, rows and max_count below 2^24, rows * query_heads / kv_heads
- * below 2^30. Which kernel runs follows from the sizes alone, never from lengths.
+ * below 2^30. Which kernel runs follows from the sizes alone, never from lengths: a page table
+ * far wider than the contexts (128 K tokens over 500 to 8000) can cost a fifth to a half more.
+ * Scores, maxima and sums are FP32: a row with a score past its range is NaN. A probability times
+ * its value scale has 11 bits where it is 2^-9 of the row's largest or more, else it is off by up
+ * to 2^-20 of that.
  */
 typedef struct q6moe_tree_attn_args {
   const uint16_t* q;         /* BF16 [rows, Hq, D], row r at q + r * q_stride */
