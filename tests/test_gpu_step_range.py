@@ -14,7 +14,7 @@ import torch
 
 from oracle import step as oracle
 from oracle.packed_q6 import bf16_round
-from q6moe import plan_pages, write_tokens
+from q6moe import paged_tree_attention, plan_pages, write_tokens
 
 from .test_gpu_step import FEW_AND_MANY, _attn, _cache, _case, _dev, _sees
 
@@ -321,3 +321,67 @@ def test_attention_small_queries_of_large_keys(device, dim, r, room, power):
     ks = (ks * np.float32(2.0**power)).astype(np.float32)
     case = (k, ks, v, vs, table, lengths, starts, page, kvh, small, most)
     _hold(_attn(device, case, None), _exact(case, None))
+
+
+@FEW_AND_MANY
+@pytest.mark.parametrize("dim,scales", [(64, torch.float32), (128, torch.bfloat16), (256, torch.float32)])
+@pytest.mark.parametrize("batch", [5, 70])
+def test_attention_odd_scales_masks_and_empty_rows(device, dim, scales, batch, r, room):
+    # value scales of 0, and some 2^+-30 times the others, in a part of the sequences; any masks, rows that see
+    # nothing, unmapped pages; NaN and infinite scales where nobody looks and a NaN that one row sees
+    rng = np.random.default_rng(batch + dim)
+    lengths = np.where(rng.random(batch) < 0.3, 0, rng.integers(0, 300, batch))
+    counts = rng.integers(0, 9, batch)
+    lengths, counts = [40, *lengths[1:].tolist()], [8, *counts[1:].tolist()]
+    case = _case(40, lengths, counts, 16, 2, r, dim, room=room)
+    k, ks, v, vs, table, _, starts = case[:7]
+    sees = [s - {2} if rng.random() < 0.8 else set() for s in _sees(rng, counts, 0, 0.4)]
+    sees[1] |= {2}  # sequence 0's row 1 alone sees its token 2
+    held = np.zeros(ks.shape[:2], bool)
+    for b, (n, c) in enumerate(zip(lengths, counts)):
+        used = set().union(*sees[starts[b]:starts[b + 1]]) if c else set()
+        t = np.array(list(range(n)) + [n + j for j in used], int)
+        held[table[b, t // 16], t % 16] = True
+        if b % 2 and len(t):
+            at = t[rng.random(len(t)) < 0.2]
+            vs[table[b, at // 16], at % 16] *= np.float32(2.0) ** rng.choice([-np.inf, -30, 30], (len(at), 1))
+        if b % 5 == 3 and n > 32:
+            table[b, 1] = -1 if b % 2 else k.shape[0] + 7
+    ks[~held], vs[~held] = np.nan, np.inf
+    case = (k, bf16_round(ks), v, bf16_round(vs), *case[4:]) if scales == torch.bfloat16 else case
+    at = table[0, 42 // 16], 42 % 16
+    case[3][at] = np.nan
+    got = _attn(device, case, sees, scales_dtype=scales)
+    assert np.isnan(got[1]).all()
+    # what nobody sees is 0 to the oracle, whose products with weights of 0 are not NaN then
+    clean = tuple(np.where(np.isfinite(x), x, 0).astype(np.float32) for x in (case[1], case[3]))
+    want = _exact((case[0], clean[0], case[2], clean[1], *case[4:]), sees)
+    none = np.array([not s and not lengths[b] for b in range(batch) for s in sees[starts[b]:starts[b + 1]]])
+    assert (got[:len(none)][none] == 0).all()
+    _hold(got, want, [i for i in range(len(got)) if i != 1])
+
+
+@FEW_AND_MANY
+def test_attention_replayed_with_odd_scales(device, r, room):
+    # one graph, whose value scales become odd and ordinary again between the replays
+    k, ks, v, vs, table, lengths, starts, page, kvh, q, most = _case(41, [900, 70, 333], [8, 5, 8], 64, 2, r, 128,
+                                                                    room=room)
+    pools = [_dev(k.reshape(*k.shape[:2], -1), device), _dev(ks, device), _dev(v.reshape(*v.shape[:2], -1), device),
+             _dev(vs, device)]
+    state = [_dev(np.asarray(t, np.int32), device) for t in (table, lengths, starts)]
+    x, out = _dev(q, device, torch.bfloat16), torch.zeros(q.shape, dtype=torch.bfloat16, device=device)
+    work = torch.empty(1 << 27, dtype=torch.uint8, device=device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged_tree_attention(x, *pools, *state, page_size=page, kv_heads=kvh, max_count=most, out=out, workspace=work)
+    for odd in (False, True, False, True):
+        changed = vs.copy()
+        if odd:
+            changed[table[0, :10:3], 7] *= np.float32(2.0**40)
+            changed[table[2, 1], 30:40] = 0
+        pools[3].copy_(_dev(changed, device))
+        out.fill_(5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        case = (k, ks, v, changed, table, lengths, starts, page, kvh, q, most)
+        _hold(out.float().cpu().numpy(), _exact(case, None))
