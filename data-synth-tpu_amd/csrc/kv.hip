@@ -441,6 +441,14 @@ extern "C" int q6moe_kv_write_rows(const q6moe_kv_write_rows_args* a, void* stre
   Q6MOE_REQUIRE(a->key_stride >= 0 && a->value_stride >= 0, "kv_write_rows: negative row stride");
   Q6MOE_REQUIRE(a->x_dtype == Q6MOE_BF16 || a->x_dtype == Q6MOE_F32, "kv_write_rows: x dtype");
   Q6MOE_REQUIRE(a->scale_dtype == Q6MOE_BF16 || a->scale_dtype == Q6MOE_F32, "kv_write_rows: scale dtype");
+  const auto apart = [](const void* x, const void* y, int64_t bytes) {
+    const uintptr_t u = reinterpret_cast<uintptr_t>(x), v = reinterpret_cast<uintptr_t>(y);
+    return (u < v ? v - u : u - v) >= (uintptr_t)bytes;
+  };
+  Q6MOE_REQUIRE(apart(a->k_codes, a->v_codes, a->pool_rows * chans) &&
+                    apart(a->k_scales, a->v_scales,
+                          a->pool_rows * (chans / a->group) * (a->scale_dtype == Q6MOE_BF16 ? 2 : 4)),
+                "kv_write_rows: the K and V pools must not overlap");
   KvRows w{{a->key, a->value}, {a->key_stride, a->value_stride}, {a->k_codes, a->v_codes},
            {a->k_scales, a->v_scales}, a->slots, a->rows, a->pool_rows};
   KvQuant q{a->key, a->x_dtype == Q6MOE_BF16, chans, a->group, chans / a->group, a->scale_dtype == Q6MOE_BF16, 0};

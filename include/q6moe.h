@@ -425,7 +425,7 @@ int q6moe_kv_release(int32_t* page_table, const int32_t* lengths, int32_t* free_
 /*
  * Keys and values of a ragged batch quantised into their slots (codes and scales as
  * q6moe_kv_quantize), K and V in one call. Rows whose slot is outside [0, pool_rows) are
- * not written. The slots that are written must be distinct.
+ * not written. The slots that are written must be distinct, and K's pools apart from V's.
  */
 typedef struct q6moe_kv_write_rows_args {
   const void* key;           /* [rows, KVH*D], row r at key + r * key_stride values */

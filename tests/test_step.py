@@ -72,6 +72,15 @@ def test_write_refusals(over, text):
     _refused(_lib.load().q6moe_kv_write_rows, _filled(_lib.KvWriteRowsArgs, **over), text)
 
 
+@pytest.mark.parametrize("k,v,ks,vs", [(0, 0, 0, 4096), (0, 639, 0, 4096), (639, 0, 0, 4096), (0, 4096, 0, 36),
+                                       (0, 4096, 36, 0)])
+def test_write_refuses_pools_that_overlap(k, v, ks, vs):
+    # 10 rows of 64 codes and an FP32 scale
+    a = _filled(_lib.KvWriteRowsArgs, pool_rows=10, head_dim=64, group=64, scale_dtype=_lib.F32, k_codes=FAKE + k,
+                v_codes=FAKE + v, k_scales=FAKE + ks, v_scales=FAKE + vs)
+    _refused(_lib.load().q6moe_kv_write_rows, a, "must not overlap")
+
+
 @pytest.mark.parametrize("over,text", [
     (dict(q=None), "null pointer"), (dict(starts=None), "null pointer"), (dict(head_dim=96), "64, 128 or 256"),
     (dict(query_heads=3, kv_heads=2), "multiple of kv_heads"), (dict(batch=0), "at most 65535"),
